@@ -231,6 +231,142 @@ int mononn_attention_noalloc(const void* q, const void* k, const void* v_t, cons
  * (mononn_engine/core/gpu/synchronization.cc:45-97). */
 int mononn_attention_noalloc_status(void* cuda_stream);
 
+/* Operators behind a prompt: positions by rotation, a key/value cache of pages, attention of new
+ * tokens over it (no counterpart in the reference, whose decoder graphs end with the prompt). They
+ * work on caller-owned device memory, allocate nothing, launch on `cuda_stream` without waiting for it
+ * and may be captured into a CUDA graph; pointers and sizes are those of the call, what indptr,
+ * lengths, page_table and positions hold is read on the device at each launch. Every call runs on the device that owns
+ * its first buffer (a stream of another device is refused) and restores the caller's current device.
+ * dtype: MONONN_F16 or MONONN_BF16 for every tensor of a call; sums, softmax and rotations are
+ * computed in 32 bits (angles in 64). Strides count elements. */
+enum { MONONN_F16 = 0, MONONN_BF16 = 1 };
+
+/* How the turning rates of a rotary embedding follow from its configuration. Pair i of r / 2 turns
+ * by f_i = theta^(-2i/r) radians a position, and with a longer context of `factor` times the
+ * `original_length` by
+ *   LINEAR  f_i / factor
+ *   BASE    the same with theta * factor^(r/(r-2)) instead of theta
+ *   RAMP    a blend that goes from f_i to f_i / factor over the pair's index, between the pairs that
+ *           make `high` and `low` turns within original_length (defaults 32 and 1); values are
+ *           multiplied by 0.1 ln(factor) + 1
+ *   BANDS   the same blend over the number of turns itself, from f_i at `high` (default 4) or more
+ *           to f_i / factor at `low` (default 1) or fewer. */
+enum {
+  MONONN_ROTARY_PLAIN = 0,
+  MONONN_ROTARY_LINEAR = 1,
+  MONONN_ROTARY_BASE = 2,
+  MONONN_ROTARY_RAMP = 3,
+  MONONN_ROTARY_BANDS = 4
+};
+#define MONONN_MAX_ROTARY_PAIRS 128
+typedef struct {
+  unsigned rotary_dim;    /* leading elements of a head that are rotated: even, 2 .. 256 */
+  int interleaved;        /* pairs (2i, 2i+1); 0: pairs (i, i + rotary_dim/2) */
+  int scaling;            /* MONONN_ROTARY_* */
+  double theta;           /* 0 = 10000 */
+  double factor;          /* of the scalings, > 0 */
+  double original_length; /* RAMP and BANDS: positions the model was trained on */
+  double low, high;       /* RAMP and BANDS: 0 = the defaults above */
+  double magnitude;       /* what rotated values are multiplied by; 0 = 1, RAMP: 0.1 ln(factor) + 1
+                             (1 for a factor of 1 or less) */
+} mononn_rotary_config;
+/* What the kernels read, a plain value owned by the caller: made once by mononn_rotary_init, or filled by hand. */
+typedef struct {
+  unsigned rotary_dim;
+  int interleaved;
+  double magnitude;
+  double turns[MONONN_MAX_ROTARY_PAIRS]; /* f_i / 2 pi */
+} mononn_rotary;
+int mononn_rotary_init(const mononn_rotary_config* config, mononn_rotary* out);
+
+/* out[t, h, :] = x[t, h, :] with its leading rotary_dim elements rotated by positions[t] (any int32);
+ * the rest is copied. `out` may be `x` itself (same strides); other overlaps are not allowed.
+ * head_dim up to 256. Without alignment to 16 bytes (addresses, strides, and 8 | head_dim; rotary_dim a
+ * multiple of 16, interleaved of 8) a slower form of the kernel runs, element by element. */
+typedef struct {
+  const void* x;
+  void* out;
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+  const int32_t* positions; /* [tokens] */
+  unsigned tokens, heads, head_dim;
+  int dtype;
+} mononn_rotary_args;
+int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* args, void* cuda_stream);
+
+/* A cache of keys and values in pages of page_size tokens. Element (token row r, head h, d) of page p is at
+ * p * page_stride + r * token_stride + h * head_stride + d in k_pages and v_pages alike, so pages may be
+ * token-major or head-major. Sequence b's keys 0 .. lengths[b]-1 are in the pages page_table[b *
+ * table_stride + key / page_size]; a length beyond max_pages * page_size counts as that. Sequences may
+ * share pages. A page number outside of 0 .. num_pages-1 is never followed: its tokens are not
+ * written, and read as zeros. New tokens are packed: sequence b has the rows indptr[b] .. indptr[b+1]-1 of
+ * the token tensors (indptr: [sequences + 1], not decreasing), and they are its LAST positions:
+ * row indptr[b] + i is at position lengths[b] - (indptr[b+1] - indptr[b]) + i, so `lengths` counts them.
+ * Rows outside of every sequence (behind indptr[sequences]) are left as they were. */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int64_t page_stride, token_stride, head_stride;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  unsigned sequences, max_pages, num_pages, page_size, kv_heads, head_dim;
+  int dtype;
+} mononn_paged_cache;
+
+/* Writes the new tokens' keys and values into their pages, the keys rotated by their position on
+ * the way (rotary NULL: as they are), and rotates the queries of the same tokens in the same launch
+ * (q NULL: none; q_out may be q itself). positions: what is rotated by instead of the position in
+ * the cache, or NULL. A token without a place (a negative position, a page number out of range) is not
+ * written; its query is rotated all the same. Two tokens that fall on one place of a
+ * shared page leave one of the two there. Alignment as mononn_rotary_apply. */
+typedef struct {
+  const void *k, *v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const void* q;
+  void* q_out;
+  int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+  const int32_t* indptr;
+  const int32_t* positions;
+  unsigned tokens, q_heads; /* rows of the token tensors */
+} mononn_paged_append_args;
+int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* rotary,
+                        const mononn_paged_append_args* args, void* cuda_stream);
+
+/* out[t, h, :] = sum_j p_j v_j,  p = softmax over the visible keys j of scale * q[t, h] . k_j,
+ * where head h reads key head h / (q_heads / kv_heads). A token at position p sees the keys j <= p
+ * (causal; otherwise all of its sequence), and with window > 0 (causal only) of those the ones with
+ * j > p - window. A row that sees nothing becomes zeros (lse: minus infinity). lse: natural
+ * logarithm of the sum of the exponentials, f32 [tokens, q_heads], or NULL. Keys that no row sees and
+ * page rows behind a length may hold anything, NaN too.
+ * max_new: at most how many new tokens a sequence has, as a hint that chooses between the kernel for
+ * few rows (single tokens, drafts) and the one for many; 0 = unknown. Results are right whatever it says.
+ * Limits: head_dim a multiple of 8 up to 128; page_size a multiple of 8; q_heads / kv_heads whole;
+ * addresses of pages, q and out, and all their strides, multiples of 16 bytes (lse, indptr: 4). */
+typedef struct {
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  const int32_t* indptr;
+  unsigned tokens, q_heads;
+  float scale; /* > 0; 0 = 1 / sqrt(head_dim) */
+  int causal;
+  unsigned window;
+  unsigned max_new;
+  void* workspace; /* of mononn_paged_attention_workspace bytes, 16-byte aligned; needs no initial
+                      state; calls that overlap on the GPU need one each */
+  size_t workspace_bytes;
+} mononn_paged_attention_args;
+int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
+                           void* cuda_stream);
+/* Bytes for calls with this cache and these arguments (0: none), whatever the device arrays hold. */
+int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
+                                     size_t* bytes);
+/* Waits for `cuda_stream`, then reports and clears the status word that the attention kernels of its
+ * device share: MONONN_OK, or MONONN_ERR_BARRIER_TIMEOUT when a bounded wait expired in one of them
+ * since the last report (its output is incomplete). */
+int mononn_paged_attention_status(void* cuda_stream);
+
 void mononn_destroy(mononn_module* m);
 const char* mononn_strerror(int code);
 /* Message of the last failing call on this thread. */

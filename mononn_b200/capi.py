@@ -19,6 +19,8 @@ EXPORTS = [
     "mononn_destroy", "mononn_strerror", "mononn_last_error", "mononn_enabled",
     "mononn_trace_stages", "mononn_plan_json", "mononn_describe", "mononn_free_string", "mononn_launch_stages", "mononn_debug_skew_barrier", "mononn_attention_noalloc",
     "mononn_infer_host", "mononn_debug_mma_issue", "mononn_attention_noalloc_status",
+    "mononn_rotary_init", "mononn_rotary_apply", "mononn_paged_append", "mononn_paged_attention",
+    "mononn_paged_attention_workspace", "mononn_paged_attention_status",
 ]
 
 
@@ -31,6 +33,47 @@ class Options(C.Structure):
 class ArgDesc(C.Structure):
     _fields_ = [("index", C.c_int), ("bytes", C.c_size_t), ("kind", C.c_int),
                 ("param_number", C.c_int)]
+
+
+class RotaryConfigArgs(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint), ("interleaved", C.c_int), ("scaling", C.c_int)] + [
+        (n, C.c_double) for n in ("theta", "factor", "original_length", "low", "high", "magnitude")]
+
+
+class RotaryTable(C.Structure):
+    _fields_ = [("rotary_dim", C.c_uint), ("interleaved", C.c_int), ("magnitude", C.c_double),
+                ("turns", C.c_double * 128)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("x_token_stride", C.c_int64),
+                ("x_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("positions", C.c_void_p), ("tokens", C.c_uint), ("heads", C.c_uint), ("head_dim", C.c_uint),
+                ("dtype", C.c_int)]
+
+
+class PagedCacheArgs(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("page_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("lengths", C.c_void_p), ("sequences", C.c_uint),
+                ("max_pages", C.c_uint), ("num_pages", C.c_uint), ("page_size", C.c_uint), ("kv_heads", C.c_uint),
+                ("head_dim", C.c_uint), ("dtype", C.c_int)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")] + [
+        ("q", C.c_void_p), ("q_out", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "q_out_token_stride", "q_out_head_stride")] + [
+        ("indptr", C.c_void_p), ("positions", C.c_void_p), ("tokens", C.c_uint), ("q_heads", C.c_uint)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p)] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + [
+        ("indptr", C.c_void_p), ("tokens", C.c_uint), ("q_heads", C.c_uint), ("scale", C.c_float),
+        ("causal", C.c_int), ("window", C.c_uint), ("max_new", C.c_uint), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t)]
 
 
 class MononnError(RuntimeError):
@@ -78,6 +121,14 @@ def lib() -> C.CDLL:
         l.mononn_attention_noalloc.argtypes = [vp, vp, vp, vp, vp, C.c_uint, C.c_uint, C.c_uint, C.c_uint,
                                                C.c_uint, C.c_uint, C.c_float, C.c_float, C.c_int, vp]
         l.mononn_attention_noalloc_status.argtypes = [vp]
+        l.mononn_rotary_init.argtypes = [C.POINTER(RotaryConfigArgs), C.POINTER(RotaryTable)]
+        l.mononn_rotary_apply.argtypes = [C.POINTER(RotaryTable), C.POINTER(RotaryArgs), vp]
+        l.mononn_paged_append.argtypes = [C.POINTER(PagedCacheArgs), C.POINTER(RotaryTable),
+                                          C.POINTER(PagedAppendArgs), vp]
+        l.mononn_paged_attention.argtypes = [C.POINTER(PagedCacheArgs), C.POINTER(PagedAttentionArgs), vp]
+        l.mononn_paged_attention_workspace.argtypes = [C.POINTER(PagedCacheArgs), C.POINTER(PagedAttentionArgs),
+                                                       C.POINTER(C.c_size_t)]
+        l.mononn_paged_attention_status.argtypes = [vp]
         dp = C.POINTER(C.c_double)
         l.mononn_debug_mma_issue.argtypes = [C.c_int, C.c_uint, C.c_uint, C.c_uint, C.c_uint, C.c_uint, dp, dp, dp]
         l.mononn_destroy.argtypes = [vp]

@@ -1,0 +1,472 @@
+// C entry points of the operators behind a prompt (declared in include/mononn.h): checks of arguments,
+// tensor maps, the division into kernels and workspaces. No device memory is read or allocated here.
+#include "paged.h"
+
+#include <climits>
+#include <cmath>
+#include <mutex>
+#include <numeric>
+#include <string>
+
+#include "../../include/mononn.h"
+#include "runtime.h"
+
+using namespace mononn;
+
+namespace {
+
+int fail(int code, const std::string& msg) {
+  set_last_error(msg);
+  return code;
+}
+int invalid(const std::string& msg) { return fail(MONONN_ERR_INVALID_ARGUMENT, msg); }
+
+#define PG_TRY(expr)                                                                     \
+  do {                                                                                   \
+    cudaError_t e__ = (expr);                                                            \
+    if (e__ != cudaSuccess)                                                              \
+      return fail(MONONN_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e__)); \
+  } while (0)
+
+// A launch on a stream of another device than the kernel's ends in this error (the stream itself cannot be
+// asked for its device while it is captured).
+int launched(cudaError_t e) {
+  if (e == cudaSuccess) return MONONN_OK;
+  cudaGetLastError();
+  if (e == cudaErrorInvalidResourceHandle)
+    return invalid("the stream belongs to another device than the buffers, or to none");
+  return fail(MONONN_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+constexpr int kMaxDevices = 64;
+struct Device {
+  bool ready = false;
+  int sm_count = 0;
+  uint32_t* status = nullptr;
+};
+Device g_devices[kMaxDevices];
+std::mutex g_mutex;
+EncodeTiledFn g_encode = nullptr;
+
+// One-time set-up of the current device.
+int set_up(int dev, const Device** out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  Device& d = g_devices[dev];
+  if (!d.ready) {
+    int major = 0;
+    PG_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+    if (major != 10) return fail(MONONN_ERR_NO_DEVICE, "the kernels are built for sm_100a only");
+    PG_TRY(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev));
+    PG_TRY(paged_status_word(&d.status));
+    PG_TRY(prepare_few_rows());
+    if (!g_encode) {
+      cudaDriverEntryPointQueryResult q;
+      void* fn = nullptr;
+      PG_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+      if (q != cudaDriverEntryPointSuccess || !fn)
+        return fail(MONONN_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+      g_encode = reinterpret_cast<EncodeTiledFn>(fn);
+    }
+    d.ready = true;
+  }
+  *out = &d;
+  return MONONN_OK;
+}
+
+// The device of a call is the one that owns its first buffer; the caller's current one comes back at the end.
+class OnDeviceOf {
+ public:
+  ~OnDeviceOf() {
+    if (previous_ >= 0) cudaSetDevice(previous_);
+  }
+  int enter(const void* buffer, const Device** out) {
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+      cudaGetLastError();
+      return fail(MONONN_ERR_NO_DEVICE, "no CUDA device");
+    }
+    cudaPointerAttributes a;
+    PG_TRY(cudaPointerGetAttributes(&a, buffer));
+    if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
+      return invalid("buffers have to be in device memory");
+    if (a.device < 0 || a.device >= kMaxDevices) return invalid("device ordinal out of range");
+    int current = 0;
+    PG_TRY(cudaGetDevice(&current));
+    if (current != a.device) {
+      PG_TRY(cudaSetDevice(a.device));
+      previous_ = current;
+    }
+    return set_up(a.device, out);
+  }
+
+ private:
+  int previous_ = -1;
+};
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+bool whole8(int64_t stride) { return (stride & 7) == 0; }
+
+// Strides that no tensor of this size can have are refused, so that the kernels' 64-bit offsets never wrap.
+bool stride_in_range(int64_t s) { return s >= 0 && s < (1ll << 39); }
+
+int check_dtype(int dtype) {
+  if (dtype != MONONN_F16 && dtype != MONONN_BF16)
+    return fail(MONONN_ERR_UNSUPPORTED, "dtype must be MONONN_F16 or MONONN_BF16");
+  return MONONN_OK;
+}
+int check_rotary(const mononn_rotary& r, unsigned head_dim) {
+  if (r.rotary_dim == 0 || (r.rotary_dim & 1u) || r.rotary_dim > 2 * MONONN_MAX_ROTARY_PAIRS || r.rotary_dim > head_dim)
+    return invalid("rotary_dim must be even, at least 2 and at most head_dim");
+  if (!std::isfinite(r.magnitude)) return invalid("rotary magnitude must be finite");
+  for (unsigned i = 0; i < r.rotary_dim / 2; ++i)
+    if (!std::isfinite(r.turns[i])) return invalid("rotary rates must be finite");
+  return MONONN_OK;
+}
+int check_cache(const mononn_paged_cache& c) {
+  if (!c.k_pages || !c.v_pages || !c.page_table || !c.lengths) return invalid("cache: null pointer");
+  if (int rc = check_dtype(c.dtype)) return rc;
+  if (c.page_size == 0 || c.kv_heads == 0 || c.head_dim == 0 || c.max_pages == 0 || c.num_pages == 0)
+    return invalid("cache: a size is zero");
+  if (c.num_pages > INT_MAX || c.kv_heads > 65536 || c.head_dim > 256 || c.sequences > (1u << 24))
+    return fail(MONONN_ERR_TOO_LARGE, "cache: num_pages < 2^31, kv_heads <= 65536, head_dim <= 256, sequences <= 2^24");
+  if (static_cast<uint64_t>(c.max_pages) * c.page_size > (1u << 30))
+    return fail(MONONN_ERR_TOO_LARGE, "cache: max_pages * page_size exceeds 2^30 keys");
+  if (!stride_in_range(c.page_stride) || !stride_in_range(c.token_stride) || !stride_in_range(c.head_stride) ||
+      c.table_stride < c.max_pages || !stride_in_range(c.table_stride))
+    return invalid("cache: strides must be in 0 .. 2^39, table_stride at least max_pages");
+  if (!aligned(c.page_table, 4) || !aligned(c.lengths, 4) || !aligned(c.k_pages, 2) || !aligned(c.v_pages, 2))
+    return invalid("cache: misaligned pointer");
+  // no two elements in one place: what is written would depend on an order
+  const int64_t d = c.head_dim;
+  if ((c.page_size > 1 && c.token_stride < d) || (c.kv_heads > 1 && c.head_stride < d) ||
+      (c.num_pages > 1 && c.page_stride < d))
+    return invalid("cache: strides are smaller than the heads they hold");
+  return MONONN_OK;
+}
+
+// Elements of 16-byte vectors are read and written whole where everything is aligned to them.
+bool rows_by_vectors(const RowsParams& p) {
+  bool ok = p.head_dim % 8 == 0 && p.rotary_dim % (p.interleaved ? 8 : 16) == 0 && whole8(p.page_stride);
+  for (const RowsSource* s : {&p.q, &p.k, &p.v})
+    if (s->heads)
+      ok = ok && aligned(s->src, 16) && aligned(s->dst, 16) && whole8(s->src_token) && whole8(s->src_head) &&
+           whole8(s->dst_token) && whole8(s->dst_head);
+  return ok;
+}
+void set_rotation(RowsParams* p, const mononn_rotary& r) {
+  p->rotary_dim = r.rotary_dim;
+  p->interleaved = r.interleaved != 0;
+  p->magnitude = static_cast<float>(r.magnitude);
+  for (unsigned i = 0; i < r.rotary_dim / 2; ++i) p->turns[i] = r.turns[i];
+}
+
+// Elements are 16 bits wide. One box is 64 elements of a head x `box` rows of one page; elements behind
+// head_dim, rows and pages out of range arrive as zeros.
+int encode_pages(CUtensorMap* map, const mononn_paged_cache& c, const void* base, uint32_t box, const char* what) {
+  const cuuint64_t dims[4] = {c.head_dim, c.page_size, c.kv_heads, c.num_pages};
+  // the stride of a dimension of one element is never used, but has to be valid
+  auto stride = [&](int64_t s, unsigned n) { return static_cast<cuuint64_t>(n > 1 ? s : (c.head_dim + 7) / 8 * 8) * 2; };
+  const cuuint64_t strides[3] = {stride(c.token_stride, c.page_size), stride(c.head_stride, c.kv_heads),
+                                 stride(c.page_stride, c.num_pages)};
+  const cuuint32_t boxes[4] = {64, box, 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUresult r = g_encode(map, c.dtype == MONONN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              4, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MONONN_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed (CUresult " +
+                                     std::to_string(static_cast<int>(r)) + ")");
+  return MONONN_OK;
+}
+
+int check_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* a) {
+  if (!cache || !a) return invalid("null argument");
+  if (int rc = check_cache(*cache)) return rc;
+  const mononn_paged_cache& c = *cache;
+  if (c.head_dim % 8 || c.head_dim > 128)
+    return fail(MONONN_ERR_UNSUPPORTED, "attention: head_dim must be a multiple of 8 up to 128");
+  if (c.page_size % 8) return fail(MONONN_ERR_UNSUPPORTED, "attention: page_size must be a multiple of 8");
+  if (!a->q || !a->out || !a->indptr) return invalid("attention: null pointer");
+  if (a->q_heads == 0 || a->q_heads % c.kv_heads) return invalid("attention: q_heads must be a multiple of kv_heads");
+  if (a->q_heads > 65536 || static_cast<uint64_t>(a->tokens) * (a->q_heads / c.kv_heads) > INT_MAX)
+    return fail(MONONN_ERR_TOO_LARGE, "attention: q_heads <= 65536, tokens * q_heads / kv_heads < 2^31");
+  if (!stride_in_range(a->q_token_stride) || !stride_in_range(a->q_head_stride) ||
+      !stride_in_range(a->out_token_stride) || !stride_in_range(a->out_head_stride))
+    return invalid("attention: strides must be in 0 .. 2^39");
+  const int64_t d = c.head_dim;
+  if ((a->q_heads > 1 && a->out_head_stride < d) || (a->tokens > 1 && a->out_token_stride < d))
+    return invalid("attention: strides of out are smaller than the heads they hold");
+  if (!aligned(c.k_pages, 16) || !aligned(c.v_pages, 16) || !whole8(c.page_stride) || !whole8(c.token_stride) ||
+      !whole8(c.head_stride) || !aligned(a->q, 16) || !whole8(a->q_token_stride) || !whole8(a->q_head_stride) ||
+      !aligned(a->out, 16) || !whole8(a->out_token_stride) || !whole8(a->out_head_stride))
+    return invalid("attention: addresses and strides of pages, q and out must be multiples of 16 bytes");
+  if (!aligned(a->lse, 4) || !aligned(a->indptr, 4)) return invalid("attention: lse and indptr must be 4-byte aligned");
+  if (!std::isfinite(a->scale) || a->scale < 0.f) return invalid("attention: scale must be positive and finite, or 0");
+  if (a->window && !a->causal) return invalid("attention: a window needs causal attention");
+  return MONONN_OK;
+}
+
+// How many CTAs, and whether an item may span them. Only sizes count that the host knows.
+constexpr uint32_t kFewWholeTiles = 8;  // caches of at most so many tiles: no item is split
+constexpr uint32_t kFewLeastUnits = 4;  // of a CTA's share
+void plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
+  const uint32_t group = a.q_heads / c.kv_heads;
+  const uint64_t capacity = static_cast<uint64_t>(c.max_pages) * c.page_size;
+  p->padded_dim = c.head_dim <= 64 ? 64 : 128;
+  p->rows = kFewRows;
+  p->keys = kFewKeys;
+  p->box = std::gcd(c.page_size, p->keys);
+  // items: at most a row tile for each `rows` rows, and a ragged one for each sequence
+  const uint64_t tiles = (capacity + p->keys - 1) / p->keys;
+  const uint64_t most_rows = static_cast<uint64_t>(a.tokens) * group;
+  const uint64_t items =
+      (most_rows / p->rows + std::min<uint64_t>(c.sequences, a.tokens)) * c.kv_heads;
+  const bool whole = tiles <= kFewWholeTiles;
+  const uint64_t wanted = whole ? items : (items * tiles + kFewLeastUnits - 1) / kFewLeastUnits;
+  p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(wanted, 2u * static_cast<unsigned>(sm_count))));
+  p->joins = !whole && p->ctas > 1;
+  p->workspace = 0;
+  if (p->joins) {
+    const size_t headers = (p->ctas * sizeof(AttentionHeader) + 255) / 256 * 256;
+    p->workspace = headers + 2 * static_cast<size_t>(p->ctas) * attention_slot_floats(*p) * sizeof(float);
+  }
+}
+}  // namespace
+
+extern "C" {
+
+int mononn_rotary_init(const mononn_rotary_config* config, mononn_rotary* out) {
+  if (!config || !out) return invalid("null argument");
+  const mononn_rotary_config& c = *config;
+  const unsigned r = c.rotary_dim;
+  if (r == 0 || (r & 1u) || r > 2 * MONONN_MAX_ROTARY_PAIRS) return invalid("rotary_dim must be even, 2 .. 256");
+  if (c.scaling < MONONN_ROTARY_PLAIN || c.scaling > MONONN_ROTARY_BANDS) return invalid("unknown rotary scaling");
+  double theta = c.theta == 0.0 ? 10000.0 : c.theta;
+  if (!(theta > 1.0) || !std::isfinite(theta)) return invalid("rotary theta must be finite and above 1");
+  const double s = c.scaling == MONONN_ROTARY_PLAIN ? 1.0 : c.factor;
+  if (!(s > 0.0) || !std::isfinite(s)) return invalid("rotary factor must be positive and finite");
+  const bool blended = c.scaling == MONONN_ROTARY_RAMP || c.scaling == MONONN_ROTARY_BANDS;
+  const double low = c.low == 0.0 ? 1.0 : c.low;
+  const double high = c.high == 0.0 ? (c.scaling == MONONN_ROTARY_RAMP ? 32.0 : 4.0) : c.high;
+  if (blended && !(c.original_length > 0.0 && std::isfinite(c.original_length)))
+    return invalid("rotary original_length must be positive and finite");
+  if (blended && !(low > 0.0 && high > low && std::isfinite(high))) return invalid("rotary turns: 0 < low < high");
+  if (!std::isfinite(c.magnitude) || c.magnitude < 0.0) return invalid("rotary magnitude must be finite and not negative");
+  const double two_pi = 6.283185307179586476925286766559;
+  if (c.scaling == MONONN_ROTARY_BASE && r > 2) theta *= std::pow(s, static_cast<double>(r) / (r - 2.0));
+  double first = 0.0, last = 0.0;
+  if (c.scaling == MONONN_ROTARY_RAMP) {
+    auto pair = [&](double turns) {
+      return r * std::log(c.original_length / (turns * two_pi)) / (2.0 * std::log(theta));
+    };
+    first = std::max(0.0, std::floor(pair(high)));
+    last = std::min(r - 1.0, std::ceil(pair(low)));
+  }
+  mononn_rotary made{};
+  made.rotary_dim = r;
+  made.interleaved = c.interleaved != 0;
+  made.magnitude = c.magnitude != 0.0 ? c.magnitude
+                   : c.scaling == MONONN_ROTARY_RAMP && s > 1.0 ? 0.1 * std::log(s) + 1.0 : 1.0;
+  for (unsigned i = 0; i < r / 2; ++i) {
+    double f = std::pow(theta, -2.0 * i / r);
+    auto blend = [&](double slow) { f = (1.0 - slow) * f + slow * f / s; };
+    auto clamp = [](double x) { return std::min(1.0, std::max(0.0, x)); };
+    if (c.scaling == MONONN_ROTARY_LINEAR) f /= s;
+    if (c.scaling == MONONN_ROTARY_RAMP) blend(clamp((i - first) / std::max(last - first, 0.001)));
+    if (c.scaling == MONONN_ROTARY_BANDS) blend(1.0 - clamp((c.original_length * f / two_pi - low) / (high - low)));
+    made.turns[i] = f / two_pi;
+  }
+  *out = made;
+  return MONONN_OK;
+}
+
+int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* args, void* cuda_stream) {
+  if (!rotary || !args) return invalid("null argument");
+  const mononn_rotary_args& a = *args;
+  if (int rc = check_dtype(a.dtype)) return rc;
+  if (a.head_dim == 0 || a.head_dim > 256 || a.heads > 65536)
+    return fail(MONONN_ERR_TOO_LARGE, "rotary: head_dim in 1 .. 256, heads <= 65536");
+  if (int rc = check_rotary(*rotary, a.head_dim)) return rc;
+  if (!stride_in_range(a.x_token_stride) || !stride_in_range(a.x_head_stride) ||
+      !stride_in_range(a.out_token_stride) || !stride_in_range(a.out_head_stride))
+    return invalid("rotary: strides must be in 0 .. 2^39");
+  if (a.tokens > INT_MAX) return fail(MONONN_ERR_TOO_LARGE, "rotary: tokens < 2^31");
+  if (a.tokens == 0 || a.heads == 0) return MONONN_OK;
+  if (!a.x || !a.out || !a.positions) return invalid("rotary: null pointer");
+  if (!aligned(a.x, 2) || !aligned(a.out, 2) || !aligned(a.positions, 4)) return invalid("rotary: misaligned pointer");
+  const int64_t d = a.head_dim;
+  if ((a.heads > 1 && a.out_head_stride < d) || (a.tokens > 1 && a.out_token_stride < d))
+    return invalid("rotary: strides of out are smaller than the heads they hold");
+  if (a.x == a.out && (a.x_token_stride != a.out_token_stride || a.x_head_stride != a.out_head_stride))
+    return invalid("rotary: in place, x and out have the same strides");
+  OnDeviceOf guard;
+  const Device* dev = nullptr;
+  if (int rc = guard.enter(a.out, &dev)) return rc;
+  RowsParams p{};
+  p.q = RowsSource{a.x, a.out, a.x_token_stride, a.x_head_stride, a.out_token_stride, a.out_head_stride, a.heads};
+  p.positions = a.positions;
+  p.tokens = a.tokens;
+  p.head_dim = a.head_dim;
+  set_rotation(&p, *rotary);
+  return launched(launch_rows(p, a.dtype == MONONN_BF16, rows_by_vectors(p), dev->sm_count,
+                              static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* rotary,
+                        const mononn_paged_append_args* args, void* cuda_stream) {
+  if (!cache || !args) return invalid("null argument");
+  if (int rc = check_cache(*cache)) return rc;
+  const mononn_paged_cache& c = *cache;
+  const mononn_paged_append_args& a = *args;
+  if (rotary)
+    if (int rc = check_rotary(*rotary, c.head_dim)) return rc;
+  if (!a.k || !a.v || !a.indptr) return invalid("append: null pointer");
+  if ((a.q == nullptr) != (a.q_out == nullptr)) return invalid("append: q and q_out go together");
+  if (a.q && a.q_heads == 0) return invalid("append: q without heads");
+  if (a.tokens > INT_MAX || a.q_heads > 65536)
+    return fail(MONONN_ERR_TOO_LARGE, "append: tokens < 2^31, q_heads <= 65536");
+  if (!stride_in_range(a.k_token_stride) || !stride_in_range(a.k_head_stride) || !stride_in_range(a.v_token_stride) ||
+      !stride_in_range(a.v_head_stride) || !stride_in_range(a.q_token_stride) || !stride_in_range(a.q_head_stride) ||
+      !stride_in_range(a.q_out_token_stride) || !stride_in_range(a.q_out_head_stride))
+    return invalid("append: strides must be in 0 .. 2^39");
+  if (!aligned(a.k, 2) || !aligned(a.v, 2) || !aligned(a.q, 2) || !aligned(a.q_out, 2) || !aligned(a.indptr, 4) ||
+      !aligned(a.positions, 4))
+    return invalid("append: misaligned pointer");
+  const int64_t d = c.head_dim;
+  if (a.q && ((a.q_heads > 1 && a.q_out_head_stride < d) || (a.tokens > 1 && a.q_out_token_stride < d)))
+    return invalid("append: strides of q_out are smaller than the heads they hold");
+  if (a.q && a.q == a.q_out &&
+      (a.q_token_stride != a.q_out_token_stride || a.q_head_stride != a.q_out_head_stride))
+    return invalid("append: in place, q and q_out have the same strides");
+  if (a.tokens == 0 || c.sequences == 0) return MONONN_OK;
+  OnDeviceOf guard;
+  const Device* dev = nullptr;
+  if (int rc = guard.enter(c.k_pages, &dev)) return rc;
+  RowsParams p{};
+  if (a.q)
+    p.q = RowsSource{a.q, a.q_out, a.q_token_stride, a.q_head_stride, a.q_out_token_stride, a.q_out_head_stride, a.q_heads};
+  p.k = RowsSource{a.k, c.k_pages, a.k_token_stride, a.k_head_stride, c.token_stride, c.head_stride, c.kv_heads};
+  p.v = RowsSource{a.v, c.v_pages, a.v_token_stride, a.v_head_stride, c.token_stride, c.head_stride, c.kv_heads};
+  p.positions = a.positions;
+  p.indptr = a.indptr;
+  p.lengths = c.lengths;
+  p.table = c.page_table;
+  p.table_stride = c.table_stride;
+  p.page_stride = c.page_stride;
+  p.tokens = a.tokens;
+  p.head_dim = c.head_dim;
+  p.sequences = c.sequences;
+  p.max_pages = c.max_pages;
+  p.num_pages = c.num_pages;
+  p.page_size = c.page_size;
+  if (rotary) set_rotation(&p, *rotary);
+  return launched(launch_rows(p, c.dtype == MONONN_BF16, rows_by_vectors(p), dev->sm_count,
+                              static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
+                                     size_t* bytes) {
+  if (!bytes) return invalid("null argument");
+  *bytes = 0;
+  if (int rc = check_attention(cache, args)) return rc;
+  if (args->tokens == 0 || cache->sequences == 0) return MONONN_OK;
+  OnDeviceOf guard;
+  const Device* dev = nullptr;
+  if (int rc = guard.enter(cache->k_pages, &dev)) return rc;
+  AttentionPlan plan;
+  plan_attention(*cache, *args, dev->sm_count, &plan);
+  *bytes = plan.workspace;
+  return MONONN_OK;
+}
+
+int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
+                           void* cuda_stream) {
+  if (int rc = check_attention(cache, args)) return rc;
+  const mononn_paged_cache& c = *cache;
+  const mononn_paged_attention_args& a = *args;
+  if (a.tokens == 0 || c.sequences == 0) return MONONN_OK;
+  OnDeviceOf guard;
+  const Device* dev = nullptr;
+  if (int rc = guard.enter(c.k_pages, &dev)) return rc;
+  AttentionPlan plan;
+  plan_attention(c, a, dev->sm_count, &plan);
+  if (plan.workspace && (!a.workspace || a.workspace_bytes < plan.workspace || !aligned(a.workspace, 16)))
+    return invalid("attention: needs a workspace of " + std::to_string(plan.workspace) + " bytes, 16-byte aligned");
+  AttentionParams p{};
+  if (int rc = encode_pages(&p.k_map, c, c.k_pages, plan.box, "k_pages")) return rc;
+  if (int rc = encode_pages(&p.v_map, c, c.v_pages, plan.box, "v_pages")) return rc;
+  p.q = a.q;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.q_token = a.q_token_stride;
+  p.q_head = a.q_head_stride;
+  p.out_token = a.out_token_stride;
+  p.out_head = a.out_head_stride;
+  p.table_stride = c.table_stride;
+  p.table = c.page_table;
+  p.lengths = c.lengths;
+  p.indptr = a.indptr;
+  if (plan.joins) {
+    p.headers = static_cast<AttentionHeader*>(a.workspace);
+    p.partial = reinterpret_cast<float*>(static_cast<char*>(a.workspace) +
+                                         (plan.ctas * sizeof(AttentionHeader) + 255) / 256 * 256);
+  }
+  p.status = dev->status;
+  p.sequences = c.sequences;
+  p.tokens = a.tokens;
+  p.kv_heads = c.kv_heads;
+  p.group = a.q_heads / c.kv_heads;
+  p.head_dim = c.head_dim;
+  p.page_size = c.page_size;
+  p.capacity = c.max_pages * c.page_size;
+  p.box = plan.box;
+  p.causal = a.causal != 0;
+  p.window = a.window;
+  p.whole_items = !plan.joins;
+  p.min_units = plan.joins ? kFewLeastUnits : 1;
+  p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
+  p.scale_log2 = p.scale * 1.4426950408889634f;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  if (int rc = launched(launch_few_rows(p, plan, c.dtype == MONONN_BF16, stream))) return rc;
+  return plan.joins ? launched(launch_join(p, plan, c.dtype == MONONN_BF16, stream)) : MONONN_OK;
+}
+
+int mononn_paged_attention_status(void* cuda_stream) {
+  int count = 0;
+  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+    cudaGetLastError();
+    return fail(MONONN_ERR_NO_DEVICE, "no CUDA device");
+  }
+  int current = 0, of_stream = 0;
+  PG_TRY(cudaGetDevice(&current));
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  of_stream = current;
+  if (cuda_stream && cuda_stream != cudaStreamLegacy && cuda_stream != cudaStreamPerThread)
+    PG_TRY(cudaStreamGetDevice(stream, &of_stream));
+  struct Back {
+    int to;
+    ~Back() {
+      if (to >= 0) cudaSetDevice(to);
+    }
+  } back{-1};
+  if (of_stream != current) {
+    PG_TRY(cudaSetDevice(of_stream));
+    back.to = current;
+  }
+  if (of_stream < 0 || of_stream >= kMaxDevices) return invalid("device ordinal out of range");
+  const Device* dev = nullptr;
+  if (int rc = set_up(of_stream, &dev)) return rc;
+  uint32_t status = 0;
+  PG_TRY(cudaMemcpyAsync(&status, dev->status, sizeof(status), cudaMemcpyDeviceToHost, stream));
+  PG_TRY(cudaStreamSynchronize(stream));
+  if (status == 0) return MONONN_OK;
+  PG_TRY(cudaMemsetAsync(dev->status, 0, sizeof(uint32_t), stream));
+  PG_TRY(cudaStreamSynchronize(stream));
+  return fail(MONONN_ERR_BARRIER_TIMEOUT, "a bounded wait expired in a paged attention kernel; its output is incomplete");
+}
+
+}  // extern "C"

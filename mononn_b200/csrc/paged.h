@@ -1,0 +1,82 @@
+// Operators behind a prompt: what their host side (paged.cc) and their kernels share.
+//
+// A call's work is divided in units: one tile of keys for one item, an item being the queries of one
+// row tile (rows = new tokens x query heads of one key head) of one sequence. Sequences differ in
+// length by orders of magnitude and their lengths are on the device only, so every CTA adds up the
+// units of the whole call itself and takes an equal, contiguous share of them: the shares differ by
+// one unit at most whatever the lengths are. A share may begin or end within an item; such pieces
+// go to the workspace with their row maxima and sums, and a second, small kernel joins
+// them in the order of the keys.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace mononn {
+
+// ------------------------------------------------------------- rotation and append
+struct RowsSource {  // tokens x heads x head_dim
+  const void* src;
+  void* dst;
+  int64_t src_token, src_head, dst_token, dst_head;
+  uint32_t heads;
+};
+struct RowsParams {
+  RowsSource q, k, v;    // q and k are rotated; k and v go into pages when `table` is set
+  const int32_t* positions;
+  const int32_t* indptr;
+  const int32_t* lengths;
+  const int32_t* table;
+  int64_t table_stride, page_stride;
+  uint32_t tokens, head_dim, sequences, max_pages, num_pages, page_size;
+  uint32_t rotary_dim, interleaved;
+  float magnitude;
+  double turns[128];
+};
+cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int sm_count, cudaStream_t stream);
+
+// ------------------------------------------------------------------------ attention
+constexpr uint32_t kFewRows = 16;     // rows of an item in the kernel for few rows
+constexpr uint32_t kFewKeys = 64;     // keys of a unit there
+
+struct AttentionHeader {  // one per CTA: the item that begins in it and goes on in the next `more` CTAs
+  uint32_t more;          // 0: none
+  uint32_t rows;
+  uint32_t first_row;     // within the sequence's (token, head of the group) rows
+  uint32_t head;          // key head
+  uint32_t token;         // first new token of the sequence
+  uint32_t pad[3];
+};
+struct AttentionParams {
+  CUtensorMap k_map, v_map;
+  const void* q;
+  void* out;
+  float* lse;
+  int64_t q_token, q_head, out_token, out_head, table_stride;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* indptr;
+  AttentionHeader* headers;
+  float* partial;           // slots 2 * CTA (an item begun earlier) and 2 * CTA + 1 (one that goes on)
+  uint32_t* status;
+  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box;
+  uint32_t causal, window, min_units, whole_items;
+  float scale, scale_log2;  // of the scores; scale * log2(e)
+};
+struct AttentionPlan {  // how a call is launched: the same for every content of its device arrays
+  uint32_t rows, keys, padded_dim, ctas;
+  uint32_t box;         // token rows that one copy brings
+  bool joins;           // an item may span CTAs: workspace and the second kernel are needed
+  size_t workspace;
+};
+// Floats of one slot: row maximum and row sum, then the rows.
+inline size_t attention_slot_floats(const AttentionPlan& p) {
+  return static_cast<size_t>(p.rows) * (2 + p.padded_dim);
+}
+size_t few_rows_smem(uint32_t padded_dim);
+cudaError_t prepare_few_rows();
+cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
+cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
+cudaError_t paged_status_word(uint32_t** out);
+
+}  // namespace mononn

@@ -1,0 +1,487 @@
+// Attention over a paged cache for few rows: single tokens, a few drafted ones, grouped heads.
+//
+// o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = scale q.k_j, in one pass over the keys with the
+// running maximum m and sum of every row. The rows of an item (new tokens x query heads that share a key
+// head) fill one 16-row matrix instruction; each of four warps takes 16 keys of every tile of 64 and
+// keeps a maximum, a sum and an output of its own, which are added up when the item ends.
+#include "paged_device.h"
+
+namespace mononn {
+namespace paged {
+
+constexpr int kWarps = 4;  // that compute
+constexpr int kThreadsFew = (kWarps + 1) * 32;
+constexpr int kSlots = 4;  // of keys or values of one tile
+
+template <int DIM>
+struct FewSmem {
+  static constexpr int kSlotBytes = static_cast<int>(kFewKeys) * DIM * 2;
+  static constexpr int kPitch = DIM + 8;  // floats between rows of the warps' outputs: no bank conflicts
+  static constexpr int kOutputs = kSlots * kSlotBytes;
+  static constexpr int kControl = kOutputs + kWarps * static_cast<int>(kFewRows) * kPitch * 4;
+  static constexpr int kBytes = kControl + 1024;
+};
+struct FewControl {
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t sums[8];
+  Share share;
+  uint32_t gave_up;
+  float maxima[kWarps][kFewRows], totals[kWarps][kFewRows];
+};
+static_assert(sizeof(FewControl) <= 1024, "control block");
+
+__device__ __forceinline__ void matrices_4(uint32_t address, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address)
+               : "memory");
+}
+__device__ __forceinline__ void matrices_4_transposed(uint32_t address, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(address)
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void multiply<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void multiply<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_constant__ AttentionParams P) {
+  extern __shared__ uint8_t raw[];
+  using M = FewSmem<DIM>;
+  constexpr int kHalves = DIM / 64;
+  constexpr int kSteps = DIM / 16;
+  uint8_t* smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
+  FewControl& C = *reinterpret_cast<FewControl*>(smem + M::kControl);
+  const uint32_t slots = smem_address(smem);
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      barrier_init(smem_address(&C.full[i]), 1);
+      barrier_init(smem_address(&C.empty[i]), kWarps);
+    }
+    C.gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&P.v_map));
+  }
+  let_next_begin();
+  earlier_done();
+  find_share<kFewRows, kFewKeys, kThreadsFew>(P, C.sums, &C.share);  // a barrier of the CTA within
+  const Share share = C.share;
+  Pieces<kFewRows, kFewKeys> piece(P, share);
+
+  uint32_t fills = 0;  // of the loading warp
+  if (warp == kWarps) {
+    TileLoader<kFewKeys, kHalves> loader(P);
+    bool fine = true;
+    while (fine && piece.next()) {
+      loader.look_up(piece.b, piece.keys, piece.first_tile);
+      for (uint32_t u = 0; fine && u < piece.count; ++u) {
+        const TileLoader<kFewKeys, kHalves> now = loader;
+        if (u + 1 < piece.count) loader.look_up(piece.b, piece.keys, piece.first_tile + u + 1);
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t slot = fills % kSlots;
+          fine = fine && barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kSlots) & 1u) ^ 1u, &C.gave_up);
+          if (!fine) break;
+          now.load(kv ? &P.v_map : &P.k_map, slots + slot * M::kSlotBytes, piece.head, smem_address(&C.full[slot]));
+          ++fills;
+        }
+      }
+      piece.done();
+    }
+  } else {
+    const float ninf = __int_as_float(0xff800000);
+    uint32_t slot = 0, parity = 0;
+    float* const outputs = reinterpret_cast<float*>(smem + M::kOutputs);
+    // ldmatrix addresses: lanes 0-7, 8-15, .. point at the rows of the four 8 x 8 matrices
+    const uint32_t key_row = warp * 16 + (lane & 7u) + ((lane >> 4) << 3), key_chunk = (lane >> 3) & 1u;
+    const uint32_t val_row = warp * 16 + (lane & 15u), val_chunk = lane >> 4;
+    AttentionHeader header{0, 0, 0, 0, 0, {0, 0, 0}};
+    // After a wait that gave up the remaining ones end at once, and the warps still meet everywhere.
+    while (piece.next()) {
+      const uint32_t rows = piece.rows();
+      // queries: rows lane / 4 and + 8 of the 16, two elements of each 8
+      uint32_t q[kSteps][4];
+      int32_t see_from[2], see_to[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t r = (lane >> 2) + 8 * i;
+        const uint32_t row = piece.tile * kFewRows + r;
+        const uint32_t token = row / P.group, head = piece.head * P.group + row % P.group;
+        const bool valid = r < rows;
+        const T* src = static_cast<const T*>(P.q) + (piece.s.token + static_cast<int64_t>(token)) * P.q_token +
+                       static_cast<int64_t>(head) * P.q_head;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t d = k * 16 + j * 8 + (lane & 3u) * 2;
+            q[k][j * 2 + i] = valid && d < P.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          }
+        const int32_t position = piece.s.length - piece.s.n + static_cast<int32_t>(token);
+        see_to[i] = valid ? (P.causal ? max(position + 1, 0) : piece.s.length) : 0x7fffffff;
+        see_from[i] = 0;
+        if (valid && P.causal && P.window)
+          see_from[i] = static_cast<int32_t>(max(static_cast<int64_t>(0), position + 1 - static_cast<int64_t>(P.window)));
+      }
+      // keys that every row sees need no test
+      const int32_t all_from = __reduce_max_sync(0xffffffffu, max(see_from[0], see_from[1]));
+      const int32_t all_to = __reduce_min_sync(0xffffffffu, min(see_to[0], see_to[1]));
+
+      float acc[kSteps * 2][4];
+#pragma unroll
+      for (int i = 0; i < kSteps * 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+      float m[2] = {ninf, ninf}, l[2] = {0.f, 0.f};
+
+      for (uint32_t u = 0; u < piece.count; ++u) {
+        const int32_t key0 = static_cast<int32_t>((piece.first_tile + u) * kFewKeys + warp * 16);
+        const bool any = key0 < piece.keys.end && key0 + 16 > piece.keys.begin;
+        const bool tested = key0 < all_from || key0 + 16 > all_to;
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+        if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
+        if (any) {
+          const uint32_t base = slots + slot * M::kSlotBytes + key_row * 128;
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            uint32_t b[4];
+            const uint32_t chunk = (k & 3) * 2 + key_chunk;
+            matrices_4(base + (k >> 2) * kFewKeys * 128 + ((chunk ^ (key_row & 7u)) << 4), b);
+            multiply<T>(s[0], q[k], b[0], b[1]);
+            multiply<T>(s[1], q[k], b[2], b[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(smem_address(&C.empty[slot]));
+        if (++slot == kSlots) slot = 0, parity ^= 1u;
+
+        uint32_t p[4];
+        if (any) {
+          if (tested) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int32_t key = key0 + i * 8 + (lane & 3u) * 2 + (j & 1);
+                if (key < see_from[j >> 1] || key >= see_to[j >> 1]) s[i][j] = ninf;
+              }
+          }
+          float top[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(fmaxf(s[0][r * 2], s[0][r * 2 + 1]), fmaxf(s[1][r * 2], s[1][r * 2 + 1]));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            top[r] = fmaxf(top[r], m[r]);
+          }
+          if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+            float f[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              f[r] = top[r] == m[r] ? 1.f : exp2_fast((m[r] - top[r]) * P.scale_log2);
+              m[r] = top[r];
+              l[r] *= f[r];
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps * 2; ++i) {
+              acc[i][0] *= f[0];
+              acc[i][1] *= f[0];
+              acc[i][2] *= f[1];
+              acc[i][3] *= f[1];
+            }
+          }
+          // a row that has seen nothing yet: exp2(-inf - 0) = 0
+          const float shift[2] = {m[0] == ninf ? 0.f : m[0] * P.scale_log2, m[1] == ninf ? 0.f : m[1] * P.scale_log2};
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              s[i][j] = exp2_fast(fmaf(s[i][j], P.scale_log2, -shift[j >> 1]));
+              l[j >> 1] += s[i][j];
+            }
+          // the probabilities take the values' type for the product: one rounding of half a step each
+          p[0] = Pair<T>::pack(s[0][0], s[0][1]);
+          p[1] = Pair<T>::pack(s[0][2], s[0][3]);
+          p[2] = Pair<T>::pack(s[1][0], s[1][1]);
+          p[3] = Pair<T>::pack(s[1][2], s[1][3]);
+        }
+        if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
+        if (any) {
+          const uint32_t base = slots + slot * M::kSlotBytes + val_row * 128;
+          // value rows that no row of the item sees may hold anything: 0 x NaN is not 0
+          const bool clear = key0 < piece.keys.begin || key0 + 16 > piece.keys.end;
+          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+          if (clear) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int32_t key = key0 + i * 8 + (lane & 3u) * 2;
+              const bool a = key >= piece.keys.begin && key < piece.keys.end;
+              const bool b = key + 1 >= piece.keys.begin && key + 1 < piece.keys.end;
+              keep[i] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k) {
+            uint32_t b[4];
+            const uint32_t chunk = (k & 3) * 2 + val_chunk;
+            matrices_4_transposed(base + (k >> 2) * kFewKeys * 128 + ((chunk ^ (val_row & 7u)) << 4), b);
+            multiply<T>(acc[k * 2], p, b[0] & keep[0], b[1] & keep[1]);
+            multiply<T>(acc[k * 2 + 1], p, b[2] & keep[0], b[3] & keep[1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) barrier_arrive(smem_address(&C.empty[slot]));
+        if (++slot == kSlots) slot = 0, parity ^= 1u;
+      }
+
+      // the four warps' results of this piece
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      }
+      warps_meet();  // the last piece's have been read
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t row = (lane >> 2) + 8 * r;
+        if (row < rows) {
+          if ((lane & 3u) == 0) {
+            C.maxima[warp][row] = m[r];
+            C.totals[warp][row] = l[r];
+          }
+          float* to = outputs + (warp * kFewRows + row) * M::kPitch + (lane & 3u) * 2;
+#pragma unroll
+          for (int i = 0; i < kSteps * 2; ++i)
+            *reinterpret_cast<float2*>(to + i * 8) = make_float2(acc[i][r * 2], acc[i][r * 2 + 1]);
+        }
+      }
+      warps_meet();
+      const bool complete = piece.begins() && piece.ends();
+      float* slot_out = nullptr;
+      if (!complete)
+        slot_out = P.partial + (2u * blockIdx.x + (piece.begins() ? 1u : 0u)) *
+                                   static_cast<size_t>(kFewRows * (2 + DIM));
+      for (uint32_t i = threadIdx.x; i < rows * (DIM / 8); i += kWarps * 32) {
+        const uint32_t row = i / (DIM / 8), d = (i % (DIM / 8)) * 8;
+        float top = C.maxima[0][row];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, C.maxima[w][row]);
+        float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = C.maxima[w][row];
+          const float f = mw == ninf ? 0.f : exp2_fast((mw - top) * P.scale_log2);
+          sum += f * C.totals[w][row];
+          const float4* from = reinterpret_cast<const float4*>(outputs + (w * kFewRows + row) * M::kPitch + d);
+          const float4 a = from[0], b = from[1];
+          o[0] += f * a.x; o[1] += f * a.y; o[2] += f * a.z; o[3] += f * a.w;
+          o[4] += f * b.x; o[5] += f * b.y; o[6] += f * b.z; o[7] += f * b.w;
+        }
+        if (complete) {
+          const uint32_t g = piece.tile * kFewRows + row;
+          const int64_t token = piece.s.token + static_cast<int64_t>(g / P.group);
+          const uint32_t head = piece.head * P.group + g % P.group;
+          const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+          if (d < P.head_dim) {
+            uint4 v;
+            v.x = Pair<T>::pack(o[0] * inverse, o[1] * inverse);
+            v.y = Pair<T>::pack(o[2] * inverse, o[3] * inverse);
+            v.z = Pair<T>::pack(o[4] * inverse, o[5] * inverse);
+            v.w = Pair<T>::pack(o[6] * inverse, o[7] * inverse);
+            *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + token * P.out_token +
+                                      static_cast<int64_t>(head) * P.out_head + d) = v;
+          }
+          if (d == 0 && P.lse)
+            P.lse[token * P.kv_heads * P.group + head] = sum == 0.f ? ninf : top * P.scale + logf(sum);
+        } else {
+          if (d == 0) {
+            slot_out[row * 2] = top;
+            slot_out[row * 2 + 1] = sum;
+          }
+          float4* to = reinterpret_cast<float4*>(slot_out + kFewRows * 2 + row * DIM + d);
+          to[0] = make_float4(o[0], o[1], o[2], o[3]);
+          to[1] = make_float4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      if (piece.begins() && !piece.ends())
+        header = AttentionHeader{piece.more(share), rows, piece.tile * kFewRows, piece.head,
+                                 static_cast<uint32_t>(piece.s.token), {0, 0, 0}};
+      piece.done();
+    }
+    if (threadIdx.x == 0 && P.headers) P.headers[blockIdx.x] = header;
+  }
+  __syncthreads();
+  if (C.gave_up && warp == kWarps) {
+    for (uint32_t f = fills > kSlots ? fills - kSlots : 0u; f < fills; ++f)
+      barrier_wait_out(smem_address(&C.full[f % kSlots]), (f / kSlots) & 1u);
+    if (lane == 0) atomicExch(P.status, 1u);
+  }
+}
+
+// Joins the pieces of the items that span CTAs: o = sum_i f_i o_i / sum_i f_i l_i, f_i = exp(m_i - m),
+// in the order of the keys. Block (CTA, group of rows): the item that begins in that CTA. A warp for
+// each row, or, where items are few and cut into many pieces, several with a part of the pieces each.
+constexpr int kJoinWarps = 8;
+template <typename T, int DIM, int ROWS, int PARTS>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttentionParams P) {
+  constexpr int kRowsHere = kJoinWarps / PARTS;
+  constexpr int kEach = DIM / 32;  // consecutive elements of a lane
+  __shared__ float sums[kJoinWarps][DIM];
+  __shared__ float tops[kJoinWarps], totals[kJoinWarps];
+  earlier_done();
+  const AttentionHeader h = P.headers[blockIdx.x];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, part = warp % PARTS;
+  const uint32_t row0 = blockIdx.y * kRowsHere;
+  if (h.more == 0 || row0 >= h.rows) return;
+  const uint32_t row = min(row0 + warp / PARTS, h.rows - 1u);
+  const float ninf = __int_as_float(0xff800000);
+  constexpr size_t kSlot = static_cast<size_t>(ROWS) * (2 + DIM);
+  float top = ninf, total = 0.f, o[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) o[i] = 0.f;
+  const uint32_t pieces = h.more + 1u;
+  const uint32_t first = pieces * part / PARTS, last = pieces * (part + 1u) / PARTS;
+#pragma unroll 4
+  for (uint32_t i = first; i < last; ++i) {
+    const float* slot = P.partial + (2u * (blockIdx.x + i) + (i == 0 ? 1u : 0u)) * kSlot;
+    const float2 ml = *reinterpret_cast<const float2*>(slot + row * 2);
+    const float* from = slot + ROWS * 2 + row * DIM + lane * kEach;
+    float v[kEach];
+    if constexpr (kEach == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(from);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    } else {
+      const float2 a = *reinterpret_cast<const float2*>(from);
+      v[0] = a.x; v[1] = a.y;
+    }
+    const float next = fmaxf(top, ml.x);
+    const float keep = top == next ? 1.f : exp2_fast((top - next) * P.scale_log2);
+    const float f = ml.x == next ? (next == ninf ? 0.f : 1.f) : exp2_fast((ml.x - next) * P.scale_log2);
+    top = next;
+    total = total * keep + f * ml.y;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) o[j] = o[j] * keep + f * v[j];
+  }
+  if constexpr (PARTS > 1) {
+    if (lane == 0) tops[warp] = top, totals[warp] = total;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) sums[warp][lane * kEach + j] = o[j];
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int p = 1; p < PARTS; ++p) top = fmaxf(top, tops[warp + p]);
+    total = 0.f;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) o[j] = 0.f;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      const float mp = tops[warp + p];
+      const float f = mp == ninf ? 0.f : exp2_fast((mp - top) * P.scale_log2);
+      total += f * totals[warp + p];
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) o[j] += f * sums[warp + p][lane * kEach + j];
+    }
+  }
+  if (part != 0 || row0 + warp / PARTS >= h.rows) return;
+  const uint32_t g = h.first_row + row;
+  const int64_t token = static_cast<int64_t>(h.token) + g / P.group;
+  const uint32_t head = h.head * P.group + g % P.group;
+  const float inverse = total == 0.f ? 0.f : 1.f / total;
+  const uint32_t d = lane * kEach;
+  if (d < P.head_dim) {
+    uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<T*>(P.out) + token * P.out_token +
+                                               static_cast<int64_t>(head) * P.out_head + d);
+#pragma unroll
+    for (int j = 0; j < kEach; j += 2) to[j / 2] = Pair<T>::pack(o[j] * inverse, o[j + 1] * inverse);
+  }
+  if (lane == 0 && P.lse)
+    P.lse[token * P.kv_heads * P.group + head] = total == 0.f ? ninf : top * P.scale + logf(total);
+}
+
+}  // namespace paged
+
+static __device__ uint32_t g_status;
+cudaError_t paged_status_word(uint32_t** out) { return cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_status); }
+
+size_t few_rows_smem(uint32_t padded_dim) {
+  return 1024 + (padded_dim == 64 ? paged::FewSmem<64>::kBytes : paged::FewSmem<128>::kBytes);
+}
+
+namespace {
+template <typename F>
+cudaError_t with_type(bool bf16, uint32_t dim, F&& f) {
+  if (bf16) return dim == 64 ? f(__nv_bfloat16(), paged::FewSmem<64>()) : f(__nv_bfloat16(), paged::FewSmem<128>());
+  return dim == 64 ? f(__half(), paged::FewSmem<64>()) : f(__half(), paged::FewSmem<128>());
+}
+template <typename K>
+cudaError_t launch(K kernel, dim3 grid, uint32_t threads, size_t smem, const AttentionParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+}  // namespace
+
+cudaError_t prepare_few_rows() {
+  for (int bf16 = 0; bf16 < 2; ++bf16)
+    for (uint32_t dim : {64u, 128u}) {
+      const cudaError_t e = with_type(bf16 != 0, dim, [&](auto t, auto m) {
+        using T = decltype(t);
+        constexpr int kDim = decltype(m)::kPitch - 8;
+        return cudaFuncSetAttribute(paged::few_rows_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(few_rows_smem(kDim)));
+      });
+      if (e != cudaSuccess) return e;
+    }
+  return cudaSuccess;
+}
+cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
+  return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
+    using T = decltype(t);
+    constexpr int kDim = decltype(m)::kPitch - 8;
+    return launch(paged::few_rows_kernel<T, kDim>, dim3(plan.ctas), paged::kThreadsFew, few_rows_smem(kDim), p, stream);
+  });
+}
+cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
+  return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
+    using T = decltype(t);
+    constexpr int kDim = decltype(m)::kPitch - 8;
+    constexpr int kParts = 4, kRowsHere = paged::kJoinWarps / kParts;
+    return launch(paged::join_kernel<T, kDim, static_cast<int>(kFewRows), kParts>,
+                  dim3(plan.ctas, (kFewRows + kRowsHere - 1) / kRowsHere), paged::kJoinWarps * 32, 0, p, stream);
+  });
+}
+
+}  // namespace mononn

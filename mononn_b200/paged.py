@@ -1,0 +1,279 @@
+"""Operators behind a prompt on torch tensors: positions by rotation, a key/value cache of pages,
+attention of new tokens over it.  The thin mirror of the mononn_rotary_* and mononn_paged_* part of
+include/mononn.h; the reference has no counterpart (its decoder graphs end with the prompt).
+
+Each operator comes as a function, and as a runner (`rotary_runner`, `PagedCache.append_runner`,
+`PagedCache.attention_runner`): the arguments are checked and their addresses and sizes taken once, and
+the returned zero-argument callable does nothing but the library call, for serving loops that reuse
+their buffers (what page tables, lengths, indptr and positions hold is read on the device at each
+call).  A runner keeps its tensors alive; its stream is the one given, or torch's current stream of
+the tensors' device when it was made.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import dataclasses
+
+from . import capi
+from .capi import check, lib
+
+_SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
+
+
+@dataclasses.dataclass(frozen=True)
+class Rotary:
+    """A rotary embedding: which elements of a head turn, in which pairs, and how fast (the scalings are
+    those of mononn_rotary_config; None or 0 stands for the default)."""
+    rotary_dim: int
+    interleaved: bool = False
+    theta: float = 10000.0
+    scaling: str = "none"  # none, linear, base, ramp, bands
+    factor: float = 1.0
+    original_length: float = 0.0
+    low: float = 0.0
+    high: float = 0.0
+    magnitude: float = 0.0
+
+    def table(self) -> capi.RotaryTable:
+        """Turning rates (shares of a full turn per position) as the kernels take them."""
+        if self.scaling not in _SCALINGS:
+            raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}")
+        if not 0 <= self.rotary_dim < 2**32:
+            raise ValueError("rotary_dim out of range")
+        c = capi.RotaryConfigArgs(self.rotary_dim, int(self.interleaved), _SCALINGS[self.scaling], self.theta,
+                                  self.factor, self.original_length, self.low, self.high, self.magnitude)
+        t = capi.RotaryTable()
+        check(lib().mononn_rotary_init(C.byref(c), C.byref(t)))
+        return t
+
+
+def _dtype(t) -> int:
+    import torch
+    if t.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"float16 or bfloat16 tensors are needed, not {t.dtype}")
+    return int(t.dtype == torch.bfloat16)
+
+
+def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
+    """A [tokens, heads, head_dim] tensor of the dtype, device and head_dim of `like`."""
+    if t.dim() != 3 or t.shape[2] != like.shape[-1]:
+        raise ValueError(f"{name} must be [tokens, heads, {like.shape[-1]}], not {list(t.shape)}")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} must have {heads} heads, not {t.shape[1]}")
+    if tokens is not None and t.shape[0] != tokens:
+        raise ValueError(f"{name} must have {tokens} tokens, not {t.shape[0]}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be {like.dtype} on {like.device}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: elements of a head must be consecutive")
+    return t
+
+
+def _ints(name: str, t, like, shape):
+    import torch
+    if t.dtype != torch.int32 or t.device != like.device:
+        raise ValueError(f"{name} must be int32 on {like.device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    if t.numel() > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _stream(device, stream) -> C.c_void_p:
+    import torch
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    return C.c_void_p(s.cuda_stream)
+
+
+def _runner(fn, args, keep):
+    def run(_keep=keep):
+        rc = fn(*args)
+        if rc:
+            check(rc)
+    return run
+
+
+def _overlap(a, b) -> bool:
+    def span(t):
+        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1
+        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _out_rows(name: str, out, src):
+    """`out` is `src` itself, or does not touch it."""
+    if out.data_ptr() == src.data_ptr() and out.stride() == src.stride():
+        return out
+    if out.untyped_storage().data_ptr() == src.untyped_storage().data_ptr() and _overlap(out, src) \
+            and not _same_grid(out, src):
+        raise ValueError(f"{name} overlaps its source: pass the source itself, or other memory")
+    return out
+
+
+def _same_grid(a, b) -> bool:
+    """Head slices of one projection: the same rows, other columns (never the same elements)."""
+    if a.stride() != b.stride() or a.stride(0) == 0 or a.dim() != 3:
+        return False
+    off = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
+    width = max(a.shape[1], b.shape[1])
+    return a.stride(1) >= a.shape[2] and a.stride(0) >= off + (width - 1) * a.stride(1) + a.shape[2] \
+        and off >= (min(a.shape[1], b.shape[1]) - 1) * a.stride(1) + a.shape[2]
+
+
+def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):
+    """A prepared `rotary`."""
+    out = x if out is None else out
+    _rows("x", x, x, None)
+    _rows("out", out, x, x.shape[1], x.shape[0])
+    _out_rows("out", out, x)
+    _ints("positions", positions, x, (x.shape[0],))
+    a = capi.RotaryArgs(x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1),
+                        positions.data_ptr(), x.shape[0], x.shape[1], x.shape[2], _dtype(x))
+    table = rotary.table()
+    args = (C.byref(table), C.byref(a), _stream(x.device, stream))
+    return _runner(lib().mononn_rotary_apply, args, (x, out, positions, table, a))
+
+
+def rotary(x, positions, rotary: Rotary, out=None, stream=None):
+    """x [tokens, heads, head_dim] with the leading rotary_dim elements of each head turned by its token's
+    position (int32 [tokens]); in place unless `out` is given. Returns the rotated tensor."""
+    rotary_runner(x, positions, rotary, out, stream)()
+    return x if out is None else out
+
+
+class PagedCache:
+    """Keys and values in pages.
+
+    k_pages, v_pages  [pages, page_size, kv_heads, head_dim] f16 or bf16, with the same strides;
+                      elements of a head consecutive (a head-major cache is the transposed view of
+                      [pages, kv_heads, page_size, head_dim])
+    page_table        int32 [sequences, most pages of a sequence]
+    lengths           int32 [sequences]: tokens of each sequence, the new ones of a call among them
+    """
+
+    def __init__(self, k_pages, v_pages, page_table, lengths):
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+            raise ValueError("k_pages and v_pages must be [pages, page_size, kv_heads, head_dim], alike in sizes and strides")
+        if k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
+            raise ValueError("k_pages and v_pages must be of one dtype on one device")
+        if k_pages.shape[3] > 1 and k_pages.stride(3) != 1:
+            raise ValueError("k_pages: elements of a head must be consecutive")
+        if page_table.dim() != 2:
+            raise ValueError("page_table must be [sequences, pages]")
+        n, most = page_table.shape
+        _ints("page_table", page_table, k_pages, (n, most))
+        _ints("lengths", lengths, k_pages, (n,))
+        self.k_pages, self.v_pages, self.page_table, self.lengths = k_pages, v_pages, page_table, lengths
+        pages, size, heads, dim = k_pages.shape
+        ps, ts, hs, _ = k_pages.stride()
+        self._args = capi.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, hs, page_table.data_ptr(),
+                                         page_table.stride(0) if n > 1 else most, lengths.data_ptr(), n, most, pages,
+                                         size, heads, dim, _dtype(k_pages))
+
+    @property
+    def kv_heads(self) -> int:
+        return self.k_pages.shape[2]
+
+    def _indptr(self, indptr):
+        return _ints("indptr", indptr, self.k_pages, (self.page_table.shape[0] + 1,))
+
+    def append_runner(self, k, v, indptr, rotary: Rotary | None = None, positions=None, q=None, q_out=None, stream=None):
+        """A prepared `append`."""
+        _rows("k", k, self.k_pages, self.kv_heads)
+        _rows("v", v, self.k_pages, self.kv_heads, k.shape[0])
+        self._indptr(indptr)
+        if positions is not None:
+            _ints("positions", positions, k, (k.shape[0],))
+        if q is None and q_out is not None:
+            raise ValueError("q_out without q")
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            _rows("q", q, self.k_pages, None, k.shape[0])
+            _rows("q_out", q_out, self.k_pages, q.shape[1], k.shape[0])
+            _out_rows("q_out", q_out, q)
+        qs, os = (q.stride(), q_out.stride()) if q is not None else ((0, 0), (0, 0))
+        a = capi.PagedAppendArgs(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                 q.data_ptr() if q is not None else None,
+                                 q_out.data_ptr() if q is not None else None, qs[0], qs[1], os[0], os[1],
+                                 indptr.data_ptr(), positions.data_ptr() if positions is not None else None,
+                                 k.shape[0], q.shape[1] if q is not None else 0)
+        table = rotary.table() if rotary is not None else None
+        args = (C.byref(self._args), C.byref(table) if table is not None else None, C.byref(a),
+                _stream(k.device, stream))
+        return _runner(lib().mononn_paged_append, args, (self, k, v, q, q_out, indptr, positions, table, a))
+
+    def append(self, k, v, indptr, rotary: Rotary | None = None, positions=None, q=None, q_out=None, stream=None):
+        """Writes the new tokens' keys and values [tokens, kv_heads, head_dim] to their places, the last
+        positions of each sequence (rows indptr[b] .. indptr[b+1]-1 are sequence b's), the keys turned by
+        `rotary`; turns the queries q [tokens, q_heads, head_dim] of the same tokens in the same launch, in
+        place unless `q_out` is given. `positions` (int32 [tokens]) replaces the cache's positions
+        as the angle. Returns the rotated queries."""
+        self.append_runner(k, v, indptr, rotary, positions, q, q_out, stream)()
+        return q if q_out is None else q_out
+
+    def attention_runner(self, q, indptr, out=None, lse=None, scale=None, causal=True, window=0, max_new=0,
+                         workspace=None, stream=None):
+        """A prepared `attention`; what it returns is in `out` (made here when none is given: `.out`)."""
+        import torch
+        _rows("q", q, self.k_pages, None)
+        self._indptr(indptr)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _rows("out", out, self.k_pages, q.shape[1], q.shape[0])
+        if lse is not None:
+            if lse.dtype != torch.float32 or lse.device != q.device or tuple(lse.shape) != tuple(q.shape[:2]) \
+                    or not lse.is_contiguous():
+                raise ValueError(f"lse must be contiguous float32 {list(q.shape[:2])} on {q.device}")
+        if scale is not None and not scale > 0:
+            raise ValueError("scale must be positive")
+        if not 0 <= window < 2**32 or not 0 <= max_new < 2**32:
+            raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
+        for name, t in (("q", q), ("lse", lse), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):
+            if t is not None and _overlap(out, t) and out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() \
+                    and not (name == "q" and _same_grid(out, q)):
+                raise ValueError(f"out overlaps {name}")
+        a = capi.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
+                                    q.stride(0), q.stride(1), out.stride(0), out.stride(1), indptr.data_ptr(),
+                                    q.shape[0], q.shape[1], 0.0 if scale is None else scale, int(causal), window,
+                                    max_new, None, 0)
+        need = C.c_size_t()
+        check(lib().mononn_paged_attention_workspace(C.byref(self._args), C.byref(a), C.byref(need)))
+        if need.value:
+            if workspace is None:
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            if workspace.device != q.device or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be contiguous on {q.device}")
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
+        run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a))
+        run.out, run.workspace = out, workspace if need.value else None
+        return run
+
+    def attention(self, q, indptr, out=None, lse=None, scale=None, causal=True, window=0, max_new=0, workspace=None,
+                  stream=None):
+        """Attention of the new tokens' queries q [tokens, q_heads, head_dim] over the cache, which holds
+        their own keys already. Rows indptr[b] .. indptr[b+1]-1 are the last positions of sequence b.
+        causal: keys up to the own position; window > 0: the last `window` of those. scale: 1 / sqrt(head_dim)
+        unless given. max_new: at most how many new tokens a sequence has, when known (it chooses the
+        kernel). lse: float32 [tokens, q_heads] for the logarithm of the sum of exponentials. The
+        workspace is allocated through torch unless given; concurrent calls need one each."""
+        run = self.attention_runner(q, indptr, out, lse, scale, causal, window, max_new, workspace, stream)
+        run()
+        if stream is not None:  # what this call allocated is in use on that stream
+            import torch
+            for t in (run.out if out is None else None, run.workspace if workspace is None else None):
+                if t is not None:
+                    t.record_stream(stream)
+        return run.out
+
+
+def paged_attention_status(stream=None) -> None:
+    """Waits for the stream and raises MononnError(-6) when a bounded wait expired in a paged attention
+    kernel of its device since the last call (the output of that attention is incomplete)."""
+    import torch
+    st = stream if stream is not None else torch.cuda.current_stream()
+    check(lib().mononn_paged_attention_status(C.c_void_p(st.cuda_stream)))

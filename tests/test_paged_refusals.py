@@ -1,0 +1,213 @@
+"""What the operators behind a prompt refuse, and the rates of their rotation: host code, no GPU needed."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from mononn_b200 import PagedCache, Rotary, capi, rotary_runner
+from tests.paged_reference import rotary_rates
+
+FAKE = 1 << 20  # an aligned address that is never followed
+
+
+def cache_args(**change):
+    base = dict(k_pages=FAKE, v_pages=FAKE, page_stride=16 * 2 * 64, token_stride=2 * 64, head_stride=64,
+                page_table=FAKE, table_stride=4, lengths=FAKE, sequences=2, max_pages=4, num_pages=9, page_size=16,
+                kv_heads=2, head_dim=64, dtype=0)
+    return capi.PagedCacheArgs(**{**base, **change})
+
+
+def attention_args(**change):
+    base = dict(q=FAKE, out=FAKE, lse=None, q_token_stride=4 * 64, q_head_stride=64, out_token_stride=4 * 64,
+                out_head_stride=64, indptr=FAKE, tokens=3, q_heads=4, scale=0.0, causal=1, window=0, max_new=0,
+                workspace=None, workspace_bytes=0)
+    return capi.PagedAttentionArgs(**{**base, **change})
+
+
+def append_args(**change):
+    base = dict(k=FAKE, v=FAKE, k_token_stride=128, k_head_stride=64, v_token_stride=128, v_head_stride=64, q=None,
+                q_out=None, indptr=FAKE, positions=None, tokens=3, q_heads=0)
+    return capi.PagedAppendArgs(**{**base, **change})
+
+
+def rotary_args(**change):
+    base = dict(x=FAKE, out=FAKE, x_token_stride=128, x_head_stride=64, out_token_stride=128, out_head_stride=64,
+                positions=FAKE, tokens=3, heads=2, head_dim=64, dtype=0)
+    return capi.RotaryArgs(**{**base, **change})
+
+
+def attend(cache=None, args=None):
+    return capi.lib().mononn_paged_attention(C.byref(cache or cache_args()), C.byref(args or attention_args()), None)
+
+
+def append(cache=None, args=None, table=None):
+    return capi.lib().mononn_paged_append(C.byref(cache or cache_args()), C.byref(table) if table else None,
+                                          C.byref(args or append_args()), None)
+
+
+# Arguments in order get as far as the device: there is none here, and the address is none of a GPU there.
+PASSES = (-5, -1)
+
+
+@pytest.mark.parametrize("change", [
+    dict(k_pages=None), dict(page_table=None), dict(lengths=None), dict(page_size=0), dict(kv_heads=0),
+    dict(head_dim=0), dict(num_pages=0), dict(max_pages=0), dict(token_stride=63), dict(head_stride=32),
+    dict(page_stride=8), dict(table_stride=3), dict(token_stride=-128), dict(page_table=FAKE + 2),
+    dict(page_stride=1 << 39)])
+def test_cache_refused(lib_built, change):
+    assert attend(cache=cache_args(**change)) == -1
+    assert append(cache=cache_args(**change)) == -1
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(dtype=2), -3), (dict(num_pages=1 << 31), -10), (dict(max_pages=1 << 27, table_stride=1 << 27), -10),
+    (dict(head_dim=264, head_stride=264), -10), (dict(sequences=(1 << 24) + 1), -10)])
+def test_cache_outside_of_the_supported(lib_built, change, code):
+    assert attend(cache=cache_args(**change)) == code
+    assert append(cache=cache_args(**change)) == code
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=None), dict(out=None), dict(indptr=None), dict(q_heads=0), dict(q_heads=3), dict(q=FAKE + 2),
+    dict(out=FAKE + 8), dict(q_token_stride=4 * 64 + 1), dict(out_head_stride=60), dict(out_head_stride=32),
+    dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(causal=0, window=5), dict(lse=FAKE + 1),
+    dict(indptr=FAKE + 2), dict(q_token_stride=-64)])
+def test_attention_refused(lib_built, change):
+    assert attend(args=attention_args(**change)) == -1
+    assert b"attention" in capi.lib().mononn_last_error()
+
+
+@pytest.mark.parametrize("cache, args, code", [
+    (dict(head_dim=60), {}, -3), (dict(head_dim=136, head_stride=136, token_stride=272), {}, -3),
+    (dict(page_size=12), {}, -3), (dict(page_size=1), {}, -3), (dict(k_pages=FAKE + 8), {}, -1),
+    (dict(token_stride=132), {}, -1), ({}, dict(tokens=1 << 31), -10), ({}, dict(q_heads=1 << 17), -10)])
+def test_attention_outside_of_the_supported(lib_built, cache, args, code):
+    assert attend(cache_args(**cache), attention_args(**args)) == code
+    need = C.c_size_t(7)
+    assert capi.lib().mononn_paged_attention_workspace(C.byref(cache_args(**cache)), C.byref(attention_args(**args)),
+                                                       C.byref(need)) == code
+    assert need.value == 0
+
+
+@pytest.mark.parametrize("change", [
+    dict(k=None), dict(v=None), dict(indptr=None), dict(q=FAKE, q_heads=2), dict(q_out=FAKE), dict(k=FAKE + 1),
+    dict(q=FAKE, q_out=FAKE, q_heads=0), dict(positions=FAKE + 1), dict(k_token_stride=-1),
+    dict(q=FAKE, q_out=FAKE, q_heads=2, q_token_stride=128, q_head_stride=64, q_out_token_stride=256, q_out_head_stride=64),
+    dict(q=FAKE, q_out=FAKE + 4096, q_heads=2, q_token_stride=128, q_head_stride=64, q_out_token_stride=128,
+         q_out_head_stride=32)])
+def test_append_refused(lib_built, change):
+    assert append(args=append_args(**change)) == -1
+    assert b"append" in capi.lib().mononn_last_error()
+
+
+@pytest.mark.parametrize("change, code", [
+    (dict(x=None), -1), (dict(positions=None), -1), (dict(dtype=3), -3), (dict(head_dim=0), -10),
+    (dict(head_dim=257), -10), (dict(out=FAKE + 1), -1), (dict(out_token_stride=256), -1), (dict(positions=FAKE + 2), -1),
+    (dict(out=FAKE + (1 << 16), out_head_stride=8), -1), (dict(x_token_stride=-1), -1)])
+def test_rotary_refused(lib_built, change, code):
+    table = Rotary(64).table()
+    assert capi.lib().mononn_rotary_apply(C.byref(table), C.byref(rotary_args(**change)), None) == code
+
+
+def test_rotary_tables_refused(lib_built):
+    for change in (dict(rotary_dim=0), dict(rotary_dim=33), dict(rotary_dim=66), dict(rotary_dim=258), dict(magnitude=math.nan)):
+        table = Rotary(64).table()
+        for k, v in change.items():
+            setattr(table, k, v)
+        assert capi.lib().mononn_rotary_apply(C.byref(table), C.byref(rotary_args()), None) == -1
+        assert append(table=table) == -1
+    table = Rotary(64).table()
+    table.turns[31] = math.inf
+    assert append(table=table) == -1
+
+
+def test_arguments_in_order_get_to_the_device(lib_built):
+    table = Rotary(64).table()
+    assert attend() in PASSES
+    assert append(table=table) in PASSES
+    assert capi.lib().mononn_rotary_apply(C.byref(table), C.byref(rotary_args()), None) in PASSES
+    if not torch.cuda.is_available():
+        assert capi.lib().mononn_paged_attention_status(None) == -5
+
+
+def test_nothing_to_do_is_fine(lib_built):
+    assert attend(args=attention_args(tokens=0)) == 0
+    assert attend(cache=cache_args(sequences=0)) == 0
+    assert append(args=append_args(tokens=0)) == 0
+    table = Rotary(64).table()
+    assert capi.lib().mononn_rotary_apply(C.byref(table), C.byref(rotary_args(tokens=0)), None) == 0
+    lib = capi.lib()
+    assert lib.mononn_paged_attention(None, C.byref(attention_args()), None) == -1
+    assert lib.mononn_paged_append(C.byref(cache_args()), None, None, None) == -1
+    assert lib.mononn_rotary_apply(None, C.byref(rotary_args()), None) == -1
+    assert lib.mononn_rotary_init(None, None) == -1
+
+
+@pytest.mark.parametrize("change", [
+    dict(rotary_dim=0), dict(rotary_dim=7), dict(rotary_dim=258), dict(theta=1.0), dict(theta=-5.0), dict(theta=math.inf),
+    dict(scaling="linear", factor=0.0), dict(scaling="base", factor=-2.0), dict(scaling="ramp", factor=2.0),
+    dict(scaling="bands", factor=2.0, original_length=100, low=4.0, high=4.0), dict(magnitude=-1.0),
+    dict(scaling="ramp", factor=math.nan, original_length=100)])
+def test_rotary_configuration_refused(lib_built, change):
+    with pytest.raises(capi.MononnError) as e:
+        Rotary(**{"rotary_dim": 64, **change}).table()
+    assert e.value.code == -1
+
+
+@pytest.mark.parametrize("r", [2, 6, 64, 96, 128, 256])
+@pytest.mark.parametrize("scaling", ["none", "linear", "base", "ramp", "bands"])
+@pytest.mark.parametrize("theta, factor, length", [(10000.0, 4.0, 4096.0), (500000.0, 8.0, 8192.0), (10000.0, 1.0, 2048.0)])
+def test_rates(lib_built, r, scaling, theta, factor, length):
+    table = Rotary(r, scaling=scaling, theta=theta, factor=factor, original_length=length).table()
+    want = rotary_rates(r, theta, scaling, factor if scaling != "none" else 1.0, length)
+    for i, f in enumerate(want):  # a few roundings of 64-bit numbers
+        assert abs(table.turns[i] * 2 * math.pi - f) <= 64 * 2.0 ** -53 * f
+    assert table.magnitude == (0.1 * math.log(factor) + 1.0 if scaling == "ramp" and factor > 1 else 1.0)
+    assert table.rotary_dim == r and table.interleaved == 0
+    assert Rotary(r, magnitude=0.5).table().magnitude == 0.5
+
+
+def small_cache(dtype=torch.float16):
+    pages = torch.zeros(4, 16, 2, 64, dtype=dtype)
+    return pages, torch.zeros_like(pages), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+
+def test_tensors_refused(lib_built):
+    k, v, table, lengths = small_cache()
+    good = PagedCache(k, v, table, lengths)
+    for bad in ((k, v[:3], table, lengths), (k, v.transpose(1, 2).contiguous().transpose(1, 2), table, lengths),
+                (k, v.bfloat16(), table, lengths), (k, v, table.long(), lengths), (k, v, table, lengths[:1]),
+                (k, v, table[0], lengths), (k.transpose(2, 3), v.transpose(2, 3), table, lengths)):
+        with pytest.raises((ValueError, TypeError)):
+            PagedCache(*bad)
+    with pytest.raises(TypeError):
+        PagedCache(k.float(), v.float(), table, lengths)
+    new = torch.zeros(3, 2, 64, dtype=torch.float16)
+    indptr = torch.zeros(3, dtype=torch.int32)
+    q = torch.zeros(3, 4, 64, dtype=torch.float16)
+    for args, kw in (((new, new[:2], indptr), {}), ((new[:, :1], new, indptr), {}), ((new, new, indptr[:2]), {}),
+                     ((new, new, indptr.long()), {}), ((new, new, indptr), dict(q_out=q)),
+                     ((new, new, indptr), dict(q=q[:2])), ((new, new, indptr), dict(q=q, q_out=q[:, :2])),
+                     ((new, new, indptr), dict(q=q, positions=torch.zeros(2, dtype=torch.int32))),
+                     ((new.bfloat16(), new, indptr), {}), ((new, new, indptr), dict(q=q[..., ::2]))):
+        with pytest.raises(ValueError):
+            good.append_runner(*args, **kw)
+    flat = torch.zeros(2 * 3 * 4 * 64, dtype=torch.float16)
+    over = flat[64:64 + 768].view(3, 4, 64)
+    with pytest.raises(ValueError):
+        good.append_runner(new, new, indptr, q=flat[:768].view(3, 4, 64), q_out=over)
+    for args, kw in (((q[..., :32], indptr), {}), ((q, indptr[:1]), {}), ((q, indptr), dict(out=q[:2])),
+                     ((q, indptr), dict(lse=torch.zeros(3, 4, dtype=torch.float16))), ((q, indptr), dict(scale=0.0)),
+                     ((q, indptr), dict(out=q)), ((q, indptr), dict(window=-1))):
+        with pytest.raises(ValueError):
+            good.attention_runner(*args, **kw)
+    x = torch.zeros(3, 4, 64, dtype=torch.float16)
+    pos = torch.zeros(3, dtype=torch.int32)
+    for args, kw in (((x, pos[:2], Rotary(64)), {}), ((x, pos.long(), Rotary(64)), {}),
+                     ((x, pos, Rotary(64)), dict(out=x[:2])), ((x[0], pos, Rotary(64)), {}),
+                     ((flat[:768].view(3, 4, 64), pos, Rotary(64)), dict(out=over))):
+        with pytest.raises(ValueError):
+            rotary_runner(*args, **kw)
+    with pytest.raises(ValueError):
+        Rotary(64, scaling="other").table()
