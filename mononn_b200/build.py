@@ -18,7 +18,7 @@ LIB = os.path.join(HERE, "libmononn_b200.so")
 HEADER = os.path.join(HERE, "..", "include", "mononn.h")
 SOURCES = ["megakernel.cu", "runtime.cu", "noalloc.cu", "mma_probe.cu", "scheduler.cc", "builders.cc",
            "spec.cc", "tuner.cc", "capi.cc", "hlo_parser.cc", "hlo_interp.cc", "hlo_lowering.cc",
-           "paged.cc", "paged_rows.cu", "paged_few.cu"]
+           "paged.cc", "paged_rows.cu", "paged_few.cu", "paged_many.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC"]
 

@@ -63,6 +63,7 @@ int set_up(int dev, const Device** out) {
     PG_TRY(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev));
     PG_TRY(paged_status_word(&d.status));
     PG_TRY(prepare_few_rows());
+    PG_TRY(prepare_many_rows());
     if (!g_encode) {
       cudaDriverEntryPointQueryResult q;
       void* fn = nullptr;
@@ -210,24 +211,29 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
   return MONONN_OK;
 }
 
-// How many CTAs, and whether an item may span them. Only sizes count that the host knows.
-constexpr uint32_t kFewWholeTiles = 8;  // caches of at most so many tiles: no item is split
-constexpr uint32_t kFewLeastUnits = 4;  // of a CTA's share
+// Which kernel, how many CTAs, and whether an item may span them. Only sizes count that the host knows.
+constexpr uint32_t kWholeKeys = 512;    // caches of at most so many keys: no item is split
+constexpr uint32_t kLeastKeys = 256;    // of a CTA's share, few rows
+constexpr uint32_t kManyLeastKeys = 512;  // of a CTA's share, many rows
 void plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
   const uint32_t group = a.q_heads / c.kv_heads;
   const uint64_t capacity = static_cast<uint64_t>(c.max_pages) * c.page_size;
+  const uint64_t new_tokens = a.max_new ? a.max_new : (a.tokens + c.sequences - 1) / c.sequences;
+  p->many = new_tokens * group > kFewRows;
   p->padded_dim = c.head_dim <= 64 ? 64 : 128;
-  p->rows = kFewRows;
-  p->keys = kFewKeys;
+  p->rows = p->many ? kManyRows : kFewRows;
+  p->keys = p->many ? kManyKeys : kFewKeys;
+  p->least_units = (p->many ? kManyLeastKeys : kLeastKeys) / p->keys;
   p->box = std::gcd(c.page_size, p->keys);
   // items: at most a row tile for each `rows` rows, and a ragged one for each sequence
   const uint64_t tiles = (capacity + p->keys - 1) / p->keys;
   const uint64_t most_rows = static_cast<uint64_t>(a.tokens) * group;
   const uint64_t items =
       (most_rows / p->rows + std::min<uint64_t>(c.sequences, a.tokens)) * c.kv_heads;
-  const bool whole = tiles <= kFewWholeTiles;
-  const uint64_t wanted = whole ? items : (items * tiles + kFewLeastUnits - 1) / kFewLeastUnits;
-  p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(wanted, 2u * static_cast<unsigned>(sm_count))));
+  const bool whole = capacity <= kWholeKeys;
+  const uint64_t wanted = whole ? items : (items * tiles + p->least_units - 1) / p->least_units;
+  const uint64_t most = static_cast<uint64_t>(p->many ? 1 : 2) * static_cast<unsigned>(sm_count);
+  p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, most)));
   p->joins = !whole && p->ctas > 1;
   p->workspace = 0;
   if (p->joins) {
@@ -427,12 +433,13 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.causal = a.causal != 0;
   p.window = a.window;
   p.whole_items = !plan.joins;
-  p.min_units = plan.joins ? kFewLeastUnits : 1;
+  p.min_units = plan.joins ? plan.least_units : 1;
   p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
   p.scale_log2 = p.scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (int rc = launched(launch_few_rows(p, plan, c.dtype == MONONN_BF16, stream))) return rc;
-  return plan.joins ? launched(launch_join(p, plan, c.dtype == MONONN_BF16, stream)) : MONONN_OK;
+  const bool bf16 = c.dtype == MONONN_BF16;
+  if (int rc = launched(plan.many ? launch_many_rows(p, plan, bf16, stream) : launch_few_rows(p, plan, bf16, stream))) return rc;
+  return plan.joins ? launched(launch_join(p, plan, bf16, stream)) : MONONN_OK;
 }
 
 int mononn_paged_attention_status(void* cuda_stream) {

@@ -38,6 +38,8 @@ cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int sm_cou
 // ------------------------------------------------------------------------ attention
 constexpr uint32_t kFewRows = 16;     // rows of an item in the kernel for few rows
 constexpr uint32_t kFewKeys = 64;     // keys of a unit there
+constexpr uint32_t kManyRows = 256;   // the same in the kernel for many rows
+constexpr uint32_t kManyKeys = 128;
 
 struct AttentionHeader {  // one per CTA: the item that begins in it and goes on in the next `more` CTAs
   uint32_t more;          // 0: none
@@ -64,7 +66,8 @@ struct AttentionParams {
   float scale, scale_log2;  // of the scores; scale * log2(e)
 };
 struct AttentionPlan {  // how a call is launched: the same for every content of its device arrays
-  uint32_t rows, keys, padded_dim, ctas;
+  bool many;            // the kernel for many rows
+  uint32_t rows, keys, padded_dim, ctas, least_units;
   uint32_t box;         // token rows that one copy brings
   bool joins;           // an item may span CTAs: workspace and the second kernel are needed
   size_t workspace;
@@ -76,7 +79,27 @@ inline size_t attention_slot_floats(const AttentionPlan& p) {
 size_t few_rows_smem(uint32_t padded_dim);
 cudaError_t prepare_few_rows();
 cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
+size_t many_rows_smem(uint32_t padded_dim);
+cudaError_t prepare_many_rows();
+cudaError_t launch_many_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
 cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
 cudaError_t paged_status_word(uint32_t** out);
+
+// A launch whose CTAs may be set up while the kernel before it still runs (they wait for its end
+// before they read or write anything; see earlier_done).
+template <typename K, typename Params>
+cudaError_t launch_dependent(K kernel, dim3 grid, uint32_t threads, size_t smem, const Params& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
 
 }  // namespace mononn

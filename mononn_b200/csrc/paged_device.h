@@ -39,27 +39,28 @@ __device__ __forceinline__ uint64_t timer_ns() {
 }
 // Bounded: after two seconds the CTA gives up, and so do all its other waits.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-static __device__ __noinline__ bool barrier_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
-  const uint64_t t0 = timer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (barrier_try(bar, parity)) return true;
-    if ((it & 63u) == 0u) {
-      if (*gave_up) return false;
-      if (timer_ns() - t0 > kWaitLimitNs) {
-        *gave_up = 1u;
-        return false;
-      }
+// Inline everywhere: a call would hold its caller to the registers of the launch.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
+  if (barrier_try(bar, parity)) return true;
+  uint64_t t0 = 0;
+#pragma unroll 1
+  for (uint32_t it = 1; !barrier_try(bar, parity); ++it) {
+    if ((it & 63u) != 0u) continue;
+    if (*gave_up) return false;
+    const uint64_t now = timer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > kWaitLimitNs) {
+      *gave_up = 1u;
+      return false;
     }
   }
+  return true;
 }
 // On the way out after that: copies of this CTA that are still in flight, bounded again.
-static __device__ __noinline__ void barrier_wait_out(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ void barrier_wait_out(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = timer_ns();
   while (!barrier_try(bar, parity) && timer_ns() - t0 <= kWaitLimitNs) {
   }
-}
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
-  return barrier_try(bar, parity) || barrier_wait_slow(bar, parity, gave_up);
 }
 // The whole warp gets the same answer.
 __device__ __forceinline__ bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {

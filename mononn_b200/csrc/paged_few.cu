@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
   let_next_begin();
   earlier_done();
   find_share<kFewRows, kFewKeys, kThreadsFew>(P, C.sums, &C.share);  // a barrier of the CTA within
-  const Share share = C.share;
+  const Share& share = C.share;
   Pieces<kFewRows, kFewKeys> piece(P, share);
 
   uint32_t fills = 0;  // of the loading warp
@@ -438,20 +438,6 @@ cudaError_t with_type(bool bf16, uint32_t dim, F&& f) {
   if (bf16) return dim == 64 ? f(__nv_bfloat16(), paged::FewSmem<64>()) : f(__nv_bfloat16(), paged::FewSmem<128>());
   return dim == 64 ? f(__half(), paged::FewSmem<64>()) : f(__half(), paged::FewSmem<128>());
 }
-template <typename K>
-cudaError_t launch(K kernel, dim3 grid, uint32_t threads, size_t smem, const AttentionParams& p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
 }  // namespace
 
 cudaError_t prepare_few_rows() {
@@ -471,16 +457,20 @@ cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan,
   return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
     using T = decltype(t);
     constexpr int kDim = decltype(m)::kPitch - 8;
-    return launch(paged::few_rows_kernel<T, kDim>, dim3(plan.ctas), paged::kThreadsFew, few_rows_smem(kDim), p, stream);
+    return launch_dependent(paged::few_rows_kernel<T, kDim>, dim3(plan.ctas), paged::kThreadsFew, few_rows_smem(kDim), p, stream);
   });
 }
 cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
   return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
     using T = decltype(t);
     constexpr int kDim = decltype(m)::kPitch - 8;
-    constexpr int kParts = 4, kRowsHere = paged::kJoinWarps / kParts;
-    return launch(paged::join_kernel<T, kDim, static_cast<int>(kFewRows), kParts>,
-                  dim3(plan.ctas, (kFewRows + kRowsHere - 1) / kRowsHere), paged::kJoinWarps * 32, 0, p, stream);
+    constexpr int kFew = static_cast<int>(kFewRows), kMany = static_cast<int>(kManyRows);
+    constexpr uint32_t kParts = 4, kRowsHere = paged::kJoinWarps / kParts;
+    if (plan.rows == kFewRows)
+      return launch_dependent(paged::join_kernel<T, kDim, kFew, kParts>, dim3(plan.ctas, kFew / kRowsHere),
+                              paged::kJoinWarps * 32, 0, p, stream);
+    return launch_dependent(paged::join_kernel<T, kDim, kMany, 1>, dim3(plan.ctas, kMany / paged::kJoinWarps),
+                            paged::kJoinWarps * 32, 0, p, stream);
   });
 }
 

@@ -169,20 +169,9 @@ __global__ void __launch_bounds__(kRowsThreads) rows_kernel(const __grid_constan
 }  // namespace paged
 
 cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.tokens);
-  cfg.blockDim = dim3(paged::kRowsThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (bf16)
-    return vectors ? cudaLaunchKernelEx(&cfg, paged::rows_kernel<__nv_bfloat16, 8>, p)
-                   : cudaLaunchKernelEx(&cfg, paged::rows_kernel<__nv_bfloat16, 1>, p);
-  return vectors ? cudaLaunchKernelEx(&cfg, paged::rows_kernel<__half, 8>, p)
-                 : cudaLaunchKernelEx(&cfg, paged::rows_kernel<__half, 1>, p);
+  auto launch = [&](auto kernel) { return launch_dependent(kernel, dim3(p.tokens), paged::kRowsThreads, 0, p, stream); };
+  if (bf16) return vectors ? launch(paged::rows_kernel<__nv_bfloat16, 8>) : launch(paged::rows_kernel<__nv_bfloat16, 1>);
+  return vectors ? launch(paged::rows_kernel<__half, 8>) : launch(paged::rows_kernel<__half, 1>);
 }
 
 }  // namespace mononn
