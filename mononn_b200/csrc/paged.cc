@@ -184,6 +184,22 @@ int encode_pages(CUtensorMap* map, const mononn_paged_cache& c, const void* base
   return MONONN_OK;
 }
 
+// One box is 64 elements of the heads of a group x the tokens of a row tile.
+int encode_queries(CUtensorMap* map, const mononn_paged_cache& c, const mononn_paged_attention_args& a, const AttentionPlan& plan) {
+  const uint32_t group = a.q_heads / c.kv_heads;
+  const cuuint64_t dims[3] = {c.head_dim, a.q_heads, a.tokens};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.q_heads > 1 ? a.q_head_stride : c.head_dim) * 2,
+                                 static_cast<cuuint64_t>(a.tokens > 1 ? a.q_token_stride : c.head_dim) * 2};
+  const cuuint32_t boxes[3] = {64, group, plan.item_rows / 2 / group}, steps[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, c.dtype == MONONN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              3, const_cast<void*>(a.q), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MONONN_ERR_CUDA, "q: cuTensorMapEncodeTiled failed (CUresult " + std::to_string(static_cast<int>(r)) + ")");
+  return MONONN_OK;
+}
+
 int check_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* a) {
   if (!cache || !a) return invalid("null argument");
   if (int rc = check_cache(*cache)) return rc;
@@ -199,8 +215,9 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
       !stride_in_range(a->out_token_stride) || !stride_in_range(a->out_head_stride))
     return invalid("attention: strides must be in 0 .. 2^39");
   const int64_t d = c.head_dim;
-  if ((a->q_heads > 1 && a->out_head_stride < d) || (a->tokens > 1 && a->out_token_stride < d))
-    return invalid("attention: strides of out are smaller than the heads they hold");
+  if ((a->q_heads > 1 && (a->out_head_stride < d || a->q_head_stride < d)) ||
+      (a->tokens > 1 && (a->out_token_stride < d || a->q_token_stride < d)))
+    return invalid("attention: strides of q or out are smaller than the heads they hold");
   if (!aligned(c.k_pages, 16) || !aligned(c.v_pages, 16) || !whole8(c.page_stride) || !whole8(c.token_stride) ||
       !whole8(c.head_stride) || !aligned(a->q, 16) || !whole8(a->q_token_stride) || !whole8(a->q_head_stride) ||
       !aligned(a->out, 16) || !whole8(a->out_token_stride) || !whole8(a->out_head_stride))
@@ -212,27 +229,35 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
 }
 
 // Which kernel, how many CTAs, and whether an item may span them. Only sizes count that the host knows.
-constexpr uint32_t kWholeKeys = 512;    // caches of at most so many keys: no item is split
-constexpr uint32_t kLeastKeys = 256;    // of a CTA's share, few rows
-constexpr uint32_t kManyLeastKeys = 512;  // of a CTA's share, many rows
-void plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
+constexpr uint32_t kWholeKeys = 512;      // caches of at most so many keys: no item is split
+constexpr uint32_t kFewLeastKeys = 256;   // of a CTA's share
+constexpr uint32_t kManyLeastKeys = 512;
+int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
   const uint32_t group = a.q_heads / c.kv_heads;
   const uint64_t capacity = static_cast<uint64_t>(c.max_pages) * c.page_size;
-  const uint64_t new_tokens = a.max_new ? a.max_new : (a.tokens + c.sequences - 1) / c.sequences;
-  p->many = new_tokens * group > kFewRows;
-  p->padded_dim = c.head_dim <= 64 ? 64 : 128;
-  p->rows = p->many ? kManyRows : kFewRows;
-  p->keys = p->many ? kManyKeys : kFewKeys;
-  p->least_units = (p->many ? kManyLeastKeys : kLeastKeys) / p->keys;
-  p->box = std::gcd(c.page_size, p->keys);
-  // items: at most a row tile for each `rows` rows, and a ragged one for each sequence
-  const uint64_t tiles = (capacity + p->keys - 1) / p->keys;
+  const uint64_t new_tokens = a.max_new ? a.max_new : (static_cast<uint64_t>(a.tokens) + c.sequences - 1) / c.sequences;
   const uint64_t most_rows = static_cast<uint64_t>(a.tokens) * group;
-  const uint64_t items =
-      (most_rows / p->rows + std::min<uint64_t>(c.sequences, a.tokens)) * c.kv_heads;
+  // a row tile for each `rows` rows at most, and a ragged one for each sequence
+  auto items = [&](uint32_t rows) { return (most_rows / rows + std::min<uint64_t>(c.sequences, a.tokens)) * c.kv_heads; };
+  auto tiles = [&](uint32_t keys) { return (capacity + keys - 1) / keys; };
+  constexpr uint64_t kMostUnits = 1ull << 31;
+  const uint64_t rows = std::min<uint64_t>(new_tokens * group, most_rows);
+  p->padded_dim = c.head_dim <= 64 ? 64 : 128;
+  const uint32_t few_rows = kFewRows * static_cast<uint32_t>(std::min<uint64_t>((rows + kFewRows - 1) / kFewRows, kFewTilesMost));
+  const uint32_t whole_tokens = group <= kTileRows ? kTileRows / group * group : 0;  // rows of a row tile of the other
+  p->many = rows > kFewTilesMost * kFewRows || items(few_rows) * tiles(kFewKeys) >= kMostUnits;
+  if (whole_tokens == 0) p->many = false;
+  p->rows = p->many ? kManyRows : few_rows;
+  p->item_rows = p->many ? 2 * whole_tokens : few_rows;
+  p->keys = p->many ? kManyKeys : kFewKeys;
+  p->least_units = (p->many ? kManyLeastKeys : kFewLeastKeys) / p->keys;
+  p->box = std::gcd(c.page_size, p->keys);
+  const uint64_t most_units = items(p->item_rows) * tiles(p->keys);
+  if (most_units >= kMostUnits)
+    return fail(MONONN_ERR_TOO_LARGE, "attention: so many new tokens over so many keys count 2^31 units of work or more");
   const bool whole = capacity <= kWholeKeys;
-  const uint64_t wanted = whole ? items : (items * tiles + p->least_units - 1) / p->least_units;
-  const uint64_t most = static_cast<uint64_t>(p->many ? 1 : 2) * static_cast<unsigned>(sm_count);
+  const uint64_t wanted = whole ? items(p->item_rows) : (most_units + p->least_units - 1) / p->least_units;
+  const uint64_t most = static_cast<uint64_t>(p->many || p->rows > kFewRows ? 1 : 2) * static_cast<unsigned>(sm_count);
   p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, most)));
   p->joins = !whole && p->ctas > 1;
   p->workspace = 0;
@@ -240,6 +265,7 @@ void plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_ar
     const size_t headers = (p->ctas * sizeof(AttentionHeader) + 255) / 256 * 256;
     p->workspace = headers + 2 * static_cast<size_t>(p->ctas) * attention_slot_floats(*p) * sizeof(float);
   }
+  return MONONN_OK;
 }
 }  // namespace
 
@@ -384,7 +410,7 @@ int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mono
   const Device* dev = nullptr;
   if (int rc = guard.enter(cache->k_pages, &dev)) return rc;
   AttentionPlan plan;
-  plan_attention(*cache, *args, dev->sm_count, &plan);
+  if (int rc = plan_attention(*cache, *args, dev->sm_count, &plan)) return rc;
   *bytes = plan.workspace;
   return MONONN_OK;
 }
@@ -399,12 +425,14 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   const Device* dev = nullptr;
   if (int rc = guard.enter(c.k_pages, &dev)) return rc;
   AttentionPlan plan;
-  plan_attention(c, a, dev->sm_count, &plan);
+  if (int rc = plan_attention(c, a, dev->sm_count, &plan)) return rc;
   if (plan.workspace && (!a.workspace || a.workspace_bytes < plan.workspace || !aligned(a.workspace, 16)))
     return invalid("attention: needs a workspace of " + std::to_string(plan.workspace) + " bytes, 16-byte aligned");
   AttentionParams p{};
   if (int rc = encode_pages(&p.k_map, c, c.k_pages, plan.box, "k_pages")) return rc;
   if (int rc = encode_pages(&p.v_map, c, c.v_pages, plan.box, "v_pages")) return rc;
+  if (plan.many)
+    if (int rc = encode_queries(&p.q_map, c, a, plan)) return rc;
   p.q = a.q;
   p.out = a.out;
   p.lse = a.lse;
@@ -430,6 +458,7 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.page_size = c.page_size;
   p.capacity = c.max_pages * c.page_size;
   p.box = plan.box;
+  p.item_rows = plan.item_rows;
   p.causal = a.causal != 0;
   p.window = a.window;
   p.whole_items = !plan.joins;

@@ -36,10 +36,10 @@ struct RowsParams {
 cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int sm_count, cudaStream_t stream);
 
 // ------------------------------------------------------------------------ attention
-constexpr uint32_t kFewRows = 16;     // rows of an item in the kernel for few rows
-constexpr uint32_t kFewKeys = 64;     // keys of a unit there
-constexpr uint32_t kManyRows = 256;   // the same in the kernel for many rows
-constexpr uint32_t kManyKeys = 128;
+// The kernel for few rows takes items of 16, 32 or 48 rows, and 64 keys a unit; the one for many rows
+// two tiles of up to 128 rows (whole tokens), and 128 keys.
+constexpr uint32_t kFewRows = 16, kFewTilesMost = 3, kFewKeys = 64;
+constexpr uint32_t kTileRows = 128, kManyRows = 2 * kTileRows, kManyKeys = 128;
 
 struct AttentionHeader {  // one per CTA: the item that begins in it and goes on in the next `more` CTAs
   uint32_t more;          // 0: none
@@ -50,7 +50,7 @@ struct AttentionHeader {  // one per CTA: the item that begins in it and goes on
   uint32_t pad[3];
 };
 struct AttentionParams {
-  CUtensorMap k_map, v_map;
+  CUtensorMap k_map, v_map, q_map;  // q_map: many rows only
   const void* q;
   void* out;
   float* lse;
@@ -61,13 +61,14 @@ struct AttentionParams {
   AttentionHeader* headers;
   float* partial;           // slots 2 * CTA (an item begun earlier) and 2 * CTA + 1 (one that goes on)
   uint32_t* status;
-  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box;
+  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box, item_rows;
   uint32_t causal, window, min_units, whole_items;
   float scale, scale_log2;  // of the scores; scale * log2(e)
 };
 struct AttentionPlan {  // how a call is launched: the same for every content of its device arrays
   bool many;            // the kernel for many rows
-  uint32_t rows, keys, padded_dim, ctas, least_units;
+  uint32_t rows, keys, padded_dim, ctas, least_units;  // rows: of a slot of the workspace
+  uint32_t item_rows;   // rows of an item, at most `rows`
   uint32_t box;         // token rows that one copy brings
   bool joins;           // an item may span CTAs: workspace and the second kernel are needed
   size_t workspace;
@@ -76,10 +77,8 @@ struct AttentionPlan {  // how a call is launched: the same for every content of
 inline size_t attention_slot_floats(const AttentionPlan& p) {
   return static_cast<size_t>(p.rows) * (2 + p.padded_dim);
 }
-size_t few_rows_smem(uint32_t padded_dim);
 cudaError_t prepare_few_rows();
 cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
-size_t many_rows_smem(uint32_t padded_dim);
 cudaError_t prepare_many_rows();
 cudaError_t launch_many_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);
 cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream);

@@ -75,6 +75,15 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       "l"(map), "r"(element), "r"(row), "r"(head), "r"(page), "r"(bar)
       : "memory");
 }
+// Box of 64 elements of the heads of a group x some tokens.
+__device__ __forceinline__ void load_queries(uint32_t dst, const CUtensorMap* map, int32_t element, int32_t head,
+                                             int32_t token, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(element), "r"(head), "r"(token), "r"(bar)
+      : "memory");
+}
 // The kernels are launched so that the next one's CTAs may be set up while the last one still runs:
 // nothing that an earlier kernel wrote is read, and nothing written, before earlier_done.
 __device__ __forceinline__ void earlier_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -108,34 +117,46 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ void copy_16(uint32_t dst, const void* src, bool wanted) {  // zeros where not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(wanted ? 16u : 0u) : "memory");
+}
+// One arrival when the copies that this thread has begun have landed.
+__device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // ------------------------------------------------------------------ division of the work
 struct Sequence {
   int32_t token, n, length;  // first new token, new tokens, keys
 };
 __device__ __forceinline__ Sequence load_sequence(const AttentionParams& P, uint32_t b) {
   const int32_t tokens = static_cast<int32_t>(P.tokens);
-  const int32_t s = min(max(P.indptr[b], 0), tokens);
-  const int32_t e = min(max(P.indptr[b + 1], s), tokens);
-  const int32_t l = min(max(P.lengths[b], 0), static_cast<int32_t>(P.capacity));
-  return Sequence{s, e - s, l};
+  const int32_t s0 = P.indptr[b], e0 = P.indptr[b + 1], l0 = P.lengths[b];
+  const int32_t s = min(max(s0, 0), tokens), e = min(max(e0, s), tokens);
+  return Sequence{s, e - s, min(max(l0, 0), static_cast<int32_t>(P.capacity))};
 }
 struct KeyRange {
-  int32_t begin, end;  // keys that some row of an item sees
+  int32_t begin, end;  // keys that some of the tokens see
 };
-template <int ROWS>
-__device__ __forceinline__ KeyRange key_range(const AttentionParams& P, const Sequence& s, uint32_t row_tile) {
+__device__ __forceinline__ KeyRange key_range(const AttentionParams& P, const Sequence& s, uint32_t first, uint32_t last) {
   KeyRange r{0, s.length};
   if (P.causal) {
-    const uint32_t first = row_tile * ROWS;
-    const uint32_t last = min(first + ROWS, static_cast<uint32_t>(s.n) * P.group) - 1u;
     const int32_t base = s.length - s.n;
-    r.end = max(0, base + static_cast<int32_t>(last / P.group) + 1);
+    r.end = max(0, base + static_cast<int32_t>(last) + 1);
     if (P.window) {
-      const int64_t b = static_cast<int64_t>(base) + first / P.group + 1 - static_cast<int64_t>(P.window);
+      const int64_t b = static_cast<int64_t>(base) + first + 1 - static_cast<int64_t>(P.window);
       r.begin = static_cast<int32_t>(max(static_cast<int64_t>(0), b));
     }
   }
   return r;
+}
+__device__ __forceinline__ uint32_t row_tiles(const AttentionParams& P, const Sequence& s) {
+  return (static_cast<uint32_t>(s.n) * P.group + P.item_rows - 1) / P.item_rows;
+}
+__device__ __forceinline__ KeyRange item_keys(const AttentionParams& P, const Sequence& s, uint32_t tile) {
+  const uint32_t first = tile * P.item_rows;
+  const uint32_t last = min(first + P.item_rows, static_cast<uint32_t>(s.n) * P.group) - 1u;
+  return key_range(P, s, first / P.group, last / P.group);
 }
 // Tiles of an item; one that sees no key has one all the same, in which its zeros are written.
 template <int KEYS>
@@ -144,112 +165,144 @@ __device__ __forceinline__ uint32_t item_tiles(const KeyRange& r) {
 }
 // Its units: as many, or one where no item is split.
 template <int KEYS>
-__device__ __forceinline__ uint32_t item_units(const AttentionParams& P, const KeyRange& r) {
-  return P.whole_items ? 1u : item_tiles<KEYS>(r);
+__device__ __forceinline__ uint32_t item_units(const AttentionParams& P, const Sequence& s, uint32_t tile) {
+  return P.whole_items ? 1u : item_tiles<KEYS>(item_keys(P, s, tile));
 }
-template <int ROWS>
-__device__ __forceinline__ uint32_t row_tiles(const AttentionParams& P, const Sequence& s) {
-  return (static_cast<uint32_t>(s.n) * P.group + ROWS - 1) / ROWS;
+// Units of one head of a sequence that is the same for the whole warp.
+template <int KEYS>
+__device__ __forceinline__ uint32_t head_units_warp(const AttentionParams& P, const Sequence& s, uint32_t tiles) {
+  uint32_t part = 0;
+  for (uint32_t t = threadIdx.x & 31u; t < tiles; t += 32u) part += item_units<KEYS>(P, s, t);
+  return __reduce_add_sync(0xffffffffu, part);
 }
-template <int ROWS, int KEYS>
-__device__ __forceinline__ uint64_t head_units(const AttentionParams& P, const Sequence& s) {
-  uint64_t u = 0;
-  const uint32_t tiles = row_tiles<ROWS>(P, s);
-  if (P.whole_items) return tiles;
-  for (uint32_t t = 0; t < tiles; ++t) u += item_units<KEYS>(P, key_range<ROWS>(P, s, t));
-  return u;
-}
-// Where a CTA's share begins, how long it is, and how all shares lie.
+// Where a CTA's share begins, how long it is, and how all shares lie: the first `longer` CTAs have
+// `each` + 1 units, the others `each`. The host has made sure that units are counted in 31 bits.
 struct Share {
-  uint64_t total;     // units of the call
-  uint64_t begin;     // first unit of this CTA
-  uint32_t units;     // units of this CTA
-  uint32_t ctas;      // CTAs that have a share
+  uint32_t units, begin, ctas, each, longer;
   uint32_t sequence, head, row_tile, skip;  // the item that holds the first unit, and its units before it
+  __device__ __forceinline__ uint32_t cta_of(uint32_t unit) const {
+    const uint32_t in_longer = (each + 1u) * longer;
+    return unit < in_longer ? unit / (each + 1u) : longer + (unit - in_longer) / each;
+  }
 };
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t ctas, uint32_t cta) {
-  return total * cta / ctas;
-}
-// Called by all THREADS threads of a CTA; `sums` has THREADS entries.
-template <int ROWS, int KEYS, int THREADS>
-__device__ __forceinline__ void find_share(const AttentionParams& P, uint64_t* sums, Share* share) {
-  const uint32_t t = threadIdx.x;
-  // sequences of this thread
-  const uint32_t each = (P.sequences + THREADS - 1) / THREADS;
-  const uint32_t b0 = min(t * each, P.sequences), b1 = min(b0 + each, P.sequences);
-  uint64_t mine = 0;
-  for (uint32_t b = b0; b < b1; ++b) mine += head_units<ROWS, KEYS>(P, load_sequence(P, b)) * P.kv_heads;
-  uint64_t upto = mine;  // inclusive sum over the warp, then over the warps
+// Called by all THREADS threads of a CTA; `sums` has an entry for each warp. A warp takes consecutive
+// sequences, its lanes too; sequences of many row tiles are summed up by the warp together.
+template <int KEYS, int THREADS>
+__device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* sums, Share* share) {
+  constexpr uint32_t kWarpsHere = THREADS / 32;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  const uint32_t per_warp = (P.sequences + kWarpsHere - 1) / kWarpsHere, each = (per_warp + 31u) / 32u;
+  const uint32_t end = min((warp + 1u) * per_warp, P.sequences);
+  const uint32_t b0 = warp * per_warp + lane * each;
+  uint32_t mine = 0;
+  Sequence s{0, 0, 0};
+  for (uint32_t i = 0; i < each; ++i) {
+    s = Sequence{0, 0, 0};
+    if (b0 + i < end) s = load_sequence(P, b0 + i);
+    const uint32_t tiles = row_tiles(P, s);
+    uint32_t u = 0;
+    if (tiles <= 2u)
+      for (uint32_t t = 0; t < tiles; ++t) u += item_units<KEYS>(P, s, t);
+    for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 2u); many; many &= many - 1u) {
+      const int from = __ffs(many) - 1;
+      const Sequence o{0, __shfl_sync(0xffffffffu, s.n, from), __shfl_sync(0xffffffffu, s.length, from)};
+      const uint32_t sum = head_units_warp<KEYS>(P, o, __shfl_sync(0xffffffffu, tiles, from));
+      if (static_cast<int>(lane) == from) u = sum;
+    }
+    mine += u * P.kv_heads;
+  }
+  uint32_t upto = mine;  // inclusive sum over the warp, then over the warps
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t o = __shfl_up_sync(0xffffffffu, upto, d);
-    if ((t & 31u) >= d) upto += o;
+    const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += o;
   }
-  if ((t & 31u) == 31u) sums[t >> 5] = upto;
-  if (t == 0) share->units = 0;
+  if (lane == 31u) sums[warp] = upto;
+  if (threadIdx.x == 0) share->units = 0;
   __syncthreads();
-  uint64_t total = 0;
+  uint32_t total = 0, before = 0;
 #pragma unroll
-  for (uint32_t w = 0; w < THREADS / 32; ++w) {
-    const uint64_t s = sums[w];
-    if (w < (t >> 5)) upto += s;
-    total += s;
+  for (uint32_t w = 0; w < kWarpsHere; ++w) {
+    const uint32_t x = sums[w];
+    if (w < warp) before += x;
+    total += x;
   }
-  const uint64_t want = (total + P.min_units - 1) / P.min_units;
-  const uint32_t ctas = want < gridDim.x ? static_cast<uint32_t>(want) : gridDim.x;
+  const uint32_t ctas = min(gridDim.x, (total + P.min_units - 1u) / P.min_units);
   if (blockIdx.x < ctas) {
-    const uint64_t u0 = share_begin(total, ctas, blockIdx.x), u1 = share_begin(total, ctas, blockIdx.x + 1);
-    uint64_t at = upto - mine;
-    if (u0 >= at && u0 < upto) {  // exactly one thread
-      uint32_t b = b0;
-      Sequence s = load_sequence(P, b);
-      uint64_t per_head = head_units<ROWS, KEYS>(P, s);
-      while (u0 >= at + per_head * P.kv_heads) {
-        at += per_head * P.kv_heads;
-        s = load_sequence(P, ++b);
-        per_head = head_units<ROWS, KEYS>(P, s);
-      }
-      const uint64_t head = (u0 - at) / per_head;
-      uint64_t left = u0 - at - head * per_head;
-      uint32_t tile = 0;
+    const uint32_t share_each = total / ctas, longer = total - share_each * ctas;
+    const uint32_t u0 = share_each * blockIdx.x + min(blockIdx.x, longer);
+    uint32_t at = before + upto - mine;
+    const uint32_t here = __ballot_sync(0xffffffffu, u0 >= at && u0 - at < mine);
+    if (here) {  // one lane of one warp; the warp goes on together
+      const int from = __ffs(here) - 1;
+      at = __shfl_sync(0xffffffffu, at, from);
+      uint32_t b = __shfl_sync(0xffffffffu, b0, from);
+      s.n = __shfl_sync(0xffffffffu, s.n, from);
+      s.length = __shfl_sync(0xffffffffu, s.length, from);
+      uint32_t per_head = 0;
       for (;;) {
-        const uint32_t u = item_units<KEYS>(P, key_range<ROWS>(P, s, tile));
-        if (left < u) break;
-        left -= u;
-        ++tile;
+        if (each > 1u) s = load_sequence(P, b);
+        per_head = head_units_warp<KEYS>(P, s, row_tiles(P, s));
+        if (u0 - at < per_head * P.kv_heads) break;
+        at += per_head * P.kv_heads;
+        ++b;
       }
-      share->total = total;
-      share->begin = u0;
-      share->ctas = ctas;
-      share->sequence = b;
-      share->head = static_cast<uint32_t>(head);
-      share->row_tile = tile;
-      share->skip = static_cast<uint32_t>(left);
-      share->units = static_cast<uint32_t>(u1 - u0);
+      const uint32_t head = (u0 - at) / per_head;
+      uint32_t left = u0 - at - head * per_head, tile = 0;
+      const uint32_t tiles = row_tiles(P, s);
+      for (uint32_t t0 = 0;; t0 += 32u) {
+        const uint32_t u = t0 + lane < tiles ? item_units<KEYS>(P, s, t0 + lane) : 0u;
+        uint32_t sum = u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const uint32_t o = __shfl_up_sync(0xffffffffu, sum, d);
+          if (lane >= d) sum += o;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, left < sum);
+        if (past) {
+          const int at_lane = __ffs(past) - 1;
+          tile = t0 + at_lane;
+          left -= __shfl_sync(0xffffffffu, sum - u, at_lane);
+          break;
+        }
+        left -= __shfl_sync(0xffffffffu, sum, 31);
+      }
+      if (lane == 0)
+        *share = Share{share_each + (blockIdx.x < longer ? 1u : 0u), u0, ctas, share_each, longer, b, head, tile, left};
     }
   }
   __syncthreads();
 }
-// Walks through the pieces of a share: what every role of a CTA does by itself.
-template <int ROWS, int KEYS>
-struct Pieces {
-  const AttentionParams& P;
-  Sequence s;
-  uint32_t b, head, tile, skip, left, tiles;
-  uint64_t at;
-  // the piece
-  KeyRange keys;
-  uint32_t first_tile, count, whole;  // key tiles first_tile .. first_tile + count - 1 of the item's `whole`
 
-  __device__ __forceinline__ Pieces(const AttentionParams& params, const Share& share)
-      : P(params), b(share.sequence), head(share.head), tile(share.row_tile), skip(share.skip),
-        left(share.units), at(share.begin) {
+// A part of a share that lies in one item: what the loading warp tells the others.
+struct Piece {
+  int32_t token, n, length;        // of the sequence
+  uint32_t head, first_row, rows;  // rows (token x group + head of the group) of the sequence
+  int32_t tile, count;             // key tiles tile .. tile + count - 1
+  int32_t keys_begin, keys_end;    // that some row of the item sees
+  uint32_t begins, ends;           // whether the item begins and ends in it
+  uint32_t valid;                  // 0: no more pieces
+  int32_t pad[3];
+  int32_t from[2], to[2];          // many rows: the key tiles from .. to - 1 that concern each of the two row tiles
+};
+// Walks through the pieces of a share; all lanes of the loading warp alike.
+template <int KEYS>
+struct Walker {
+  const AttentionParams& P;
+  const Share& share;
+  Sequence s;
+  uint32_t b, head, tile, skip, left, tiles, at, whole;
+  Piece piece;
+  __device__ __forceinline__ Walker(const AttentionParams& params, const Share& sh)
+      : P(params), share(sh), s{0, 0, 0}, b(sh.sequence), head(sh.head), tile(sh.row_tile), skip(sh.skip),
+        left(sh.units), tiles(0), at(sh.begin), whole(0), piece{} {
     if (left) {
       s = load_sequence(P, b);
-      tiles = row_tiles<ROWS>(P, s);
+      tiles = row_tiles(P, s);
     }
   }
   __device__ __forceinline__ bool next() {
+    piece.valid = left != 0;
     if (left == 0) return false;
     if (tile == tiles) {  // on to the next head, or the next sequence that has new tokens
       tile = 0;
@@ -258,34 +311,52 @@ struct Pieces {
         do {
           s = load_sequence(P, ++b);
         } while (s.n == 0);
-        tiles = row_tiles<ROWS>(P, s);
+        tiles = row_tiles(P, s);
       }
     }
-    keys = key_range<ROWS>(P, s, tile);
+    const KeyRange keys = item_keys(P, s, tile);
     whole = item_tiles<KEYS>(keys);
-    first_tile = (keys.end > keys.begin ? keys.begin / KEYS : 0u) + skip;
-    count = P.whole_items ? whole : min(whole - skip, left);
+    piece.token = s.token;
+    piece.n = s.n;
+    piece.length = s.length;
+    piece.head = head;
+    piece.first_row = tile * P.item_rows;
+    piece.rows = min(P.item_rows, static_cast<uint32_t>(s.n) * P.group - piece.first_row);
+    piece.tile = static_cast<int32_t>((keys.end > keys.begin ? keys.begin / KEYS : 0u) + skip);
+    piece.count = static_cast<int32_t>(P.whole_items ? whole : min(whole - skip, left));
+    piece.keys_begin = keys.begin;
+    piece.keys_end = keys.end;
+    piece.begins = skip == 0;
+    piece.ends = skip + piece.count == whole;
     return true;
   }
-  __device__ __forceinline__ bool begins() const { return skip == 0; }
-  __device__ __forceinline__ bool ends() const { return skip + count == whole; }
-  __device__ __forceinline__ uint32_t rows() const {
-    return min(static_cast<uint32_t>(ROWS), static_cast<uint32_t>(s.n) * P.group - tile * ROWS);
-  }
-  // CTAs behind this one that have more of the piece's item
-  __device__ __forceinline__ uint32_t more(const Share& share) const {
-    const uint64_t last = at + (whole - skip) - 1;  // the item's last unit
-    const uint64_t cta = ((last + 1) * share.ctas - 1) / share.total;
-    return static_cast<uint32_t>(cta) - blockIdx.x;
-  }
   __device__ __forceinline__ void done() {
-    const uint32_t units = P.whole_items ? 1u : count;
+    const uint32_t units = P.whole_items ? 1u : static_cast<uint32_t>(piece.count);
     left -= units;
     at += units;
     ++tile;
     skip = 0;
   }
+  // Behind the last piece: whether its item goes on, and in how many CTAs.
+  __device__ __forceinline__ void write_header() const {
+    AttentionHeader h{0, 0, 0, 0, 0, {0, 0, 0}};
+    if (share.units != 0 && piece.begins && !piece.ends) {
+      const uint32_t last = at + whole - static_cast<uint32_t>(piece.count) - 1u;  // the item's last unit
+      h = AttentionHeader{share.cta_of(last) - blockIdx.x, piece.rows, piece.first_row, piece.head,
+                          static_cast<uint32_t>(piece.token), {0, 0, 0}};
+    }
+    P.headers[blockIdx.x] = h;
+  }
 };
+__device__ __forceinline__ void put_piece(Piece* to, const Piece& p, uint32_t lane) {
+  if (lane != 0) return;
+  int4* d = reinterpret_cast<int4*>(to);
+  d[0] = make_int4(p.token, p.n, p.length, static_cast<int>(p.head));
+  d[1] = make_int4(static_cast<int>(p.first_row), static_cast<int>(p.rows), p.tile, p.count);
+  d[2] = make_int4(p.keys_begin, p.keys_end, static_cast<int>(p.begins), static_cast<int>(p.ends));
+  d[3] = make_int4(static_cast<int>(p.valid), 0, 0, 0);
+  d[4] = make_int4(p.from[0], p.from[1], p.to[0], p.to[1]);
+}
 
 // The warp that loads: boxes of a tile of keys, one lane each; page numbers are read a tile ahead.
 template <int KEYS, int HALVES>
@@ -296,10 +367,10 @@ struct TileLoader {
   int32_t page, row;
   bool wanted;
   __device__ __forceinline__ TileLoader(const AttentionParams& params)
-      : P(params), lane(threadIdx.x & 31u), boxes(KEYS / params.box) {}
-  __device__ __forceinline__ void look_up(uint32_t b, const KeyRange& keys, uint32_t tile) {
+      : P(params), lane(threadIdx.x & 31u), boxes(KEYS / params.box), page(-1), row(0), wanted(false) {}
+  __device__ __forceinline__ void look_up(uint32_t b, const Piece& piece, uint32_t tile) {
     const int32_t key = static_cast<int32_t>(tile * KEYS + lane * P.box);
-    wanted = lane < boxes && key < keys.end && key + static_cast<int32_t>(P.box) > keys.begin;
+    wanted = lane < boxes && key < piece.keys_end && key + static_cast<int32_t>(P.box) > piece.keys_begin;
     page = -1;
     row = 0;
     if (wanted) {

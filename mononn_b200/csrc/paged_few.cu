@@ -9,26 +9,38 @@
 namespace mononn {
 namespace paged {
 
-constexpr int kWarps = 4;  // that compute
-constexpr int kThreadsFew = (kWarps + 1) * 32;
-constexpr int kSlots = 4;  // of keys or values of one tile
+constexpr int kKeyGroups = 4;  // warps that share a row tile
+constexpr int kPieces = 2;     // told ahead
 
-template <int DIM>
-struct FewSmem {
+template <int DIM, int TILES>
+struct FewShape {
+  static constexpr int kRows = static_cast<int>(kFewRows) * TILES;
+  static constexpr int kWarps = kKeyGroups * TILES;  // that compute
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kCtas = TILES == 1 ? 2 : 1;   // of an SM
   static constexpr int kSlotBytes = static_cast<int>(kFewKeys) * DIM * 2;
+  // keys or values of one tile each
+  static constexpr int kSlots = (TILES == 1 ? 4 : TILES == 2 ? 8 : 6) * (128 / DIM);
   static constexpr int kPitch = DIM + 8;  // floats between rows of the warps' outputs: no bank conflicts
-  static constexpr int kOutputs = kSlots * kSlotBytes;
-  static constexpr int kControl = kOutputs + kWarps * static_cast<int>(kFewRows) * kPitch * 4;
-  static constexpr int kBytes = kControl + 1024;
+  static constexpr int kQueries = kSlots * kSlotBytes, kQueryBytes = kRows * DIM * 2;
+  static constexpr int kOutputs = kQueries + kPieces * kQueryBytes;
+  static constexpr int kControl = kOutputs + kKeyGroups * kRows * kPitch * 4;
+  static constexpr int kSmem = 1024 + kControl + 2304;
 };
+template <int DIM, int TILES>
 struct FewControl {
-  uint64_t full[kSlots], empty[kSlots];
-  uint64_t sums[8];
+  using S = FewShape<DIM, TILES>;
+  uint64_t full[S::kSlots], empty[S::kSlots], told[kPieces], taken[kPieces], meeting;
+  alignas(16) Piece pieces[kPieces];
   Share share;
+  uint32_t sums[S::kWarps + 1];
   uint32_t gave_up;
-  float maxima[kWarps][kFewRows], totals[kWarps][kFewRows];
+  float maxima[kKeyGroups][S::kRows], totals[kKeyGroups][S::kRows];
 };
-static_assert(sizeof(FewControl) <= 1024, "control block");
+static_assert(sizeof(FewControl<64, 1>) <= 2304 && sizeof(FewControl<64, 2>) <= 2304 && sizeof(FewControl<64, 3>) <= 2304 &&
+                  sizeof(FewControl<128, 3>) <= 2304, "control block");
+static_assert(FewShape<128, 1>::kSmem <= 113 * 1024 && FewShape<128, 2>::kSmem <= 227 * 1024 &&
+                  FewShape<128, 3>::kSmem <= 227 * 1024 && FewShape<64, 1>::kSmem <= 113 * 1024, "shared memory");
 
 __device__ __forceinline__ void matrices_4(uint32_t address, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -61,16 +73,25 @@ __device__ __forceinline__ void multiply<__nv_bfloat16>(float (&c)[4], const uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+// The warps that compute, bounded like every other wait.
+__device__ __forceinline__ bool warps_meet(uint32_t bar, uint32_t& phase, volatile uint32_t* gave_up) {
+  __syncwarp();
+  if ((threadIdx.x & 31u) == 0u) barrier_arrive(bar);
+  const bool fine = barrier_wait_warp(bar, phase, gave_up);
+  phase ^= 1u;
+  return fine;
+}
 
-template <typename T, int DIM>
-__global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_constant__ AttentionParams P) {
+template <typename T, int DIM, int TILES>
+__global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, TILES>::kCtas)
+    few_rows_kernel(const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t raw[];
-  using M = FewSmem<DIM>;
-  constexpr int kHalves = DIM / 64;
-  constexpr int kSteps = DIM / 16;
+  using S = FewShape<DIM, TILES>;
+  constexpr int kHalves = DIM / 64, kSteps = DIM / 16, kSlots = S::kSlots, kWarps = S::kWarps, kRows = S::kRows;
+  // 13 warps leave 128 registers a thread: queries are read again for every tile of keys then
+  constexpr bool kHoldQueries = TILES < 3 || DIM == 64;
   uint8_t* smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
-  FewControl& C = *reinterpret_cast<FewControl*>(smem + M::kControl);
+  auto& C = *reinterpret_cast<FewControl<DIM, TILES>*>(smem + S::kControl);
   const uint32_t slots = smem_address(smem);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -79,6 +100,11 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
       barrier_init(smem_address(&C.full[i]), 1);
       barrier_init(smem_address(&C.empty[i]), kWarps);
     }
+    for (int i = 0; i < kPieces; ++i) {
+      barrier_init(smem_address(&C.told[i]), 33);
+      barrier_init(smem_address(&C.taken[i]), kWarps);
+    }
+    barrier_init(smem_address(&C.meeting), kWarps);
     C.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));
@@ -86,60 +112,82 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
   }
   let_next_begin();
   earlier_done();
-  find_share<kFewRows, kFewKeys, kThreadsFew>(P, C.sums, &C.share);  // a barrier of the CTA within
-  const Share& share = C.share;
-  Pieces<kFewRows, kFewKeys> piece(P, share);
-
+  find_share<kFewKeys, S::kThreads>(P, C.sums, &C.share);  // barriers of the CTA within
   uint32_t fills = 0;  // of the loading warp
+
   if (warp == kWarps) {
     TileLoader<kFewKeys, kHalves> loader(P);
+    Walker<kFewKeys> walk(P, C.share);
     bool fine = true;
-    while (fine && piece.next()) {
-      loader.look_up(piece.b, piece.keys, piece.first_tile);
-      for (uint32_t u = 0; fine && u < piece.count; ++u) {
+    for (uint32_t i = 0; fine; ++i) {
+      const bool some = walk.next();
+      if (some) loader.look_up(walk.b, walk.piece, walk.piece.tile);
+      const uint32_t at = i % kPieces, told = smem_address(&C.told[at]);
+      fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
+      if (!fine) break;
+      if (some) {  // the queries of the piece, consecutive lanes along a row
+        constexpr uint32_t kParts = DIM / 8;
+        const uint32_t tile = slots + S::kQueries + at * S::kQueryBytes;
+#pragma unroll 4
+        for (uint32_t j = lane; j < kRows * kParts; j += 32) {
+          const uint32_t row = j / kParts, part = j % kParts, g = walk.piece.first_row + row, token = g / P.group;
+          const bool wanted = row < walk.piece.rows && part * 8 < P.head_dim;
+          const T* src = static_cast<const T*>(P.q);
+          if (wanted)
+            src += (walk.piece.token + static_cast<int64_t>(token)) * P.q_token +
+                   static_cast<int64_t>(walk.piece.head * P.group + g - token * P.group) * P.q_head + part * 8;
+          copy_16(tile + (part >> 3) * (kRows * 128) + row * 128 + (((part & 7u) ^ (row & 7u)) << 4), src, wanted);
+        }
+      }
+      put_piece(&C.pieces[at], walk.piece, lane);
+      arrive_after_copies(told);
+      if (lane == 0) barrier_arrive(told);
+      if (!some) break;
+      for (int32_t u = 0; fine && u < walk.piece.count; ++u) {
         const TileLoader<kFewKeys, kHalves> now = loader;
-        if (u + 1 < piece.count) loader.look_up(piece.b, piece.keys, piece.first_tile + u + 1);
+        if (u + 1 < walk.piece.count) loader.look_up(walk.b, walk.piece, walk.piece.tile + u + 1);
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t slot = fills % kSlots;
           fine = fine && barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kSlots) & 1u) ^ 1u, &C.gave_up);
           if (!fine) break;
-          now.load(kv ? &P.v_map : &P.k_map, slots + slot * M::kSlotBytes, piece.head, smem_address(&C.full[slot]));
+          now.load(kv ? &P.v_map : &P.k_map, slots + slot * S::kSlotBytes, walk.piece.head, smem_address(&C.full[slot]));
           ++fills;
         }
       }
-      piece.done();
+      walk.done();
     }
+    if (lane == 0 && P.headers) walk.write_header();
   } else {
     const float ninf = __int_as_float(0xff800000);
-    uint32_t slot = 0, parity = 0;
-    float* const outputs = reinterpret_cast<float*>(smem + M::kOutputs);
+    uint32_t slot = 0, parity = 0, meetings = 0;
+    float* const outputs = reinterpret_cast<float*>(smem + S::kOutputs);
+    const uint32_t group = warp % kKeyGroups, row_tile = warp / kKeyGroups;
     // ldmatrix addresses: lanes 0-7, 8-15, .. point at the rows of the four 8 x 8 matrices
-    const uint32_t key_row = warp * 16 + (lane & 7u) + ((lane >> 4) << 3), key_chunk = (lane >> 3) & 1u;
-    const uint32_t val_row = warp * 16 + (lane & 15u), val_chunk = lane >> 4;
-    AttentionHeader header{0, 0, 0, 0, 0, {0, 0, 0}};
-    // After a wait that gave up the remaining ones end at once, and the warps still meet everywhere.
-    while (piece.next()) {
-      const uint32_t rows = piece.rows();
-      // queries: rows lane / 4 and + 8 of the 16, two elements of each 8
-      uint32_t q[kSteps][4];
+    const uint32_t key_row = group * 16 + (lane & 7u) + ((lane >> 4) << 3), key_chunk = (lane >> 3) & 1u;
+    const uint32_t val_row = group * 16 + (lane & 15u), val_chunk = lane >> 4;
+    const uint32_t query_row = row_tile * 16 + (lane & 15u), query_chunk = lane >> 4;
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t at = n % kPieces;
+      if (!barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up)) break;
+      const Piece& piece = C.pieces[at];
+      if (piece.valid == 0) break;
+      const int32_t count = piece.count, tile0 = piece.tile, keys_begin = piece.keys_begin, keys_end = piece.keys_end;
+      const uint32_t queries = slots + S::kQueries + at * S::kQueryBytes + query_row * 128;
+      auto query = [&](int k, uint32_t (&r)[4]) {
+        matrices_4(queries + (k >> 2) * (kRows * 128) + ((((k & 3) * 2 + query_chunk) ^ (query_row & 7u)) << 4), r);
+      };
+      uint32_t held[kHoldQueries ? kSteps : 1][4];
+      if constexpr (kHoldQueries) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) query(k, held[k]);
+      }
       int32_t see_from[2], see_to[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t r = (lane >> 2) + 8 * i;
-        const uint32_t row = piece.tile * kFewRows + r;
-        const uint32_t token = row / P.group, head = piece.head * P.group + row % P.group;
-        const bool valid = r < rows;
-        const T* src = static_cast<const T*>(P.q) + (piece.s.token + static_cast<int64_t>(token)) * P.q_token +
-                       static_cast<int64_t>(head) * P.q_head;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t d = k * 16 + j * 8 + (lane & 3u) * 2;
-            q[k][j * 2 + i] = valid && d < P.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-          }
-        const int32_t position = piece.s.length - piece.s.n + static_cast<int32_t>(token);
-        see_to[i] = valid ? (P.causal ? max(position + 1, 0) : piece.s.length) : 0x7fffffff;
+        const uint32_t r = row_tile * 16 + (lane >> 2) + 8 * i;
+        const bool valid = r < piece.rows;
+        const int32_t position = piece.length - piece.n + static_cast<int32_t>((piece.first_row + r) / P.group);
+        see_to[i] = valid ? (P.causal ? max(position + 1, 0) : piece.length) : 0x7fffffff;
         see_from[i] = 0;
         if (valid && P.causal && P.window)
           see_from[i] = static_cast<int32_t>(max(static_cast<int64_t>(0), position + 1 - static_cast<int64_t>(P.window)));
@@ -147,6 +195,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
       // keys that every row sees need no test
       const int32_t all_from = __reduce_max_sync(0xffffffffu, max(see_from[0], see_from[1]));
       const int32_t all_to = __reduce_min_sync(0xffffffffu, min(see_to[0], see_to[1]));
+      const bool idle = row_tile * 16 >= piece.rows;
 
       float acc[kSteps * 2][4];
 #pragma unroll
@@ -155,9 +204,9 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
         for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
       float m[2] = {ninf, ninf}, l[2] = {0.f, 0.f};
 
-      for (uint32_t u = 0; u < piece.count; ++u) {
-        const int32_t key0 = static_cast<int32_t>((piece.first_tile + u) * kFewKeys + warp * 16);
-        const bool any = key0 < piece.keys.end && key0 + 16 > piece.keys.begin;
+      for (int32_t u = 0; u < count; ++u) {
+        const int32_t key0 = (tile0 + u) * static_cast<int32_t>(kFewKeys) + static_cast<int32_t>(group) * 16;
+        const bool any = !idle && key0 < keys_end && key0 + 16 > keys_begin;
         const bool tested = key0 < all_from || key0 + 16 > all_to;
         float s[2][4];
 #pragma unroll
@@ -166,14 +215,17 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
           for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
         if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
         if (any) {
-          const uint32_t base = slots + slot * M::kSlotBytes + key_row * 128;
+          const uint32_t base = slots + slot * S::kSlotBytes + key_row * 128;
 #pragma unroll
           for (int k = 0; k < kSteps; ++k) {
             uint32_t b[4];
             const uint32_t chunk = (k & 3) * 2 + key_chunk;
             matrices_4(base + (k >> 2) * kFewKeys * 128 + ((chunk ^ (key_row & 7u)) << 4), b);
-            multiply<T>(s[0], q[k], b[0], b[1]);
-            multiply<T>(s[1], q[k], b[2], b[3]);
+            uint32_t fresh[4];
+            if constexpr (!kHoldQueries) query(k, fresh);
+            const uint32_t(&q)[4] = kHoldQueries ? held[kHoldQueries ? k : 0] : fresh;
+            multiply<T>(s[0], q, b[0], b[1]);
+            multiply<T>(s[1], q, b[2], b[3]);
           }
         }
         __syncwarp();
@@ -232,16 +284,16 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
         }
         if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
         if (any) {
-          const uint32_t base = slots + slot * M::kSlotBytes + val_row * 128;
+          const uint32_t base = slots + slot * S::kSlotBytes + val_row * 128;
           // value rows that no row of the item sees may hold anything: 0 x NaN is not 0
-          const bool clear = key0 < piece.keys.begin || key0 + 16 > piece.keys.end;
+          const bool clear = key0 < keys_begin || key0 + 16 > keys_end;
           uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
           if (clear) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const int32_t key = key0 + i * 8 + (lane & 3u) * 2;
-              const bool a = key >= piece.keys.begin && key < piece.keys.end;
-              const bool b = key + 1 >= piece.keys.begin && key + 1 < piece.keys.end;
+              const bool a = key >= keys_begin && key < keys_end;
+              const bool b = key + 1 >= keys_begin && key + 1 < keys_end;
               keep[i] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
             }
           }
@@ -259,52 +311,52 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
         if (++slot == kSlots) slot = 0, parity ^= 1u;
       }
 
-      // the four warps' results of this piece
+      // the results of the warps that share a row tile
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       }
-      warps_meet();  // the last piece's have been read
+      const uint32_t rows = piece.rows;
+      if (!warps_meet(smem_address(&C.meeting), meetings, &C.gave_up)) break;  // the last piece's have been read
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t row = (lane >> 2) + 8 * r;
+        const uint32_t row = row_tile * 16 + (lane >> 2) + 8 * r;
         if (row < rows) {
           if ((lane & 3u) == 0) {
-            C.maxima[warp][row] = m[r];
-            C.totals[warp][row] = l[r];
+            C.maxima[group][row] = m[r];
+            C.totals[group][row] = l[r];
           }
-          float* to = outputs + (warp * kFewRows + row) * M::kPitch + (lane & 3u) * 2;
+          float* to = outputs + (group * kRows + row) * S::kPitch + (lane & 3u) * 2;
 #pragma unroll
           for (int i = 0; i < kSteps * 2; ++i)
             *reinterpret_cast<float2*>(to + i * 8) = make_float2(acc[i][r * 2], acc[i][r * 2 + 1]);
         }
       }
-      warps_meet();
-      const bool complete = piece.begins() && piece.ends();
+      if (!warps_meet(smem_address(&C.meeting), meetings, &C.gave_up)) break;
+      const bool complete = piece.begins && piece.ends;
       float* slot_out = nullptr;
       if (!complete)
-        slot_out = P.partial + (2u * blockIdx.x + (piece.begins() ? 1u : 0u)) *
-                                   static_cast<size_t>(kFewRows * (2 + DIM));
+        slot_out = P.partial + (2u * blockIdx.x + (piece.begins ? 1u : 0u)) * static_cast<size_t>(kRows * (2 + DIM));
       for (uint32_t i = threadIdx.x; i < rows * (DIM / 8); i += kWarps * 32) {
         const uint32_t row = i / (DIM / 8), d = (i % (DIM / 8)) * 8;
         float top = C.maxima[0][row];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, C.maxima[w][row]);
+        for (int w = 1; w < kKeyGroups; ++w) top = fmaxf(top, C.maxima[w][row]);
         float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kKeyGroups; ++w) {
           const float mw = C.maxima[w][row];
           const float f = mw == ninf ? 0.f : exp2_fast((mw - top) * P.scale_log2);
           sum += f * C.totals[w][row];
-          const float4* from = reinterpret_cast<const float4*>(outputs + (w * kFewRows + row) * M::kPitch + d);
+          const float4* from = reinterpret_cast<const float4*>(outputs + (w * kRows + row) * S::kPitch + d);
           const float4 a = from[0], b = from[1];
           o[0] += f * a.x; o[1] += f * a.y; o[2] += f * a.z; o[3] += f * a.w;
           o[4] += f * b.x; o[5] += f * b.y; o[6] += f * b.z; o[7] += f * b.w;
         }
         if (complete) {
-          const uint32_t g = piece.tile * kFewRows + row;
-          const int64_t token = piece.s.token + static_cast<int64_t>(g / P.group);
+          const uint32_t g = piece.first_row + row;
+          const int64_t token = piece.token + static_cast<int64_t>(g / P.group);
           const uint32_t head = piece.head * P.group + g % P.group;
           const float inverse = sum == 0.f ? 0.f : 1.f / sum;
           if (d < P.head_dim) {
@@ -323,20 +375,18 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
             slot_out[row * 2] = top;
             slot_out[row * 2 + 1] = sum;
           }
-          float4* to = reinterpret_cast<float4*>(slot_out + kFewRows * 2 + row * DIM + d);
+          float4* to = reinterpret_cast<float4*>(slot_out + kRows * 2 + row * DIM + d);
           to[0] = make_float4(o[0], o[1], o[2], o[3]);
           to[1] = make_float4(o[4], o[5], o[6], o[7]);
         }
       }
-      if (piece.begins() && !piece.ends())
-        header = AttentionHeader{piece.more(share), rows, piece.tile * kFewRows, piece.head,
-                                 static_cast<uint32_t>(piece.s.token), {0, 0, 0}};
-      piece.done();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
-    if (threadIdx.x == 0 && P.headers) P.headers[blockIdx.x] = header;
   }
   __syncthreads();
   if (C.gave_up && warp == kWarps) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
     for (uint32_t f = fills > kSlots ? fills - kSlots : 0u; f < fills; ++f)
       barrier_wait_out(smem_address(&C.full[f % kSlots]), (f / kSlots) & 1u);
     if (lane == 0) atomicExch(P.status, 1u);
@@ -428,50 +478,52 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
 static __device__ uint32_t g_status;
 cudaError_t paged_status_word(uint32_t** out) { return cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_status); }
 
-size_t few_rows_smem(uint32_t padded_dim) {
-  return 1024 + (padded_dim == 64 ? paged::FewSmem<64>::kBytes : paged::FewSmem<128>::kBytes);
-}
-
 namespace {
+// f(kernel, its shape) for the type, the padded head size and the row tiles of a call
+template <typename T, int DIM, typename F>
+cudaError_t with_tiles(uint32_t tiles, F&& f) {
+  if (tiles == 1) return f(paged::few_rows_kernel<T, DIM, 1>, paged::FewShape<DIM, 1>());
+  if (tiles == 2) return f(paged::few_rows_kernel<T, DIM, 2>, paged::FewShape<DIM, 2>());
+  return f(paged::few_rows_kernel<T, DIM, 3>, paged::FewShape<DIM, 3>());
+}
 template <typename F>
-cudaError_t with_type(bool bf16, uint32_t dim, F&& f) {
-  if (bf16) return dim == 64 ? f(__nv_bfloat16(), paged::FewSmem<64>()) : f(__nv_bfloat16(), paged::FewSmem<128>());
-  return dim == 64 ? f(__half(), paged::FewSmem<64>()) : f(__half(), paged::FewSmem<128>());
+cudaError_t with_kernel(bool bf16, uint32_t dim, uint32_t tiles, F&& f) {
+  if (bf16) return dim == 64 ? with_tiles<__nv_bfloat16, 64>(tiles, f) : with_tiles<__nv_bfloat16, 128>(tiles, f);
+  return dim == 64 ? with_tiles<__half, 64>(tiles, f) : with_tiles<__half, 128>(tiles, f);
+}
+template <typename T, int DIM>
+cudaError_t join(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
+  auto go = [&](auto kernel, uint32_t rows, uint32_t parts) {
+    return launch_dependent(kernel, dim3(plan.ctas, rows * parts / paged::kJoinWarps), paged::kJoinWarps * 32, 0, p, stream);
+  };
+  switch (plan.rows) {
+    case 16: return go(paged::join_kernel<T, DIM, 16, 8>, 16, 8);
+    case 32: return go(paged::join_kernel<T, DIM, 32, 4>, 32, 4);
+    case 48: return go(paged::join_kernel<T, DIM, 48, 4>, 48, 4);
+    default: return go(paged::join_kernel<T, DIM, static_cast<int>(kManyRows), 1>, kManyRows, 1);
+  }
 }
 }  // namespace
 
 cudaError_t prepare_few_rows() {
   for (int bf16 = 0; bf16 < 2; ++bf16)
-    for (uint32_t dim : {64u, 128u}) {
-      const cudaError_t e = with_type(bf16 != 0, dim, [&](auto t, auto m) {
-        using T = decltype(t);
-        constexpr int kDim = decltype(m)::kPitch - 8;
-        return cudaFuncSetAttribute(paged::few_rows_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(few_rows_smem(kDim)));
-      });
-      if (e != cudaSuccess) return e;
-    }
+    for (uint32_t dim : {64u, 128u})
+      for (uint32_t tiles = 1; tiles <= kFewTilesMost; ++tiles) {
+        const cudaError_t e = with_kernel(bf16 != 0, dim, tiles, [](auto kernel, auto shape) {
+          return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(shape)::kSmem);
+        });
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
-  return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
-    using T = decltype(t);
-    constexpr int kDim = decltype(m)::kPitch - 8;
-    return launch_dependent(paged::few_rows_kernel<T, kDim>, dim3(plan.ctas), paged::kThreadsFew, few_rows_smem(kDim), p, stream);
+  return with_kernel(bf16, plan.padded_dim, plan.rows / kFewRows, [&](auto kernel, auto shape) {
+    return launch_dependent(kernel, dim3(plan.ctas), decltype(shape)::kThreads, decltype(shape)::kSmem, p, stream);
   });
 }
 cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
-  return with_type(bf16, plan.padded_dim, [&](auto t, auto m) {
-    using T = decltype(t);
-    constexpr int kDim = decltype(m)::kPitch - 8;
-    constexpr int kFew = static_cast<int>(kFewRows), kMany = static_cast<int>(kManyRows);
-    constexpr uint32_t kParts = 4, kRowsHere = paged::kJoinWarps / kParts;
-    if (plan.rows == kFewRows)
-      return launch_dependent(paged::join_kernel<T, kDim, kFew, kParts>, dim3(plan.ctas, kFew / kRowsHere),
-                              paged::kJoinWarps * 32, 0, p, stream);
-    return launch_dependent(paged::join_kernel<T, kDim, kMany, 1>, dim3(plan.ctas, kMany / paged::kJoinWarps),
-                            paged::kJoinWarps * 32, 0, p, stream);
-  });
+  if (bf16) return plan.padded_dim == 64 ? join<__nv_bfloat16, 64>(p, plan, stream) : join<__nv_bfloat16, 128>(p, plan, stream);
+  return plan.padded_dim == 64 ? join<__half, 64>(p, plan, stream) : join<__half, 128>(p, plan, stream);
 }
 
 }  // namespace mononn

@@ -15,30 +15,33 @@
 namespace mononn {
 namespace paged {
 
-constexpr int kTileRows = 128;
 constexpr int kRows = static_cast<int>(kManyRows), kKeys = static_cast<int>(kManyKeys);
 constexpr int kThreadsMany = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 9;  // 10 and 11 only make up the group whose registers go to the others
-constexpr uint32_t kSoftmaxRegisters = 200, kOtherRegisters = 104, kLaunchRegisters = 168;
+constexpr int kPieces = 4;                  // told ahead
+constexpr uint32_t kSoftmaxRegisters = 216, kOtherRegisters = 72, kLaunchRegisters = 168;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreadsMany * kLaunchRegisters, "register split");
 constexpr float kRise = 8.0f;  // in powers of two
 
 template <int DIM>
 struct ManySmem {
-  static constexpr int kTileBytes = kTileRows * DIM * 2;  // of queries, keys or values
-  static constexpr int kSlots = DIM == 64 ? 8 : 5;
+  static constexpr int kTileBytes = static_cast<int>(kTileRows) * DIM * 2;  // of queries, keys or values
+  static constexpr int kSlots = DIM == 64 ? 8 : 4;
   static constexpr int kRing = 2 * kTileBytes;
-  static constexpr int kControl = kRing + kSlots * kTileBytes;
-  static constexpr int kBytes = kControl + 512;
+  static constexpr int kStage = kRing + kSlots * kTileBytes;  // 4 KB of each softmax warp, for its rows' way out
+  static constexpr int kControl = kStage + 8 * 4096;
+  static constexpr int kBytes = kControl + 1024;
 };
 struct ManyControl {
   uint64_t full[8], empty[8];
-  uint64_t scores[2], probabilities[2], queries[2], outputs[2], drained;
-  uint64_t sums[12];
+  uint64_t scores[2], probabilities[2], queries[2], queries_free[2], outputs[2], told[kPieces], taken[kPieces], drained;
+  alignas(16) Piece pieces[kPieces];
   Share share;
+  uint32_t sums[12];
   uint32_t gave_up, tmem;
 };
-static_assert(sizeof(ManyControl) <= 512, "control block");
+static_assert(sizeof(ManyControl) <= 1024, "control block");
+static_assert(ManySmem<128>::kBytes + 1024 <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -94,6 +97,15 @@ __device__ __forceinline__ void loads_done(uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : MONONN_P8(r, 0), MONONN_P8(r, 8), MONONN_P8(r, 16), MONONN_P8(r, 24)::"memory");
 }
+// The registers of a load that an earlier wait covered: nothing that uses them moves before it.
+__device__ __forceinline__ void loaded(uint32_t* r) {
+  asm volatile("" : MONONN_P8(r, 0), MONONN_P8(r, 8), MONONN_P8(r, 16), MONONN_P8(r, 24)::"memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // the same for 16 columns
 __device__ __forceinline__ void load_columns_16(uint32_t address, uint32_t* r) {
   asm volatile(
@@ -122,20 +134,19 @@ __device__ __forceinline__ void hide(uint32_t* s, int first, int32_t to, int32_t
     if (first + j < to || first + j >= from) s[j] = 0xff800000u;
 }
 
-// What a row tile of a piece has to do: units from .. to - 1 hold keys that some of its rows see.
-struct TileRange {
-  int32_t from, to;
-  __device__ __forceinline__ bool has(int32_t unit) const { return unit >= from && unit < to; }
-};
-__device__ __forceinline__ TileRange tile_range(const AttentionParams& P, const Pieces<kRows, kKeys>& piece, uint32_t t) {
-  TileRange r{0, 0};
-  if (t * kTileRows >= piece.rows()) return r;
-  const KeyRange k = key_range<kTileRows>(P, piece.s, piece.tile * 2 + t);
-  if (k.end <= k.begin) return r;
-  r.from = max(static_cast<int32_t>(piece.first_tile), k.begin / kKeys);
-  r.to = min(static_cast<int32_t>(piece.first_tile + piece.count), (k.end + kKeys - 1) / kKeys);
-  if (r.to < r.from) r.to = r.from;
-  return r;
+// The key tiles of a piece that hold keys which some row of row tile t sees.
+__device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
+  const uint32_t half = P.item_rows / 2;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    p.from[t] = p.to[t] = 0;
+    if (t * half >= p.rows) continue;
+    const uint32_t first = p.first_row + t * half, last = p.first_row + min((t + 1) * half, p.rows) - 1u;
+    const KeyRange k = key_range(P, Sequence{p.token, p.n, p.length}, first / P.group, last / P.group);
+    if (k.end <= k.begin) continue;
+    p.from[t] = max(p.tile, k.begin / kKeys);
+    p.to[t] = max(p.from[t], min(p.tile + p.count, (k.end + kKeys - 1) / kKeys));
+  }
 }
 
 template <typename T, int DIM>
@@ -156,14 +167,20 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     for (int t = 0; t < 2; ++t) {
       barrier_init(smem_address(&C.scores[t]), 1);
       barrier_init(smem_address(&C.probabilities[t]), 4);
-      barrier_init(smem_address(&C.queries[t]), 4);
+      barrier_init(smem_address(&C.queries[t]), 1);
+      barrier_init(smem_address(&C.queries_free[t]), 1);
       barrier_init(smem_address(&C.outputs[t]), 1);
+    }
+    for (int i = 0; i < kPieces; ++i) {
+      barrier_init(smem_address(&C.told[i]), 1);
+      barrier_init(smem_address(&C.taken[i]), 9);  // the softmax warps and the one that issues the products
     }
     barrier_init(smem_address(&C.drained), 1);
     C.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.v_map));
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&P.q_map));
   }
   let_next_begin();
   earlier_done();
@@ -172,45 +189,78 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     before_sync();
   }
-  find_share<kRows, kKeys, kThreadsMany>(P, C.sums, &C.share);  // barriers of the CTA within
+  find_share<kKeys, kThreadsMany>(P, C.sums, &C.share);  // barriers of the CTA within
   after_sync();
   const uint32_t tmem = *const_cast<volatile uint32_t*>(&C.tmem);
-  const Share& share = C.share;
-  Pieces<kRows, kKeys> piece(P, share);
-  AttentionHeader header{0, 0, 0, 0, 0, {0, 0, 0}};
-  uint32_t fills = 0;
+  uint32_t fills = 0;  // of the loading warp
   bool fine = true;
-
-  if (warp >= kMmaWarp)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-  else
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-
+  // Each group of warps within its own branch: code behind a meeting of both is held to the fewer registers.
+  if (warp >= kMmaWarp) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
   if (warp == kLoadWarp) {
     TileLoader<kKeys, kHalves> loader(P);
-    while (fine && piece.next()) {
-      loader.look_up(piece.b, piece.keys, piece.first_tile);
-      for (uint32_t u = 0; fine && u < piece.count; ++u) {
+    Walker<kKeys> walk(P, C.share);
+    const uint32_t half = P.item_rows / 2, half_tokens = half / P.group;
+    uint32_t query_loads[2] = {0, 0};
+    for (uint32_t i = 0; fine; ++i) {
+      const bool some = walk.next();
+      if (some) {
+        loader.look_up(walk.b, walk.piece, walk.piece.tile);
+        set_ranges(P, walk.piece);
+      }
+      const uint32_t at = i % kPieces;
+      fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
+      if (!fine) break;
+      put_piece(&C.pieces[at], walk.piece, lane);
+      if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
+      __syncwarp();
+      if (!some) break;
+      for (int32_t u = 0; fine && u < walk.piece.count; ++u) {
         const TileLoader<kKeys, kHalves> now = loader;
-        if (u + 1 < piece.count) loader.look_up(piece.b, piece.keys, piece.first_tile + u + 1);
+        if (u + 1 < walk.piece.count) loader.look_up(walk.b, walk.piece, walk.piece.tile + u + 1);
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t slot = fills % kSlots;
           fine = fine && barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kSlots) & 1u) ^ 1u, &C.gave_up);
           if (!fine) break;
-          now.load(kv ? &P.v_map : &P.k_map, ring + slot * M::kTileBytes, piece.head, smem_address(&C.full[slot]));
+          now.load(kv ? &P.v_map : &P.k_map, ring + slot * M::kTileBytes, walk.piece.head, smem_address(&C.full[slot]));
           ++fills;
+          if (u == 0 && kv == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (walk.piece.to[t] <= walk.piece.from[t]) continue;
+              fine = fine && barrier_wait_warp(smem_address(&C.queries_free[t]), (query_loads[t] & 1u) ^ 1u, &C.gave_up);
+              if (!fine) break;
+              ++query_loads[t];
+              if (lane == 0) {
+                const uint32_t bar = smem_address(&C.queries[t]);
+                barrier_arrive_bytes(bar, half * 128u * kHalves);
+                const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+                  load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
+                               static_cast<int32_t>(walk.piece.head * P.group), token, bar);
+              }
+              __syncwarp();
+            }
+          }
         }
       }
-      piece.done();
+      walk.done();
     }
+    if (lane == 0 && P.headers) walk.write_header();
   } else if (warp == kMmaWarp) {
     uint32_t used = 0;               // ring slots taken before this piece
     uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0};
     const bool issuer = elected();
     constexpr uint32_t kScores = instruction<T>(kKeys, false), kOutput = instruction<T>(DIM, true);
-    while (fine && piece.next()) {
-      const TileRange range[2] = {tile_range(P, piece, 0), tile_range(P, piece, 1)};
-      const int32_t first = static_cast<int32_t>(piece.first_tile), end = first + static_cast<int32_t>(piece.count);
+    for (uint32_t n = 0; fine; ++n) {
+      const uint32_t at = n % kPieces;
+      fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
+      const Piece& piece = C.pieces[at];
+      if (!fine || piece.valid == 0) break;
+      const int32_t first = piece.tile, end = first + piece.count;
+      const int32_t from[2] = {piece.from[0], piece.from[1]}, to[2] = {piece.to[0], piece.to[1]};
+      const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
       // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
       for (int32_t u = first - 1; fine && u < end; ++u) {
         const uint32_t v_fill = used + 2u * static_cast<uint32_t>(u - first) + 1u, k_fill = v_fill + 1u;
@@ -220,12 +270,11 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           if (!fine) break;
           // value rows that no row sees may hold anything: 0 x NaN is not 0
           const int32_t key0 = u * kKeys;
-          if (key0 < piece.keys.begin || key0 + kKeys > piece.keys.end) {
-            const int32_t from = piece.keys.begin - key0, to = piece.keys.end - key0;
+          if (key0 < keys_begin || key0 + kKeys > keys_end) {
             uint8_t* const tile = smem + M::kRing + slot * M::kTileBytes;
             for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
               const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
-              if (r < from || r >= to) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+              if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
             }
             shared_to_async();
             __syncwarp();
@@ -238,7 +287,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const uint32_t s = tmem + t * 128, o = tmem + 256 + t * 128;
-          if (u >= first && range[t].has(u)) {
+          if (u >= from[t] && u < to[t]) {
             fine = fine && barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up);
             if (!fine) break;
             probability_phase[t] ^= 1u;
@@ -247,13 +296,13 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               const uint64_t v = operand(ring + (v_fill % kSlots) * M::kTileBytes, kKeys * 128 / 16);
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
-                product_tensor(o, s + k * 8, v + k * (16 * 128 / 16), kOutput, k > 0 || u > range[t].from);
-              if (u + 1 == range[t].to) commit(smem_address(&C.outputs[t]));
+                product_tensor(o, s + k * 8, v + k * (16 * 128 / 16), kOutput, k > 0 || u > from[t]);
+              if (u + 1 == to[t]) commit(smem_address(&C.outputs[t]));
             }
             __syncwarp();
           }
-          if (range[t].has(u + 1)) {
-            if (u + 1 == range[t].from) {
+          if (u + 1 >= from[t] && u + 1 < to[t]) {
+            if (u + 1 == from[t]) {
               fine = fine && barrier_wait_warp(smem_address(&C.queries[t]), query_phase[t], &C.gave_up);
               if (!fine) break;
               query_phase[t] ^= 1u;
@@ -264,10 +313,11 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               const uint64_t k_tile = operand(ring + (k_fill % kSlots) * M::kTileBytes, 1);
 #pragma unroll
               for (int k = 0; k < DIM / 16; ++k) {
-                const uint32_t at = (k >> 2) * (kTileRows * 128 / 16) + (k & 3) * 2;
+                const uint32_t at = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
                 product_shared(s, q + at, k_tile + at, kScores, k > 0);
               }
               commit(smem_address(&C.scores[t]));
+              if (u + 2 == to[t]) commit(smem_address(&C.queries_free[t]));
             }
             __syncwarp();
           }
@@ -278,58 +328,46 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         }
         __syncwarp();
       }
-      used += 2u * piece.count;
-      piece.done();
+      used += 2u * static_cast<uint32_t>(end - first);
+      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
     if (!fine) {
       if (issuer) commit(smem_address(&C.drained));
       barrier_wait_out(smem_address(&C.drained), 0);
     }
-  } else if (warp < kMmaWarp) {
+  }
+  } else {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+  {
     const uint32_t t = warp >> 2, thread = threadIdx.x & 127u;
     const uint32_t lanes = (warp & 3u) << 21;  // this warp's rows of tensor memory: lane 32 x (warp & 3), bits 16 up
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
     const float ninf = __int_as_float(0xff800000);
     uint32_t score_phase = 0, output_phase = 0;
-    while (fine && piece.next()) {
-      const TileRange range = tile_range(P, piece, t);
-      const uint32_t rows = piece.rows();
-      const uint32_t r = t * kTileRows + thread;  // row of the item
-      const bool valid = r < rows;
-      const uint32_t g = piece.tile * kRows + r;
-      const uint32_t token = g / P.group, head = piece.head * P.group + g % P.group;
+    const uint32_t half = P.item_rows / 2;
+    uint8_t* const stage = smem + M::kStage + warp * 4096;
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t at = n % kPieces;
+      fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
+      const Piece& piece = C.pieces[at];
+      if (!fine || piece.valid == 0) break;
+      const uint32_t r = t * half + thread;  // row of the item
+      const bool valid = thread < half && r < piece.rows;
+      const uint32_t g = piece.first_row + r;
+      const int32_t from = piece.from[t], to = piece.to[t];
       float m = ninf, l = 0.f;
-      if (range.to > range.from) {
-        // queries: consecutive lanes take consecutive parts of a row
-        uint8_t* const q_tile = smem + t * M::kTileBytes;
-        constexpr uint32_t kParts = DIM / 8;
-#pragma unroll 4
-        for (uint32_t i = thread; i < kTileRows * kParts; i += 128) {
-          const uint32_t row = i / kParts, part = i % kParts;
-          const uint32_t gr = piece.tile * kRows + t * kTileRows + row;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (t * kTileRows + row < rows && part * 8 < P.head_dim) {
-            const uint32_t tok = gr / P.group;
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(P.q) + (piece.s.token + static_cast<int64_t>(tok)) * P.q_token +
-                                                static_cast<int64_t>(piece.head * P.group + gr - tok * P.group) * P.q_head + part * 8);
-          }
-          *reinterpret_cast<uint4*>(q_tile + (part >> 3) * (kTileRows * 128) + row * 128 + (((part & 7u) ^ (row & 7u)) << 4)) = v;
-        }
-        shared_to_async();
-        __syncwarp();
-        if (lane == 0) barrier_arrive(smem_address(&C.queries[t]));
-
-        const int32_t position = piece.s.length - piece.s.n + static_cast<int32_t>(token);
+      if (to > from) {
+        const int32_t position = piece.length - piece.n + static_cast<int32_t>(g / P.group);
         int32_t see_from = 0, see_to = 0x7fffffff;
         if (valid) {
-          see_to = P.causal ? max(position + 1, 0) : piece.s.length;
+          see_to = P.causal ? max(position + 1, 0) : piece.length;
           if (P.causal && P.window)
             see_from = static_cast<int32_t>(max(static_cast<int64_t>(0), position + 1 - static_cast<int64_t>(P.window)));
         }
         const int32_t all_from = __reduce_max_sync(0xffffffffu, see_from);
         const int32_t all_to = __reduce_min_sync(0xffffffffu, see_to);
 
-        for (int32_t u = range.from; u < range.to; ++u) {
+        for (int32_t u = from; u < to; ++u) {
           fine = barrier_wait_warp(smem_address(&C.scores[t]), score_phase, &C.gave_up);
           if (!fine) break;
           score_phase ^= 1u;
@@ -337,29 +375,29 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           const int32_t key0 = u * kKeys;
           const bool tested = key0 < all_from || key0 + kKeys > all_to;
           const int32_t hide_to = see_from - key0, hide_from = see_to - key0;
-          // The scores are read twice, a part at a time: once for the maximum, once for the probabilities.
-          // All 128 of them in registers spill.
-          float top = ninf;
-          {
-            uint32_t s[2][32];
-            load_columns(s_at, s[0]);
+          uint32_t s[kKeys];
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 32) {
-              uint32_t* now = s[(i >> 5) & 1];
-              loads_done(now);
-              if (i + 32 < kKeys) load_columns(s_at + i + 32, s[((i >> 5) + 1) & 1]);
-              if (tested) hide(now, i, hide_to, hide_from);
-              float part[4] = {__uint_as_float(now[0]), __uint_as_float(now[1]), __uint_as_float(now[2]), __uint_as_float(now[3])};
+          for (int i = 0; i < kKeys; i += 32) load_columns(s_at + i, s + i);
+          loads_done(s);
 #pragma unroll
-              for (int j = 4; j < 32; ++j) part[j & 3] = fmaxf(part[j & 3], __uint_as_float(now[j]));
-              top = fmaxf(top, fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-            }
+          for (int i = 32; i < kKeys; i += 32) loaded(s + i);
+          if (tested) {
+#pragma unroll
+            for (int i = 0; i < kKeys; i += 32) hide(s + i, i, hide_to, hide_from);
           }
-          if (u == range.from) {
+          float part[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
+#pragma unroll
+          for (int j = 4; j < kKeys; j += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              part[i] = j + 4 < kKeys ? max3(part[i], __uint_as_float(s[j + i]), __uint_as_float(s[j + 4 + i]))
+                                      : fmaxf(part[i], __uint_as_float(s[j + i]));
+          const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
+          if (u == from) {
             m = top;
           } else {
             // the scores of this unit are there, so the last unit's O is complete
-            const bool rise = (top - m) * P.scale_log2 > kRise;
+            const bool rise = valid && (top - m) * P.scale_log2 > kRise;
             if (__any_sync(0xffffffffu, rise)) {
               const float f = rise ? exp2_fast((m - top) * P.scale_log2) : 1.f;
               if (rise) m = top;
@@ -378,25 +416,17 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           }
           const float shift = m == ninf ? 0.f : m * P.scale_log2;
           float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          {
-            uint32_t s[2][32];
-            load_columns(s_at, s[0]);
 #pragma unroll
-            for (int i = 0; i < kKeys; i += 32) {
-              uint32_t* now = s[(i >> 5) & 1];
-              loads_done(now);
-              if (i + 32 < kKeys) load_columns(s_at + i + 32, s[((i >> 5) + 1) & 1]);
-              if (tested) hide(now, i, hide_to, hide_from);
-              uint32_t p[16];
+          for (int i = 0; i < kKeys; i += 32) {
+            uint32_t p[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float a = exp2_fast(fmaf(__uint_as_float(now[2 * j]), P.scale_log2, -shift));
-                const float b = exp2_fast(fmaf(__uint_as_float(now[2 * j + 1]), P.scale_log2, -shift));
-                sum[j & 3] += a + b;
-                p[j] = Pair<T>::pack(a, b);  // one rounding to the values' type
-              }
-              store_columns_16(s_at + i / 2, p);  // over scores that have been read
+            for (int j = 0; j < 16; ++j) {
+              const float a = exp2_fast(fmaf(__uint_as_float(s[i + 2 * j]), P.scale_log2, -shift));
+              const float b = exp2_fast(fmaf(__uint_as_float(s[i + 2 * j + 1]), P.scale_log2, -shift));
+              sum[j & 3] += a + b;
+              p[j] = Pair<T>::pack(a, b);  // one rounding to the values' type
             }
+            store_columns_16(s_at + i / 2, p);  // over scores that have been read
           }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           stores_done();
@@ -410,20 +440,22 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         output_phase ^= 1u;
         after_sync();
       }
-      const bool any = range.to > range.from;
-      const bool complete = piece.begins() && piece.ends();
-      if (t * kTileRows < rows) {
-        const int64_t at = piece.s.token + static_cast<int64_t>(token);
-        const float inverse = l == 0.f ? 0.f : 1.f / l;
-        float* slot = complete ? nullptr
-                               : P.partial + (2u * blockIdx.x + (piece.begins() ? 1u : 0u)) *
-                                                 static_cast<size_t>(kRows * (2 + DIM));
-        if (valid) {
-          if (!complete)
-            *reinterpret_cast<float2*>(slot + r * 2) = make_float2(m, l);
-          else if (P.lse)
-            P.lse[at * P.kv_heads * P.group + head] = l == 0.f ? ninf : m * P.scale + logf(l);
+      if (t * half < piece.rows) {
+        const bool any = to > from, complete = piece.begins && piece.ends;
+        const uint32_t token = g / P.group, head = piece.head * P.group + (g - token * P.group);
+        const int64_t row_of = piece.token + static_cast<int64_t>(token);
+        const float inverse = !complete ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        uint64_t row_at;  // where this thread's row goes
+        if (complete) {
+          row_at = reinterpret_cast<uint64_t>(static_cast<T*>(P.out) + row_of * P.out_token + static_cast<int64_t>(head) * P.out_head);
+          if (valid && P.lse) P.lse[row_of * P.kv_heads * P.group + head] = l == 0.f ? ninf : m * P.scale + logf(l);
+        } else {
+          float* slot = P.partial + (2u * blockIdx.x + (piece.begins ? 1u : 0u)) * static_cast<size_t>(kRows * (2 + DIM));
+          row_at = reinterpret_cast<uint64_t>(slot + kRows * 2 + r * DIM);
+          if (valid) *reinterpret_cast<float2*>(slot + r * 2) = make_float2(m, l);
         }
+        // 32 columns at a time through this warp's stage, so that eight lanes write 128 bytes of a row together
+        const uint32_t rows_here = __popc(__ballot_sync(0xffffffffu, valid));  // the first ones
 #pragma unroll 1
         for (int i = 0; i < DIM; i += 32) {
           uint32_t o[32];
@@ -434,33 +466,43 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = 0u;
           }
-          if (!valid) continue;
-          if (complete) {
-            T* to = static_cast<T*>(P.out) + at * P.out_token + static_cast<int64_t>(head) * P.out_head + i;
+          uint8_t* const mine = stage + lane * 128;
+          if (complete) {  // 64 bytes: two turns fill a row of the stage
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (static_cast<uint32_t>(i + j) < P.head_dim) {
-                uint4 v;
-                v.x = Pair<T>::pack(__uint_as_float(o[j]) * inverse, __uint_as_float(o[j + 1]) * inverse);
-                v.y = Pair<T>::pack(__uint_as_float(o[j + 2]) * inverse, __uint_as_float(o[j + 3]) * inverse);
-                v.z = Pair<T>::pack(__uint_as_float(o[j + 4]) * inverse, __uint_as_float(o[j + 5]) * inverse);
-                v.w = Pair<T>::pack(__uint_as_float(o[j + 6]) * inverse, __uint_as_float(o[j + 7]) * inverse);
-                *reinterpret_cast<uint4*>(to + j) = v;
-              }
+            for (int j = 0; j < 32; j += 8) {
+              uint4 v;
+              v.x = Pair<T>::pack(__uint_as_float(o[j]) * inverse, __uint_as_float(o[j + 1]) * inverse);
+              v.y = Pair<T>::pack(__uint_as_float(o[j + 2]) * inverse, __uint_as_float(o[j + 3]) * inverse);
+              v.z = Pair<T>::pack(__uint_as_float(o[j + 4]) * inverse, __uint_as_float(o[j + 5]) * inverse);
+              v.w = Pair<T>::pack(__uint_as_float(o[j + 6]) * inverse, __uint_as_float(o[j + 7]) * inverse);
+              const uint32_t part = (i & 32) / 8 + j / 8;
+              *reinterpret_cast<uint4*>(mine + ((part ^ (lane & 7u)) << 4)) = v;
+            }
+            if ((i & 32) == 0) continue;
           } else {
-            uint4* to = reinterpret_cast<uint4*>(slot + kRows * 2 + r * DIM + i);
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) to[j / 4] = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int j = 0; j < 32; j += 4)
+              *reinterpret_cast<uint4*>(mine + ((static_cast<uint32_t>(j / 4) ^ (lane & 7u)) << 4)) =
+                  make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
+          __syncwarp();
+          const uint32_t part = lane & 7u;
+          const uint32_t element = complete ? static_cast<uint32_t>(i - 32) + part * 8 : static_cast<uint32_t>(i) + part * 4;
+          const uint32_t offset = complete ? element * 2 : element * 4;
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) {
+            const uint32_t row = j * 4 + (lane >> 3);
+            const uint64_t to_row = __shfl_sync(0xffffffffu, row_at, row);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((part ^ (row & 7u)) << 4));
+            if (row < rows_here && (!complete || element < P.head_dim)) *reinterpret_cast<uint4*>(to_row + offset) = v;
+          }
+          __syncwarp();
         }
         before_sync();
       }
-      if (piece.begins() && !piece.ends())
-        header = AttentionHeader{piece.more(share), rows, piece.tile * kRows, piece.head,
-                                 static_cast<uint32_t>(piece.s.token), {0, 0, 0}};
-      piece.done();
+      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
-    if (threadIdx.x == 0 && P.headers) P.headers[blockIdx.x] = header;
+  }
   }
   before_sync();
   __syncthreads();
@@ -476,9 +518,6 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 
 }  // namespace paged
 
-size_t many_rows_smem(uint32_t padded_dim) {
-  return 1024 + (padded_dim == 64 ? paged::ManySmem<64>::kBytes : paged::ManySmem<128>::kBytes);
-}
 namespace {
 template <typename T, int DIM>
 cudaError_t prepare() {
@@ -488,11 +527,11 @@ cudaError_t prepare() {
   if (e != cudaSuccess) return e;
   if (a.numRegs < static_cast<int>(paged::kLaunchRegisters)) return cudaErrorInvalidDeviceFunction;
   return cudaFuncSetAttribute(paged::many_rows_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              static_cast<int>(many_rows_smem(DIM)));
+                              1024 + paged::ManySmem<DIM>::kBytes);
 }
 template <typename T, int DIM>
 cudaError_t launch(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
-  return launch_dependent(paged::many_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsMany, many_rows_smem(DIM), p,
+  return launch_dependent(paged::many_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsMany, 1024 + paged::ManySmem<DIM>::kBytes, p,
                           stream);
 }
 }  // namespace

@@ -13,9 +13,9 @@ constexpr int kRowsThreads = 256;
 
 // V elements at once, of type T
 template <typename T, int V>
-struct Piece;
+struct Vector;
 template <typename T>
-struct Piece<T, 8> {
+struct Vector<T, 8> {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
@@ -34,7 +34,7 @@ struct Piece<T, 8> {
   }
 };
 template <typename T>
-struct Piece<T, 1> {
+struct Vector<T, 1> {
   T v;
   __device__ __forceinline__ void load(const T* p) { v = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = v; }
@@ -74,13 +74,13 @@ __device__ __forceinline__ void rotate_heads(const RowsSource& s, const T* src, 
     if (j >= turned) {
       const uint32_t d = rd + (j - turned) * V;
       for (uint32_t h = head0; h < s.heads; h += step) {
-        Piece<T, V> a;
+        Vector<T, V> a;
         a.load(src + h * s.src_head + d);
         a.store(dst + h * s.dst_head + d);
       }
     } else if (interleaved && V == 8) {
       for (uint32_t h = head0; h < s.heads; h += step) {
-        Piece<T, V> a;
+        Vector<T, V> a;
         a.load(src + h * s.src_head + j * V);
         float x[V], y[V];
         a.get(x);
@@ -96,7 +96,7 @@ __device__ __forceinline__ void rotate_heads(const RowsSource& s, const T* src, 
     } else {
       const uint32_t d0 = interleaved ? 2 * j : j * V, d1 = interleaved ? 2 * j + 1 : rd / 2 + j * V;
       for (uint32_t h = head0; h < s.heads; h += step) {
-        Piece<T, V> a, b;
+        Vector<T, V> a, b;
         a.load(src + h * s.src_head + d0);
         b.load(src + h * s.src_head + d1);
         float x[V], y[V], u[V], w[V];
