@@ -245,14 +245,15 @@ int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_arg
   p->padded_dim = c.head_dim <= 64 ? 64 : 128;
   const uint32_t few_rows = kFewRows * static_cast<uint32_t>(std::min<uint64_t>((rows + kFewRows - 1) / kFewRows, kFewTilesMost));
   const uint32_t whole_tokens = group <= kTileRows ? kTileRows / group * group : 0;  // rows of a row tile of the other
-  p->many = rows > kFewTilesMost * kFewRows || items(few_rows) * tiles(kFewKeys) >= kMostUnits;
+  p->many = rows > kFewTilesMost * kFewRows || items(few_rows) * (tiles(kFewKeys) + 2) >= kMostUnits;
   if (whole_tokens == 0) p->many = false;
   p->rows = p->many ? kManyRows : few_rows;
   p->item_rows = p->many ? 2 * whole_tokens : few_rows;
   p->keys = p->many ? kManyKeys : kFewKeys;
   p->least_units = (p->many ? kManyLeastKeys : kFewLeastKeys) / p->keys;
   p->box = std::gcd(c.page_size, p->keys);
-  const uint64_t most_units = items(p->item_rows) * tiles(p->keys);
+  p->item_cost = p->many ? 1 : p->padded_dim == 64 ? 2 : 1;
+  const uint64_t most_units = items(p->item_rows) * (tiles(p->keys) + p->item_cost);
   if (most_units >= kMostUnits)
     return fail(MONONN_ERR_TOO_LARGE, "attention: so many new tokens over so many keys count 2^31 units of work or more");
   const bool whole = capacity <= kWholeKeys;
@@ -459,6 +460,7 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.capacity = c.max_pages * c.page_size;
   p.box = plan.box;
   p.item_rows = plan.item_rows;
+  p.item_cost = plan.item_cost;
   p.causal = a.causal != 0;
   p.window = a.window;
   p.whole_items = !plan.joins;

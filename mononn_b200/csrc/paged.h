@@ -61,7 +61,7 @@ struct AttentionParams {
   AttentionHeader* headers;
   float* partial;           // slots 2 * CTA (an item begun earlier) and 2 * CTA + 1 (one that goes on)
   uint32_t* status;
-  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box, item_rows;
+  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box, item_rows, item_cost;
   uint32_t causal, window, min_units, whole_items;
   float scale, scale_log2;  // of the scores; scale * log2(e)
 };
@@ -69,6 +69,7 @@ struct AttentionPlan {  // how a call is launched: the same for every content of
   bool many;            // the kernel for many rows
   uint32_t rows, keys, padded_dim, ctas, least_units;  // rows: of a slot of the workspace
   uint32_t item_rows;   // rows of an item, at most `rows`
+  uint32_t item_cost;   // units that stand for an item's work beside its keys
   uint32_t box;         // token rows that one copy brings
   bool joins;           // an item may span CTAs: workspace and the second kernel are needed
   size_t workspace;

@@ -163,10 +163,11 @@ template <int KEYS>
 __device__ __forceinline__ uint32_t item_tiles(const KeyRange& r) {
   return r.end > r.begin ? (r.end + KEYS - 1) / KEYS - r.begin / KEYS : 1u;
 }
-// Its units: as many, or one where no item is split.
+// Its units: as many, behind the ones that stand for what an item takes beside its keys (queries, joining the
+// warps, the way out); one in all where no item is split.
 template <int KEYS>
 __device__ __forceinline__ uint32_t item_units(const AttentionParams& P, const Sequence& s, uint32_t tile) {
-  return P.whole_items ? 1u : item_tiles<KEYS>(item_keys(P, s, tile));
+  return P.whole_items ? 1u : P.item_cost + item_tiles<KEYS>(item_keys(P, s, tile));
 }
 // Units of one head of a sequence that is the same for the whole warp.
 template <int KEYS>
@@ -179,7 +180,7 @@ __device__ __forceinline__ uint32_t head_units_warp(const AttentionParams& P, co
 // `each` + 1 units, the others `each`. The host has made sure that units are counted in 31 bits.
 struct Share {
   uint32_t units, begin, ctas, each, longer;
-  uint32_t sequence, head, row_tile, skip;  // the item that holds the first unit, and its units before it
+  uint32_t sequence, head, row_tile, skip;  // the item that holds the first unit, and its units before that
   __device__ __forceinline__ uint32_t cta_of(uint32_t unit) const {
     const uint32_t in_longer = (each + 1u) * longer;
     return unit < in_longer ? unit / (each + 1u) : longer + (unit - in_longer) / each;
@@ -282,7 +283,8 @@ struct Piece {
   int32_t keys_begin, keys_end;    // that some row of the item sees
   uint32_t begins, ends;           // whether the item begins and ends in it
   uint32_t valid;                  // 0: no more pieces
-  int32_t pad[3];
+  uint32_t sequence;
+  int32_t pad[2];
   int32_t from[2], to[2];          // many rows: the key tiles from .. to - 1 that concern each of the two row tiles
 };
 // Walks through the pieces of a share; all lanes of the loading warp alike.
@@ -291,57 +293,71 @@ struct Walker {
   const AttentionParams& P;
   const Share& share;
   Sequence s;
-  uint32_t b, head, tile, skip, left, tiles, at, whole;
+  uint32_t b, head, tile, skip, left, tiles, at, whole, goes_on;  // goes_on: tiles of the item behind the piece
   Piece piece;
   __device__ __forceinline__ Walker(const AttentionParams& params, const Share& sh)
       : P(params), share(sh), s{0, 0, 0}, b(sh.sequence), head(sh.head), tile(sh.row_tile), skip(sh.skip),
-        left(sh.units), tiles(0), at(sh.begin), whole(0), piece{} {
+        left(sh.units), tiles(0), at(sh.begin), whole(0), goes_on(0), piece{} {
     if (left) {
       s = load_sequence(P, b);
       tiles = row_tiles(P, s);
     }
   }
   __device__ __forceinline__ bool next() {
-    piece.valid = left != 0;
-    if (left == 0) return false;
-    if (tile == tiles) {  // on to the next head, or the next sequence that has new tokens
-      tile = 0;
-      if (++head == P.kv_heads) {
-        head = 0;
-        do {
-          s = load_sequence(P, ++b);
-        } while (s.n == 0);
-        tiles = row_tiles(P, s);
+    uint32_t units = 0, done = 0;
+    KeyRange keys{0, 0};
+    for (;;) {
+      piece.valid = left != 0;
+      if (left == 0) return false;
+      if (tile == tiles) {  // on to the next head, or the next sequence that has new tokens
+        tile = 0;
+        if (++head == P.kv_heads) {
+          head = 0;
+          do {
+            s = load_sequence(P, ++b);
+          } while (s.n == 0);
+          tiles = row_tiles(P, s);
+        }
       }
+      keys = item_keys(P, s, tile);
+      whole = item_tiles<KEYS>(keys);
+      if (P.whole_items) {
+        units = 1u;
+        done = 0;
+        piece.count = static_cast<int32_t>(whole);
+      } else {
+        units = min(P.item_cost + whole - skip, left);
+        done = skip > P.item_cost ? skip - P.item_cost : 0u;
+        const uint32_t upto = skip + units;
+        piece.count = static_cast<int32_t>((upto > P.item_cost ? upto - P.item_cost : 0u) - done);
+      }
+      left -= units;
+      at += units;
+      if (piece.count != 0) break;
+      // the share ends before the item's first tile: the next CTA begins the item
     }
-    const KeyRange keys = item_keys(P, s, tile);
-    whole = item_tiles<KEYS>(keys);
+    piece.sequence = b;
     piece.token = s.token;
     piece.n = s.n;
     piece.length = s.length;
     piece.head = head;
     piece.first_row = tile * P.item_rows;
     piece.rows = min(P.item_rows, static_cast<uint32_t>(s.n) * P.group - piece.first_row);
-    piece.tile = static_cast<int32_t>((keys.end > keys.begin ? keys.begin / KEYS : 0u) + skip);
-    piece.count = static_cast<int32_t>(P.whole_items ? whole : min(whole - skip, left));
+    piece.tile = static_cast<int32_t>((keys.end > keys.begin ? keys.begin / KEYS : 0u) + done);
     piece.keys_begin = keys.begin;
     piece.keys_end = keys.end;
-    piece.begins = skip == 0;
-    piece.ends = skip + piece.count == whole;
-    return true;
-  }
-  __device__ __forceinline__ void done() {
-    const uint32_t units = P.whole_items ? 1u : static_cast<uint32_t>(piece.count);
-    left -= units;
-    at += units;
+    piece.begins = done == 0;
+    piece.ends = done + piece.count == whole;
+    goes_on = whole - done - static_cast<uint32_t>(piece.count);
     ++tile;
     skip = 0;
+    return true;
   }
   // Behind the last piece: whether its item goes on, and in how many CTAs.
   __device__ __forceinline__ void write_header() const {
     AttentionHeader h{0, 0, 0, 0, 0, {0, 0, 0}};
     if (share.units != 0 && piece.begins && !piece.ends) {
-      const uint32_t last = at + whole - static_cast<uint32_t>(piece.count) - 1u;  // the item's last unit
+      const uint32_t last = at + goes_on - 1u;  // the item's last unit
       h = AttentionHeader{share.cta_of(last) - blockIdx.x, piece.rows, piece.first_row, piece.head,
                           static_cast<uint32_t>(piece.token), {0, 0, 0}};
     }
@@ -354,41 +370,60 @@ __device__ __forceinline__ void put_piece(Piece* to, const Piece& p, uint32_t la
   d[0] = make_int4(p.token, p.n, p.length, static_cast<int>(p.head));
   d[1] = make_int4(static_cast<int>(p.first_row), static_cast<int>(p.rows), p.tile, p.count);
   d[2] = make_int4(p.keys_begin, p.keys_end, static_cast<int>(p.begins), static_cast<int>(p.ends));
-  d[3] = make_int4(static_cast<int>(p.valid), 0, 0, 0);
+  d[3] = make_int4(static_cast<int>(p.valid), static_cast<int>(p.sequence), 0, 0);
   d[4] = make_int4(p.from[0], p.from[1], p.to[0], p.to[1]);
 }
 
-// The warp that loads: boxes of a tile of keys, one lane each; page numbers are read a tile ahead.
+// A warp that loads tiles of keys or values: boxes of one page each, a lane to a box. Page numbers are
+// read for 32 boxes at a time, and those one such window ahead.
 template <int KEYS, int HALVES>
 struct TileLoader {
   const AttentionParams& P;
-  const uint32_t lane;
-  const uint32_t boxes;
-  int32_t page, row;
-  bool wanted;
+  const uint32_t lane, boxes, window;  // boxes of a tile, tiles of a window
+  uint32_t sequence, first;            // first tile of the present window
+  int32_t keys_begin, keys_end;
+  int32_t page, row, next_page, next_row;  // row below 0: not wanted
   __device__ __forceinline__ TileLoader(const AttentionParams& params)
-      : P(params), lane(threadIdx.x & 31u), boxes(KEYS / params.box), page(-1), row(0), wanted(false) {}
-  __device__ __forceinline__ void look_up(uint32_t b, const Piece& piece, uint32_t tile) {
-    const int32_t key = static_cast<int32_t>(tile * KEYS + lane * P.box);
-    wanted = lane < boxes && key < piece.keys_end && key + static_cast<int32_t>(P.box) > piece.keys_begin;
-    page = -1;
-    row = 0;
-    if (wanted) {
+      : P(params), lane(threadIdx.x & 31u), boxes(KEYS / params.box), window(32u / boxes), sequence(0), first(0),
+        keys_begin(0), keys_end(0), page(-1), row(-1), next_page(-1), next_row(-1) {}
+  __device__ __forceinline__ void look_up(uint32_t tile0, int32_t& page_of, int32_t& row_of) const {
+    const int32_t key = static_cast<int32_t>(tile0 * KEYS + lane * P.box);
+    page_of = -1;
+    row_of = -1;
+    if (key < keys_end && key + static_cast<int32_t>(P.box) > keys_begin) {
       const uint32_t p = static_cast<uint32_t>(key) / P.page_size;
-      row = key - static_cast<int32_t>(p * P.page_size);
-      page = P.table[static_cast<int64_t>(b) * P.table_stride + p];
+      row_of = key - static_cast<int32_t>(p * P.page_size);
+      page_of = P.table[static_cast<int64_t>(sequence) * P.table_stride + p];
     }
   }
-  // Loads the tile of this look-up into `dst` (HALVES blocks of KEYS rows of 128 bytes, swizzled).
+  __device__ __forceinline__ void begin(const Piece& piece) {
+    sequence = piece.sequence;
+    keys_begin = piece.keys_begin;
+    // no further than the piece itself goes
+    keys_end = min(piece.keys_end, (piece.tile + piece.count) * KEYS);
+    first = static_cast<uint32_t>(piece.tile);
+    look_up(first, page, row);
+    look_up(first + window, next_page, next_row);
+  }
+  // Loads a tile, the next one of the piece, into `dst` (HALVES blocks of KEYS rows of 128 bytes, swizzled).
   // Boxes without a visible key are left out: what the slot holds there is from earlier.
-  __device__ __forceinline__ void load(const CUtensorMap* map, uint32_t dst, uint32_t head, uint32_t bar) const {
+  __device__ __forceinline__ void load(const CUtensorMap* map, uint32_t tile, uint32_t dst, uint32_t head, uint32_t bar) {
+    if (tile - first == window) {
+      first = tile;
+      page = next_page;
+      row = next_row;
+      look_up(first + window, next_page, next_row);
+    }
+    const uint32_t from = (tile - first) * boxes + (lane & (boxes - 1u));
+    const int32_t p = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, row, from);
+    const bool wanted = lane < boxes && r >= 0;
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, wanted));
     if (lane == 0) barrier_arrive_bytes(bar, count * P.box * 128u * HALVES);
     __syncwarp();
     if (wanted) {
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
-        load_box(dst + h * KEYS * 128 + lane * P.box * 128u, map, h * 64, row, static_cast<int32_t>(head), page, bar);
+        load_box(dst + h * KEYS * 128 + lane * P.box * 128u, map, h * 64, r, static_cast<int32_t>(head), p, bar);
     }
   }
 };

@@ -16,7 +16,7 @@ template <int DIM, int TILES>
 struct FewShape {
   static constexpr int kRows = static_cast<int>(kFewRows) * TILES;
   static constexpr int kWarps = kKeyGroups * TILES;  // that compute
-  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kThreads = (kWarps + 2) * 32;  // one more that loads keys, one that loads values
   static constexpr int kCtas = TILES == 1 ? 2 : 1;   // of an SM
   static constexpr int kSlotBytes = static_cast<int>(kFewKeys) * DIM * 2;
   // keys or values of one tile each
@@ -33,7 +33,7 @@ struct FewControl {
   uint64_t full[S::kSlots], empty[S::kSlots], told[kPieces], taken[kPieces], meeting;
   alignas(16) Piece pieces[kPieces];
   Share share;
-  uint32_t sums[S::kWarps + 1];
+  uint32_t sums[S::kWarps + 2];
   uint32_t gave_up;
   float maxima[kKeyGroups][S::kRows], totals[kKeyGroups][S::kRows];
 };
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
     }
     for (int i = 0; i < kPieces; ++i) {
       barrier_init(smem_address(&C.told[i]), 33);
-      barrier_init(smem_address(&C.taken[i]), kWarps);
+      barrier_init(smem_address(&C.taken[i]), kWarps + 1);
     }
     barrier_init(smem_address(&C.meeting), kWarps);
     C.gave_up = 0;
@@ -113,7 +113,9 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
   let_next_begin();
   earlier_done();
   find_share<kFewKeys, S::kThreads>(P, C.sums, &C.share);  // barriers of the CTA within
-  uint32_t fills = 0;  // of the loading warp
+  // Slots 0, 2, .. hold keys, 1, 3, .. values.
+  constexpr uint32_t kPairs = kSlots / 2;
+  uint32_t fills = 0;  // of this loading warp
 
   if (warp == kWarps) {
     TileLoader<kFewKeys, kHalves> loader(P);
@@ -121,10 +123,11 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
     bool fine = true;
     for (uint32_t i = 0; fine; ++i) {
       const bool some = walk.next();
-      if (some) loader.look_up(walk.b, walk.piece, walk.piece.tile);
+      if (some) loader.begin(walk.piece);
       const uint32_t at = i % kPieces, told = smem_address(&C.told[at]);
       fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
       if (!fine) break;
+      put_piece(&C.pieces[at], walk.piece, lane);
       if (some) {  // the queries of the piece, consecutive lanes along a row
         constexpr uint32_t kParts = DIM / 8;
         const uint32_t tile = slots + S::kQueries + at * S::kQueryBytes;
@@ -139,24 +142,39 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
           copy_16(tile + (part >> 3) * (kRows * 128) + row * 128 + (((part & 7u) ^ (row & 7u)) << 4), src, wanted);
         }
       }
-      put_piece(&C.pieces[at], walk.piece, lane);
       arrive_after_copies(told);
       if (lane == 0) barrier_arrive(told);
       if (!some) break;
-      for (int32_t u = 0; fine && u < walk.piece.count; ++u) {
-        const TileLoader<kFewKeys, kHalves> now = loader;
-        if (u + 1 < walk.piece.count) loader.look_up(walk.b, walk.piece, walk.piece.tile + u + 1);
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t slot = fills % kSlots;
-          fine = fine && barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kSlots) & 1u) ^ 1u, &C.gave_up);
-          if (!fine) break;
-          now.load(kv ? &P.v_map : &P.k_map, slots + slot * S::kSlotBytes, walk.piece.head, smem_address(&C.full[slot]));
-          ++fills;
-        }
+      for (int32_t u = 0; u < walk.piece.count; ++u) {
+        const uint32_t slot = fills % kPairs * 2u;
+        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+        if (!fine) break;
+        loader.load(&P.k_map, walk.piece.tile + u, slots + slot * S::kSlotBytes, walk.piece.head, smem_address(&C.full[slot]));
+        ++fills;
       }
-      walk.done();
     }
     if (lane == 0 && P.headers) walk.write_header();
+  } else if (warp == kWarps + 1) {
+    TileLoader<kFewKeys, kHalves> loader(P);
+    bool fine = true;
+    for (uint32_t i = 0; fine; ++i) {
+      const uint32_t at = i % kPieces;
+      fine = barrier_wait_warp(smem_address(&C.told[at]), (i / kPieces) & 1u, &C.gave_up);
+      const Piece& piece = C.pieces[at];
+      if (!fine || piece.valid == 0) break;
+      const int32_t tile = piece.tile, count = piece.count;
+      const uint32_t head = piece.head;
+      loader.begin(piece);
+      __syncwarp();
+      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
+      for (int32_t u = 0; u < count; ++u) {
+        const uint32_t slot = fills % kPairs * 2u + 1u;
+        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+        if (!fine) break;
+        loader.load(&P.v_map, tile + u, slots + slot * S::kSlotBytes, head, smem_address(&C.full[slot]));
+        ++fills;
+      }
+    }
   } else {
     const float ninf = __int_as_float(0xff800000);
     uint32_t slot = 0, parity = 0, meetings = 0;
@@ -385,10 +403,10 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
     }
   }
   __syncthreads();
-  if (C.gave_up && warp == kWarps) {
+  if (C.gave_up && warp >= kWarps) {
     asm volatile("cp.async.wait_all;" ::: "memory");
-    for (uint32_t f = fills > kSlots ? fills - kSlots : 0u; f < fills; ++f)
-      barrier_wait_out(smem_address(&C.full[f % kSlots]), (f / kSlots) & 1u);
+    for (uint32_t f = fills > kPairs ? fills - kPairs : 0u; f < fills; ++f)
+      barrier_wait_out(smem_address(&C.full[f % kPairs * 2u + (warp - kWarps)]), (f / kPairs) & 1u);
     if (lane == 0) atomicExch(P.status, 1u);
   }
 }

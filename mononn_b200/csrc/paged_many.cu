@@ -6,7 +6,7 @@
 //                   running maximum, probabilities back to tensor memory, row sums in registers
 //   warp 8          issues the matrix products: S = Q K^T (both operands in shared memory), O += P V (P in
 //                   tensor memory, in the place of the scores it was made from)
-//   warp 9          loads keys and values, page by page, into a ring of tiles
+//   warps 9, 10     load keys (and queries) and values, page by page, into a ring of tiles
 // While one row tile's softmax runs, the tensor cores work on the other's products.
 // O stays in tensor memory. It is rescaled only when a row's maximum has risen by more than
 // 2^8 since its reference was set: until then probabilities are above 1, by 2^8 at most, which costs no accuracy.
@@ -17,7 +17,7 @@ namespace paged {
 
 constexpr int kRows = static_cast<int>(kManyRows), kKeys = static_cast<int>(kManyKeys);
 constexpr int kThreadsMany = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;  // 10 and 11 only make up the group whose registers go to the others
+constexpr int kMmaWarp = 8, kKeyWarp = 9, kValueWarp = 10;  // 11 only makes up the group whose registers go to the others
 constexpr int kPieces = 4;                  // told ahead
 constexpr uint32_t kSoftmaxRegisters = 216, kOtherRegisters = 72, kLaunchRegisters = 168;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreadsMany * kLaunchRegisters, "register split");
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     }
     for (int i = 0; i < kPieces; ++i) {
       barrier_init(smem_address(&C.told[i]), 1);
-      barrier_init(smem_address(&C.taken[i]), 9);  // the softmax warps and the one that issues the products
+      barrier_init(smem_address(&C.taken[i]), 10);  // all but the warp that tells
     }
     barrier_init(smem_address(&C.drained), 1);
     C.gave_up = 0;
@@ -192,12 +192,14 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   find_share<kKeys, kThreadsMany>(P, C.sums, &C.share);  // barriers of the CTA within
   after_sync();
   const uint32_t tmem = *const_cast<volatile uint32_t*>(&C.tmem);
-  uint32_t fills = 0;  // of the loading warp
+  // Slots 0, 2, .. of the ring hold keys, 1, 3, .. values.
+  constexpr uint32_t kPairs = kSlots / 2;
+  uint32_t fills = 0;  // of this loading warp
   bool fine = true;
   // Each group of warps within its own branch: code behind a meeting of both is held to the fewer registers.
   if (warp >= kMmaWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-  if (warp == kLoadWarp) {
+  if (warp == kKeyWarp) {
     TileLoader<kKeys, kHalves> loader(P);
     Walker<kKeys> walk(P, C.share);
     const uint32_t half = P.item_rows / 2, half_tokens = half / P.group;
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     for (uint32_t i = 0; fine; ++i) {
       const bool some = walk.next();
       if (some) {
-        loader.look_up(walk.b, walk.piece, walk.piece.tile);
+        loader.begin(walk.piece);
         set_ranges(P, walk.piece);
       }
       const uint32_t at = i % kPieces;
@@ -215,41 +217,57 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
       __syncwarp();
       if (!some) break;
-      for (int32_t u = 0; fine && u < walk.piece.count; ++u) {
-        const TileLoader<kKeys, kHalves> now = loader;
-        if (u + 1 < walk.piece.count) loader.look_up(walk.b, walk.piece, walk.piece.tile + u + 1);
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t slot = fills % kSlots;
-          fine = fine && barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kSlots) & 1u) ^ 1u, &C.gave_up);
-          if (!fine) break;
-          now.load(kv ? &P.v_map : &P.k_map, ring + slot * M::kTileBytes, walk.piece.head, smem_address(&C.full[slot]));
-          ++fills;
-          if (u == 0 && kv == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
+      for (int32_t u = 0; u < walk.piece.count; ++u) {
+        const uint32_t slot = fills % kPairs * 2u;
+        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+        if (!fine) break;
+        loader.load(&P.k_map, walk.piece.tile + u, ring + slot * M::kTileBytes, walk.piece.head, smem_address(&C.full[slot]));
+        ++fills;
+        if (u == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (walk.piece.to[t] <= walk.piece.from[t]) continue;
-              fine = fine && barrier_wait_warp(smem_address(&C.queries_free[t]), (query_loads[t] & 1u) ^ 1u, &C.gave_up);
-              if (!fine) break;
-              ++query_loads[t];
-              if (lane == 0) {
-                const uint32_t bar = smem_address(&C.queries[t]);
-                barrier_arrive_bytes(bar, half * 128u * kHalves);
-                const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
+          for (int t = 0; t < 2; ++t) {
+            if (walk.piece.to[t] <= walk.piece.from[t]) continue;
+            fine = fine && barrier_wait_warp(smem_address(&C.queries_free[t]), (query_loads[t] & 1u) ^ 1u, &C.gave_up);
+            if (!fine) break;
+            ++query_loads[t];
+            if (lane == 0) {
+              const uint32_t bar = smem_address(&C.queries[t]);
+              barrier_arrive_bytes(bar, half * 128u * kHalves);
+              const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-                  load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
-                               static_cast<int32_t>(walk.piece.head * P.group), token, bar);
-              }
-              __syncwarp();
+              for (int h = 0; h < kHalves; ++h)
+                load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
+                             static_cast<int32_t>(walk.piece.head * P.group), token, bar);
             }
+            __syncwarp();
           }
+          if (!fine) break;
         }
       }
-      walk.done();
     }
     if (lane == 0 && P.headers) walk.write_header();
+  } else if (warp == kValueWarp) {
+    TileLoader<kKeys, kHalves> loader(P);
+    for (uint32_t i = 0; fine; ++i) {
+      const uint32_t at = i % kPieces;
+      fine = barrier_wait_warp(smem_address(&C.told[at]), (i / kPieces) & 1u, &C.gave_up);
+      const Piece& piece = C.pieces[at];
+      if (!fine || piece.valid == 0) break;
+      const int32_t tile = piece.tile, count = piece.count;
+      const uint32_t head = piece.head;
+      loader.begin(piece);
+      __syncwarp();
+      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
+      for (int32_t u = 0; u < count; ++u) {
+        const uint32_t slot = fills % kPairs * 2u + 1u;
+        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+        if (!fine) break;
+        loader.load(&P.v_map, tile + u, ring + slot * M::kTileBytes, head, smem_address(&C.full[slot]));
+        ++fills;
+      }
+    }
   } else if (warp == kMmaWarp) {
-    uint32_t used = 0;               // ring slots taken before this piece
+    uint32_t used = 0;  // units before this piece
     uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0};
     const bool issuer = elected();
     constexpr uint32_t kScores = instruction<T>(kKeys, false), kOutput = instruction<T>(DIM, true);
@@ -263,15 +281,15 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
       // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
       for (int32_t u = first - 1; fine && u < end; ++u) {
-        const uint32_t v_fill = used + 2u * static_cast<uint32_t>(u - first) + 1u, k_fill = v_fill + 1u;
+        const uint32_t v_fill = used + static_cast<uint32_t>(u - first), k_fill = v_fill + 1u;
+        const uint32_t v_slot = v_fill % kPairs * 2u + 1u, k_slot = k_fill % kPairs * 2u;
         if (u >= first) {
-          const uint32_t slot = v_fill % kSlots;
-          fine = barrier_wait_warp(smem_address(&C.full[slot]), (v_fill / kSlots) & 1u, &C.gave_up);
+          fine = barrier_wait_warp(smem_address(&C.full[v_slot]), (v_fill / kPairs) & 1u, &C.gave_up);
           if (!fine) break;
           // value rows that no row sees may hold anything: 0 x NaN is not 0
           const int32_t key0 = u * kKeys;
           if (key0 < keys_begin || key0 + kKeys > keys_end) {
-            uint8_t* const tile = smem + M::kRing + slot * M::kTileBytes;
+            uint8_t* const tile = smem + M::kRing + v_slot * M::kTileBytes;
             for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
               const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
               if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
@@ -281,7 +299,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           }
         }
         if (u + 1 < end) {
-          fine = barrier_wait_warp(smem_address(&C.full[k_fill % kSlots]), (k_fill / kSlots) & 1u, &C.gave_up);
+          fine = barrier_wait_warp(smem_address(&C.full[k_slot]), (k_fill / kPairs) & 1u, &C.gave_up);
           if (!fine) break;
         }
 #pragma unroll
@@ -293,7 +311,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             probability_phase[t] ^= 1u;
             after_sync();
             if (issuer) {
-              const uint64_t v = operand(ring + (v_fill % kSlots) * M::kTileBytes, kKeys * 128 / 16);
+              const uint64_t v = operand(ring + v_slot * M::kTileBytes, kKeys * 128 / 16);
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k)
                 product_tensor(o, s + k * 8, v + k * (16 * 128 / 16), kOutput, k > 0 || u > from[t]);
@@ -310,7 +328,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             }
             if (issuer) {
               const uint64_t q = operand(base + t * M::kTileBytes, 1);
-              const uint64_t k_tile = operand(ring + (k_fill % kSlots) * M::kTileBytes, 1);
+              const uint64_t k_tile = operand(ring + k_slot * M::kTileBytes, 1);
 #pragma unroll
               for (int k = 0; k < DIM / 16; ++k) {
                 const uint32_t at = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
@@ -323,12 +341,12 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           }
         }
         if (issuer && fine) {
-          if (u >= first) commit(smem_address(&C.empty[v_fill % kSlots]));
-          if (u + 1 < end) commit(smem_address(&C.empty[k_fill % kSlots]));
+          if (u >= first) commit(smem_address(&C.empty[v_slot]));
+          if (u + 1 < end) commit(smem_address(&C.empty[k_slot]));
         }
         __syncwarp();
       }
-      used += 2u * static_cast<uint32_t>(end - first);
+      used += static_cast<uint32_t>(end - first);
       if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
     if (!fine) {
@@ -507,9 +525,9 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   before_sync();
   __syncthreads();
   after_sync();
-  if (C.gave_up && warp == kLoadWarp) {
-    for (uint32_t f = fills > kSlots ? fills - kSlots : 0u; f < fills; ++f)
-      barrier_wait_out(smem_address(&C.full[f % kSlots]), (f / kSlots) & 1u);
+  if (C.gave_up && (warp == kKeyWarp || warp == kValueWarp)) {
+    for (uint32_t f = fills > kPairs ? fills - kPairs : 0u; f < fills; ++f)
+      barrier_wait_out(smem_address(&C.full[f % kPairs * 2u + (warp - kKeyWarp)]), (f / kPairs) & 1u);
     if (lane == 0) atomicExch(P.status, 1u);
   }
   if (warp == kMmaWarp)
