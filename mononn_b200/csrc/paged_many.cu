@@ -106,6 +106,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+__device__ __forceinline__ void store_columns(uint32_t address, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::MONONN_I8(r, 0),
+      MONONN_I8(r, 8), MONONN_I8(r, 16), MONONN_I8(r, 24), "r"(address)
+      : "memory");
+}
 // the same for 16 columns
 __device__ __forceinline__ void load_columns_16(uint32_t address, uint32_t* r) {
   asm volatile(
@@ -128,12 +136,109 @@ __device__ __forceinline__ void store_columns_16(uint32_t address, const uint32_
 __device__ __forceinline__ void stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Columns that the row does not see: before `to`, and from `from` on.
-__device__ __forceinline__ void hide(uint32_t* s, int first, int32_t to, int32_t from) {
+__device__ __forceinline__ void hide(uint32_t (&s)[32], int32_t to, int32_t from) {
+  const uint32_t seen = (to <= 0 ? 0xffffffffu : to >= 32 ? 0u : 0xffffffffu << to) &
+                        (from <= 0 ? 0u : from >= 32 ? 0xffffffffu : ~(0xffffffffu << from));
 #pragma unroll
   for (int j = 0; j < 32; ++j)
-    if (first + j < to || first + j >= from) s[j] = 0xff800000u;
+    if (!(seen & (1u << j))) s[j] = 0xff800000u;
 }
-
+// Highest of 32 scores in four parts.
+__device__ __forceinline__ void highest_32(const uint32_t* s, float (&part)[4]) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[i] = max3(part[i], __uint_as_float(s[j + 2 * i]), __uint_as_float(s[j + 2 * i + 1]));
+}
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t multiply_add_two(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t multiply_two(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float at_least(float x, float low) {  // NaN stays NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
+  return r;
+}
+// Kept in its order, which is that of the loop below: the exponentials of one group beside the sums of the last.
+__device__ __forceinline__ float exp2_in_order(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^x for two x of at most 127 on the arithmetic pipes: 2^n from the integer nearest to x, times a polynomial of degree
+// 4 on -1/2 .. 1/2 (smallest largest relative error, 2.6e-6, found by exchange of its extrema). Below -126.5
+// it is 0, as for a key that is hidden.
+__device__ __forceinline__ float2 exp2_polynomial(uint64_t x) {
+  const float2 v = apart(x);
+  x = two(at_least(v.x, -127.f), at_least(v.y, -127.f));
+  const uint64_t moved = add_two(x, two(12582912.f, 12582912.f));  // 1.5 x 2^23: the integer is in the low bits
+  const uint64_t whole = add_two(moved, two(-12582912.f, -12582912.f));
+  const uint64_t f = multiply_add_two(whole, two(-1.f, -1.f), x);
+  uint64_t y = two(0.00957010191f, 0.00957010191f);
+  y = multiply_add_two(y, f, two(0.0559178603f, 0.0559178603f));
+  y = multiply_add_two(y, f, two(0.240247448f, 0.240247448f));
+  y = multiply_add_two(y, f, two(0.693121815f, 0.693121815f));
+  y = multiply_add_two(y, f, two(0.999999261f, 0.999999261f));
+  const float2 n = apart(moved);
+  return apart(multiply_two(y, two(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
+                                   __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u))));
+}
+// The probabilities exp2(scale x s + shift) of 32 scores, rounded to T once and stored from column `at` on, and their sum.
+// The special-function units take 8 cycles for the exponentials of a warp and bound this loop: one of eight goes to
+// the arithmetic pipes instead, which have time left.
+template <typename T>
+__device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t at, uint64_t scales, uint64_t shifts, uint64_t (&sum)[2]) {
+  uint32_t p[16];
+#pragma unroll
+  for (int g = 0; g <= 4; ++g) {
+    if (g < 4) {
+#pragma unroll
+      for (int j = g * 8; j < g * 8 + 8; j += 2) {
+        const uint64_t x = multiply_add_two(two(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), scales, shifts);
+        float2 e = apart(x);
+        if (j % 16 == 14) {
+          e = exp2_polynomial(x);
+        } else {
+          e.x = exp2_in_order(e.x);
+          e.y = exp2_in_order(e.y);
+        }
+        s[j] = __float_as_uint(e.x);
+        s[j + 1] = __float_as_uint(e.y);
+      }
+    }
+    if (g > 0) {
+      const int h = g - 1;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float a = __uint_as_float(s[h * 8 + j]), b = __uint_as_float(s[h * 8 + j + 1]);
+        sum[(j >> 1) & 1] = add_two(sum[(j >> 1) & 1], two(a, b));
+        p[h * 4 + j / 2] = Pair<T>::pack(a, b);
+      }
+    }
+  }
+  store_columns_16(at, p);  // over scores that have been read
+}
 // The key tiles of a piece that hold keys which some row of row tile t sees.
 __device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
   const uint32_t half = P.item_rows / 2;
@@ -392,24 +497,35 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           after_sync();
           const int32_t key0 = u * kKeys;
           const bool tested = key0 < all_from || key0 + kKeys > all_to;
-          const int32_t hide_to = see_from - key0, hide_from = see_to - key0;
-          uint32_t s[kKeys];
-#pragma unroll
-          for (int i = 0; i < kKeys; i += 32) load_columns(s_at + i, s + i);
-          loads_done(s);
-#pragma unroll
-          for (int i = 32; i < kKeys; i += 32) loaded(s + i);
+          // The code of a unit is kept small (it is run by eight warps beside four others' that differ): the scores are
+          // read twice, for the maximum and for the probabilities, and hidden ones are put back as such.
+          float part[4] = {ninf, ninf, ninf, ninf};
+          uint32_t s[32], other[32];
           if (tested) {
-#pragma unroll
-            for (int i = 0; i < kKeys; i += 32) hide(s + i, i, hide_to, hide_from);
+#pragma unroll 1
+            for (int i = kKeys - 32; i >= 0; i -= 32) {
+              load_columns(s_at + i, s);
+              loads_done(s);
+              hide(s, see_from - key0 - i, see_to - key0 - i);
+              highest_32(s, part);
+              store_columns(s_at + i, s);
+            }
+            stores_done();
+          } else {
+            uint32_t rest[64];
+            load_columns(s_at, s);
+            load_columns(s_at + 32, other);
+            load_columns(s_at + 64, rest);
+            load_columns(s_at + 96, rest + 32);
+            loads_done(s);
+            loaded(other);
+            loaded(rest);
+            loaded(rest + 32);
+            highest_32(s, part);
+            highest_32(other, part);
+            highest_32(rest, part);
+            highest_32(rest + 32, part);
           }
-          float part[4] = {__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]), __uint_as_float(s[3])};
-#pragma unroll
-          for (int j = 4; j < kKeys; j += 8)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              part[i] = j + 4 < kKeys ? max3(part[i], __uint_as_float(s[j + i]), __uint_as_float(s[j + 4 + i]))
-                                      : fmaxf(part[i], __uint_as_float(s[j + i]));
           const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
           if (u == from) {
             m = top;
@@ -433,20 +549,19 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             }
           }
           const float shift = m == ninf ? 0.f : m * P.scale_log2;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < kKeys; i += 32) {
-            uint32_t p[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float a = exp2_fast(fmaf(__uint_as_float(s[i + 2 * j]), P.scale_log2, -shift));
-              const float b = exp2_fast(fmaf(__uint_as_float(s[i + 2 * j + 1]), P.scale_log2, -shift));
-              sum[j & 3] += a + b;
-              p[j] = Pair<T>::pack(a, b);  // one rounding to the values' type
-            }
-            store_columns_16(s_at + i / 2, p);  // over scores that have been read
+          const uint64_t scales = two(P.scale_log2, P.scale_log2), shifts = two(-shift, -shift);
+          uint64_t sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+#pragma unroll 1
+          for (int i = 0; i < kKeys; i += 64) {
+            load_columns(s_at + i + 32, other);
+            probabilities<T>(s, s_at + i / 2, scales, shifts, sum);
+            loads_done(other);
+            if (i == 0) load_columns(s_at + 64, s);
+            probabilities<T>(other, s_at + i / 2 + 16, scales, shifts, sum);
+            loads_done(s);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          const float2 sums = apart(add_two(sum[0], sum[1]));
+          l += sums.x + sums.y;
           stores_done();
           before_sync();
           __syncwarp();

@@ -130,10 +130,11 @@ class Problem:
                 p = p.reshape(q.shape[1], n, 0)
             o = torch.einsum("hqk,khd->qhd", p, vv)
             size = torch.einsum("hqk,khd->qhd", p, vv.abs())
-            # a score is a 32-bit sum of dim products, at worst each of them rounded; then scale and exponent
+            # a score is a 32-bit sum of dim products, at worst each of them rounded; then scale and exponent. An
+            # exponential is off by 2^-22 of itself, or 2.6e-6 + a few 2^-24 < 2^-18 where a polynomial makes it.
             terms = terms.masked_fill(~see, 0.0)
             worst = terms.amax(-1) if self.lens[b] else torch.zeros(q.shape[1], n, device=device, dtype=torch.float64)
-            off = worst * (self.dim + 4) * 2.0 ** -24 + 2.0 ** -20
+            off = worst * (self.dim + 4) * 2.0 ** -24 + 2.0 ** -18
             off_o = off.permute(1, 0)[..., None]
             limit = u(self.dtype) * o.abs() + (u(self.dtype) + 2 * off_o) * (1 + u(self.dtype)) * size + tiny(self.dtype)
             if self.dtype == torch.float16:  # probabilities below the type's normal range
