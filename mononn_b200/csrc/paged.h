@@ -29,7 +29,7 @@ struct RowsParams {
   const int32_t* table;
   int64_t table_stride, page_stride;
   uint32_t tokens, head_dim, sequences, max_pages, num_pages, page_size;
-  uint32_t rotary_dim, interleaved;
+  uint32_t rotary_dim, interleaved, block_tokens;
   float magnitude;
   double turns[128];
 };

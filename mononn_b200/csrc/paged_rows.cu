@@ -10,6 +10,7 @@ namespace mononn {
 namespace paged {
 
 constexpr int kRowsThreads = 256;
+constexpr uint32_t kRowsTokens = 4;  // of a block, at most
 
 // V elements at once, of type T
 template <typename T, int V>
@@ -60,116 +61,159 @@ __device__ __forceinline__ uint32_t sequence_of(const int32_t* indptr, uint32_t 
   return low;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void rotate_heads(const RowsSource& s, const T* src, T* dst, uint32_t rd, uint32_t dim,
-                                             bool interleaved, const float* cosines, const float* sines) {
-  // of each head: pieces that are rotated, then pieces that are copied
-  const uint32_t turned = interleaved ? (V == 8 ? rd / 8 : rd / 2) : rd / 2 / V;
-  const uint32_t each = turned + (dim - rd) / V;
-  if (each == 0) return;
-  if (threadIdx.x >= each * (kRowsThreads / each) && each <= kRowsThreads) return;
-  const uint32_t step = each <= kRowsThreads ? kRowsThreads / each : 1u;
-  const uint32_t head0 = each <= kRowsThreads ? threadIdx.x / each : 0u;
-  for (uint32_t j = each <= kRowsThreads ? threadIdx.x % each : threadIdx.x; j < each; j += kRowsThreads) {
-    if (j >= turned) {
-      const uint32_t d = rd + (j - turned) * V;
-      for (uint32_t h = head0; h < s.heads; h += step) {
-        Vector<T, V> a;
-        a.load(src + h * s.src_head + d);
-        a.store(dst + h * s.dst_head + d);
-      }
-    } else if (interleaved && V == 8) {
-      for (uint32_t h = head0; h < s.heads; h += step) {
-        Vector<T, V> a;
-        a.load(src + h * s.src_head + j * V);
-        float x[V], y[V];
-        a.get(x);
+// What a block knows of its tokens.
+struct RowsShared {
+  float cosines[kRowsTokens][128], sines[kRowsTokens][128];
+  int64_t page_at[kRowsTokens];  // of the token's row in the pages, in elements; below 0: none
+  int32_t position[kRowsTokens];
+  bool member[kRowsTokens];      // of some sequence
+};
+enum RowsMode { kCopy, kPairs, kNeighbours };
+
+// The vectors `first` .. `first` + each - 1 of every head of every token of a block, a thread to a vector: consecutive
+// threads along a head, then along heads and tokens. 64 bytes of each thread are on their way at a time.
+template <typename T, int V, RowsMode MODE>
+__device__ __forceinline__ void move_rows(const RowsSource& s, const RowsShared& S, uint32_t token0, uint32_t tokens,
+                                          bool to_pages, uint32_t first, uint32_t each, uint32_t rd) {
+  if (each == 0 || s.heads == 0) return;
+  for (uint32_t j0 = 0; j0 < each; j0 += kRowsThreads) {
+    const uint32_t wide = min(each - j0, static_cast<uint32_t>(kRowsThreads));
+    const uint32_t step = kRowsThreads / wide;  // rows at once
+    if (threadIdx.x >= step * wide) continue;
+    const uint32_t j = j0 + threadIdx.x % wide;
+    // element of the vector, and of its partner
+    const uint32_t d0 = MODE == kCopy ? first + j * V : MODE == kPairs ? j * V : (V == 8 ? j * V : 2 * j);
+    const uint32_t d1 = MODE == kPairs ? rd / 2 + j * V : 2 * j + 1;
+    constexpr bool kTwo = MODE == kPairs || (MODE == kNeighbours && V == 1);
+    uint32_t t = threadIdx.x / wide / s.heads, h = threadIdx.x / wide % s.heads;
+    const uint32_t step_t = step / s.heads, step_h = step % s.heads;
+    constexpr int kAtOnce = kTwo ? 2 : 4;
+    while (t < tokens) {
+      Vector<T, V> a[kAtOnce], b[kAtOnce];
+      T* to[kAtOnce];
+      uint32_t of[kAtOnce];
 #pragma unroll
-        for (int i = 0; i + 1 < V; i += 2) {
-          const float c = cosines[j * (V / 2) + i / 2], n = sines[j * (V / 2) + i / 2];
-          y[i] = x[i] * c - x[i + 1] * n;
-          y[i + 1] = x[i + 1] * c + x[i] * n;
+      for (int u = 0; u < kAtOnce; ++u) {
+        to[u] = nullptr;
+        of[u] = t;
+        if (t < tokens && (to_pages ? S.page_at[t] >= 0 : S.member[t])) {
+          const int64_t token = token0 + t;
+          const T* from = static_cast<const T*>(s.src) + token * s.src_token + h * s.src_head;
+          to[u] = static_cast<T*>(s.dst) + (to_pages ? S.page_at[t] : token * s.dst_token) + h * s.dst_head;
+          a[u].load(from + d0);
+          if (kTwo) b[u].load(from + d1);
         }
-        a.set(y);
-        a.store(dst + h * s.dst_head + j * V);
+        t += step_t;
+        h += step_h;
+        if (h >= s.heads) h -= s.heads, ++t;
       }
-    } else {
-      const uint32_t d0 = interleaved ? 2 * j : j * V, d1 = interleaved ? 2 * j + 1 : rd / 2 + j * V;
-      for (uint32_t h = head0; h < s.heads; h += step) {
-        Vector<T, V> a, b;
-        a.load(src + h * s.src_head + d0);
-        b.load(src + h * s.src_head + d1);
-        float x[V], y[V], u[V], w[V];
-        a.get(x);
-        b.get(y);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float c = cosines[j * V + i], n = sines[j * V + i];
-          u[i] = x[i] * c - y[i] * n;
-          w[i] = y[i] * c + x[i] * n;
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (to[u] == nullptr) continue;
+        const float* cosines = S.cosines[of[u]];
+        const float* sines = S.sines[of[u]];
+        if constexpr (MODE == kNeighbours && V == 8) {
+          float x[V], y[V];
+          a[u].get(x);
+          const float4 c = *reinterpret_cast<const float4*>(cosines + j * 4), n = *reinterpret_cast<const float4*>(sines + j * 4);
+          const float cs[4] = {c.x, c.y, c.z, c.w}, ns[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+          for (int i = 0; i < V; i += 2) {
+            y[i] = x[i] * cs[i / 2] - x[i + 1] * ns[i / 2];
+            y[i + 1] = x[i + 1] * cs[i / 2] + x[i] * ns[i / 2];
+          }
+          a[u].set(y);
+        } else if constexpr (kTwo) {
+          float x[V], y[V], p[V], q[V];
+          a[u].get(x);
+          b[u].get(y);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float c = cosines[j * V + i], n = sines[j * V + i];
+            p[i] = x[i] * c - y[i] * n;
+            q[i] = y[i] * c + x[i] * n;
+          }
+          a[u].set(p);
+          b[u].set(q);
+          b[u].store(to[u] + d1);
         }
-        a.set(u);
-        b.set(w);
-        a.store(dst + h * s.dst_head + d0);
-        b.store(dst + h * s.dst_head + d1);
+        a[u].store(to[u] + d0);
       }
     }
   }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kRowsThreads) rows_kernel(const __grid_constant__ RowsParams P) {
-  __shared__ float cosines[128], sines[128];
+__global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_constant__ RowsParams P) {
+  __shared__ RowsShared S;
   let_next_begin();
   earlier_done();
-  const uint32_t token = blockIdx.x;
-  int64_t page_at = -1;  // of the token's row, in elements
-  int32_t position = 0;
-  bool member = true;
-  if (P.indptr) {
-    const uint32_t b = sequence_of(P.indptr, P.sequences, static_cast<int32_t>(token));
-    member = b < P.sequences && P.indptr[b] <= static_cast<int32_t>(token);
-    if (member) {
-      const int32_t begin = P.indptr[b], end = P.indptr[b + 1];
-      const int64_t at = static_cast<int64_t>(P.lengths[b]) - (static_cast<int64_t>(end) - begin) + (token - begin);
-      position = static_cast<int32_t>(at);
-      if (at >= 0 && at < static_cast<int64_t>(P.max_pages) * P.page_size) {
-        const uint32_t n = static_cast<uint32_t>(at) / P.page_size;
-        const int32_t page = P.table[static_cast<int64_t>(b) * P.table_stride + n];
-        if (page >= 0 && static_cast<uint32_t>(page) < P.num_pages)
-          page_at = page * P.page_stride + static_cast<int64_t>(static_cast<uint32_t>(at) - n * P.page_size) * P.k.dst_token;
+  const uint32_t token0 = blockIdx.x * P.block_tokens, tokens = min(P.block_tokens, P.tokens - token0);
+  const uint32_t warp = threadIdx.x >> 5;
+  if (warp < tokens) {  // a warp to a token
+    const uint32_t token = token0 + warp;
+    int64_t page_at = -1;
+    int32_t position = 0;
+    bool member = true;
+    if (P.indptr) {
+      const uint32_t b = sequence_of(P.indptr, P.sequences, static_cast<int32_t>(token));
+      member = b < P.sequences;
+      if (member) {
+        const int32_t begin = P.indptr[b], end = P.indptr[b + 1], length = P.lengths[b];
+        member = begin <= static_cast<int32_t>(token);
+        const int64_t at = static_cast<int64_t>(length) - (static_cast<int64_t>(end) - begin) + (static_cast<int64_t>(token) - begin);
+        position = static_cast<int32_t>(at);
+        if (member && at >= 0 && at < static_cast<int64_t>(P.max_pages) * P.page_size) {
+          const uint32_t n = static_cast<uint32_t>(at) / P.page_size;
+          const int32_t page = P.table[static_cast<int64_t>(b) * P.table_stride + n];
+          if (page >= 0 && static_cast<uint32_t>(page) < P.num_pages)
+            page_at = page * P.page_stride + static_cast<int64_t>(static_cast<uint32_t>(at) - n * P.page_size) * P.k.dst_token;
+        }
       }
     }
-  }
-  if (!member) return;
-  if (P.rotary_dim) {
     if (P.positions) position = P.positions[token];
-    if (threadIdx.x < P.rotary_dim / 2) {
-      const double turns = position * P.turns[threadIdx.x];
-      const float part = static_cast<float>(2.0 * (turns - rint(turns)));
+    if ((threadIdx.x & 31u) == 0u) {
+      S.page_at[warp] = page_at;
+      S.position[warp] = position;
+      S.member[warp] = member;
+    }
+  }
+  __syncthreads();
+  const uint32_t rd = P.rotary_dim, pairs = rd / 2;
+  if (rd) {
+    for (uint32_t i = threadIdx.x; i < tokens * 128; i += kRowsThreads) {
+      const uint32_t t = i >> 7, p = i & 127u;
+      if (p >= pairs) continue;
+      const double turns = S.position[t] * P.turns[p];
       float s, c;
-      sincospif(part, &s, &c);
-      cosines[threadIdx.x] = c * P.magnitude;
-      sines[threadIdx.x] = s * P.magnitude;
+      sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
+      S.cosines[t][p] = c * P.magnitude;
+      S.sines[t][p] = s * P.magnitude;
     }
     __syncthreads();
+    if (P.interleaved) {
+      const uint32_t n = V == 8 ? rd / 8 : pairs;
+      move_rows<T, V, kNeighbours>(P.q, S, token0, tokens, false, 0, n, rd);
+      move_rows<T, V, kNeighbours>(P.k, S, token0, tokens, true, 0, n, rd);
+    } else {
+      move_rows<T, V, kPairs>(P.q, S, token0, tokens, false, 0, pairs / V, rd);
+      move_rows<T, V, kPairs>(P.k, S, token0, tokens, true, 0, pairs / V, rd);
+    }
   }
-  if (P.q.heads)
-    rotate_heads<T, V>(P.q, static_cast<const T*>(P.q.src) + token * P.q.src_token,
-                       static_cast<T*>(P.q.dst) + token * P.q.dst_token, P.rotary_dim, P.head_dim, P.interleaved != 0,
-                       cosines, sines);
-  if (page_at >= 0) {
-    rotate_heads<T, V>(P.k, static_cast<const T*>(P.k.src) + token * P.k.src_token, static_cast<T*>(P.k.dst) + page_at,
-                       P.rotary_dim, P.head_dim, P.interleaved != 0, cosines, sines);
-    rotate_heads<T, V>(P.v, static_cast<const T*>(P.v.src) + token * P.v.src_token, static_cast<T*>(P.v.dst) + page_at,
-                       0, P.head_dim, false, cosines, sines);
+  if (rd < P.head_dim) {
+    move_rows<T, V, kCopy>(P.q, S, token0, tokens, false, rd, (P.head_dim - rd) / V, rd);
+    move_rows<T, V, kCopy>(P.k, S, token0, tokens, true, rd, (P.head_dim - rd) / V, rd);
   }
+  move_rows<T, V, kCopy>(P.v, S, token0, tokens, true, 0, P.head_dim / V, rd);
 }
 
 }  // namespace paged
 
-cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int, cudaStream_t stream) {
-  auto launch = [&](auto kernel) { return launch_dependent(kernel, dim3(p.tokens), paged::kRowsThreads, 0, p, stream); };
+cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int sm_count, cudaStream_t stream) {
+  RowsParams p = params;
+  p.block_tokens = p.tokens >= 4u * static_cast<unsigned>(sm_count) ? paged::kRowsTokens : 1u;
+  const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens);
+  auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, paged::kRowsThreads, 0, p, stream); };
   if (bf16) return vectors ? launch(paged::rows_kernel<__nv_bfloat16, 8>) : launch(paged::rows_kernel<__nv_bfloat16, 1>);
   return vectors ? launch(paged::rows_kernel<__half, 8>) : launch(paged::rows_kernel<__half, 1>);
 }
