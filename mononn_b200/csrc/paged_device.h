@@ -32,24 +32,20 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0u;
 }
-__device__ __forceinline__ uint64_t timer_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+__device__ __forceinline__ uint32_t clock_now() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
   return t;
 }
-// Bounded: after two seconds the CTA gives up, and so do all its other waits.
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
-// Inline everywhere: a call would hold its caller to the registers of the launch.
+// Bounded: after 2^31 cycles, about a second, the CTA gives up, and so do all its other waits. Inline
+// everywhere (a call would hold its caller to the registers of the launch), so it is kept small.
+constexpr uint32_t kWaitLimit = 1u << 31;
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up) {
   if (barrier_try(bar, parity)) return true;
-  uint64_t t0 = 0;
+  const uint32_t t0 = clock_now();
 #pragma unroll 1
-  for (uint32_t it = 1; !barrier_try(bar, parity); ++it) {
-    if ((it & 63u) != 0u) continue;
-    if (*gave_up) return false;
-    const uint64_t now = timer_ns();
-    if (t0 == 0) t0 = now;
-    if (now - t0 > kWaitLimitNs) {
+  while (!barrier_try(bar, parity)) {
+    if (*gave_up || clock_now() - t0 >= kWaitLimit) {
       *gave_up = 1u;
       return false;
     }
@@ -58,8 +54,9 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
 }
 // On the way out after that: copies of this CTA that are still in flight, bounded again.
 __device__ __forceinline__ void barrier_wait_out(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = timer_ns();
-  while (!barrier_try(bar, parity) && timer_ns() - t0 <= kWaitLimitNs) {
+  const uint32_t t0 = clock_now();
+#pragma unroll 1
+  while (!barrier_try(bar, parity) && clock_now() - t0 < kWaitLimit) {
   }
 }
 // The whole warp gets the same answer.
@@ -173,6 +170,7 @@ __device__ __forceinline__ uint32_t item_units(const AttentionParams& P, const S
 template <int KEYS>
 __device__ __forceinline__ uint32_t head_units_warp(const AttentionParams& P, const Sequence& s, uint32_t tiles) {
   uint32_t part = 0;
+#pragma unroll 1
   for (uint32_t t = threadIdx.x & 31u; t < tiles; t += 32u) part += item_units<KEYS>(P, s, t);
   return __reduce_add_sync(0xffffffffu, part);
 }
@@ -197,13 +195,16 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
   const uint32_t b0 = warp * per_warp + lane * each;
   uint32_t mine = 0;
   Sequence s{0, 0, 0};
+#pragma unroll 1
   for (uint32_t i = 0; i < each; ++i) {
     s = Sequence{0, 0, 0};
     if (b0 + i < end) s = load_sequence(P, b0 + i);
     const uint32_t tiles = row_tiles(P, s);
     uint32_t u = 0;
     if (tiles <= 2u)
+#pragma unroll 1
       for (uint32_t t = 0; t < tiles; ++t) u += item_units<KEYS>(P, s, t);
+#pragma unroll 1
     for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 2u); many; many &= many - 1u) {
       const int from = __ffs(many) - 1;
       const Sequence o{0, __shfl_sync(0xffffffffu, s.n, from), __shfl_sync(0xffffffffu, s.length, from)};
@@ -241,6 +242,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
       s.n = __shfl_sync(0xffffffffu, s.n, from);
       s.length = __shfl_sync(0xffffffffu, s.length, from);
       uint32_t per_head = 0;
+#pragma unroll 1
       for (;;) {
         if (each > 1u) s = load_sequence(P, b);
         per_head = head_units_warp<KEYS>(P, s, row_tiles(P, s));
@@ -251,6 +253,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
       const uint32_t head = (u0 - at) / per_head;
       uint32_t left = u0 - at - head * per_head, tile = 0;
       const uint32_t tiles = row_tiles(P, s);
+#pragma unroll 1
       for (uint32_t t0 = 0;; t0 += 32u) {
         const uint32_t u = t0 + lane < tiles ? item_units<KEYS>(P, s, t0 + lane) : 0u;
         uint32_t sum = u;

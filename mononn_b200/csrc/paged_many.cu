@@ -2,11 +2,11 @@
 //
 // The same one pass over the keys as the kernel for few rows, on the fifth-generation tensor cores. An item has
 // up to 256 rows, two tiles of 128; a unit is 128 keys, loaded once for both. Roles of a CTA (one per SM):
-//   warps 0-3, 4-7  the softmax of one row tile each, a thread to a row: scores from tensor memory,
+//   warps 4-7, 8-11 the softmax of one row tile each, a thread to a row: scores from tensor memory,
 //                   running maximum, probabilities back to tensor memory, row sums in registers
-//   warp 8          issues the matrix products: S = Q K^T (both operands in shared memory), O += P V (P in
+//   warp 0          issues the matrix products: S = Q K^T (both operands in shared memory), O += P V (P in
 //                   tensor memory, in the place of the scores it was made from)
-//   warps 9, 10     load keys (and queries) and values, page by page, into a ring of tiles
+//   warps 1, 2      load keys (and queries) and values, page by page, into a ring of tiles
 // While one row tile's softmax runs, the tensor cores work on the other's products.
 // O stays in tensor memory. It is rescaled only when a row's maximum has risen by more than
 // 2^8 since its reference was set: until then probabilities are above 1, by 2^8 at most, which costs no accuracy.
@@ -17,7 +17,7 @@ namespace paged {
 
 constexpr int kRows = static_cast<int>(kManyRows), kKeys = static_cast<int>(kManyKeys);
 constexpr int kThreadsMany = 384;
-constexpr int kMmaWarp = 8, kKeyWarp = 9, kValueWarp = 10;  // 11 only makes up the group whose registers go to the others
+constexpr int kMmaWarp = 0, kKeyWarp = 1, kValueWarp = 2, kSoftmaxWarp = 4;  // 3 only makes up the group whose registers go to the others
 constexpr int kPieces = 4;                  // told ahead
 constexpr uint32_t kSoftmaxRegisters = 216, kOtherRegisters = 72, kLaunchRegisters = 168;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreadsMany * kLaunchRegisters, "register split");
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   uint32_t fills = 0;  // of this loading warp
   bool fine = true;
   // Each group of warps within its own branch: code behind a meeting of both is held to the fewer registers.
-  if (warp >= kMmaWarp) {
+  if (warp < kSoftmaxWarp) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
   if (warp == kKeyWarp) {
     TileLoader<kKeys, kHalves> loader(P);
@@ -462,13 +462,13 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   } else {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
   {
-    const uint32_t t = warp >> 2, thread = threadIdx.x & 127u;
+    const uint32_t t = (warp - kSoftmaxWarp) >> 2, thread = threadIdx.x & 127u;
     const uint32_t lanes = (warp & 3u) << 21;  // this warp's rows of tensor memory: lane 32 x (warp & 3), bits 16 up
     const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
     const float ninf = __int_as_float(0xff800000);
     uint32_t score_phase = 0, output_phase = 0;
     const uint32_t half = P.item_rows / 2;
-    uint8_t* const stage = smem + M::kStage + warp * 4096;
+    uint8_t* const stage = smem + M::kStage + (warp - kSoftmaxWarp) * 4096;
     for (uint32_t n = 0;; ++n) {
       const uint32_t at = n % kPieces;
       fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
