@@ -26,15 +26,22 @@ constexpr float kRise = 8.0f;  // in powers of two
 template <int DIM>
 struct ManySmem {
   static constexpr int kTileBytes = static_cast<int>(kTileRows) * DIM * 2;  // of queries, keys or values
-  static constexpr int kSlots = DIM == 64 ? 8 : 4;
+  // A slot of the ring holds the values of one unit and the keys of the next: what one step of the products needs.
+  static constexpr int kPairs = DIM == 64 ? 4 : 2;
   static constexpr int kRing = 2 * kTileBytes;
-  static constexpr int kStage = kRing + kSlots * kTileBytes;  // 4 KB of each softmax warp, for its rows' way out
+  static constexpr int kStage = kRing + 2 * kPairs * kTileBytes;  // 4 KB of each softmax warp, for its rows' way out
   static constexpr int kControl = kStage + 8 * 4096;
   static constexpr int kBytes = kControl + 1024;
+  // Tensor memory, 512 columns: 128 of scores and DIM of outputs for each row tile. The probabilities (64
+  // columns) have a place of their own where DIM leaves one, otherwise that of the scores.
+  static constexpr bool kApart = DIM == 64;
+  static __device__ __forceinline__ uint32_t score_column(uint32_t t) { return t * 128; }
+  static __device__ __forceinline__ uint32_t probability_column(uint32_t t) { return kApart ? 256 + t * 64 : t * 128; }
+  static __device__ __forceinline__ uint32_t output_column(uint32_t t) { return kApart ? 384 + t * 64 : 256 + t * 128; }
 };
 struct ManyControl {
-  uint64_t full[8], empty[8];
-  uint64_t scores[2], probabilities[2], queries[2], queries_free[2], outputs[2], told[kPieces], taken[kPieces], drained;
+  uint64_t full[4], empty[4];  // of pairs
+  uint64_t scores[2], scores_read[2], probabilities[2], queries[2], queries_free[2], outputs[2], told[kPieces], taken[kPieces], drained;
   alignas(16) Piece pieces[kPieces];
   Share share;
   uint32_t sums[12];
@@ -258,19 +265,21 @@ template <typename T, int DIM>
 __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t raw[];
   using M = ManySmem<DIM>;
-  constexpr int kHalves = DIM / 64, kSlots = M::kSlots;
+  constexpr int kHalves = DIM / 64;
+  constexpr bool kApart = M::kApart;
   uint8_t* smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
   ManyControl& C = *reinterpret_cast<ManyControl*>(smem + M::kControl);
   const uint32_t base = smem_address(smem), ring = base + M::kRing;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) {
-      barrier_init(smem_address(&C.full[i]), 1);
+    for (int i = 0; i < M::kPairs; ++i) {
+      barrier_init(smem_address(&C.full[i]), 2);
       barrier_init(smem_address(&C.empty[i]), 1);
     }
     for (int t = 0; t < 2; ++t) {
       barrier_init(smem_address(&C.scores[t]), 1);
+      barrier_init(smem_address(&C.scores_read[t]), 4);
       barrier_init(smem_address(&C.probabilities[t]), 4);
       barrier_init(smem_address(&C.queries[t]), 1);
       barrier_init(smem_address(&C.queries_free[t]), 1);
@@ -297,8 +306,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   find_share<kKeys, kThreadsMany>(P, C.sums, &C.share);  // barriers of the CTA within
   after_sync();
   const uint32_t tmem = *const_cast<volatile uint32_t*>(&C.tmem);
-  // Slots 0, 2, .. of the ring hold keys, 1, 3, .. values.
-  constexpr uint32_t kPairs = kSlots / 2;
+  constexpr uint32_t kPairs = M::kPairs;
   uint32_t fills = 0;  // of this loading warp
   bool fine = true;
   // Each group of warps within its own branch: code behind a meeting of both is held to the fewer registers.
@@ -322,12 +330,17 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
       __syncwarp();
       if (!some) break;
-      for (int32_t u = 0; u < walk.piece.count; ++u) {
-        const uint32_t slot = fills % kPairs * 2u;
+      for (int32_t u = 0; u <= walk.piece.count; ++u) {
+        const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
         fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
         if (!fine) break;
-        loader.load(&P.k_map, walk.piece.tile + u, ring + slot * M::kTileBytes, walk.piece.head, smem_address(&C.full[slot]));
         ++fills;
+        if (u == walk.piece.count) {  // the last values come alone
+          if (lane == 0) barrier_arrive(full);
+          __syncwarp();
+          break;
+        }
+        loader.load(&P.k_map, walk.piece.tile + u, ring + slot * 2u * M::kTileBytes, walk.piece.head, full);
         if (u == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -363,17 +376,22 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       loader.begin(piece);
       __syncwarp();
       if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
-      for (int32_t u = 0; u < count; ++u) {
-        const uint32_t slot = fills % kPairs * 2u + 1u;
+      for (int32_t u = -1; u < count; ++u) {
+        const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
         fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
         if (!fine) break;
-        loader.load(&P.v_map, tile + u, ring + slot * M::kTileBytes, head, smem_address(&C.full[slot]));
         ++fills;
+        if (u < 0) {  // the first keys come alone
+          if (lane == 0) barrier_arrive(full);
+          __syncwarp();
+        } else {
+          loader.load(&P.v_map, tile + u, ring + (slot * 2u + 1u) * M::kTileBytes, head, full);
+        }
       }
     }
   } else if (warp == kMmaWarp) {
-    uint32_t used = 0;  // units before this piece
-    uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0};
+    uint32_t step = 0;  // slots of the ring taken so far
+    uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0}, read_phase[2] = {1, 1};
     const bool issuer = elected();
     constexpr uint32_t kScores = instruction<T>(kKeys, false), kOutput = instruction<T>(DIM, true);
     for (uint32_t n = 0; fine; ++n) {
@@ -386,72 +404,68 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
       // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
       for (int32_t u = first - 1; fine && u < end; ++u) {
-        const uint32_t v_fill = used + static_cast<uint32_t>(u - first), k_fill = v_fill + 1u;
-        const uint32_t v_slot = v_fill % kPairs * 2u + 1u, k_slot = k_fill % kPairs * 2u;
-        if (u >= first) {
-          fine = barrier_wait_warp(smem_address(&C.full[v_slot]), (v_fill / kPairs) & 1u, &C.gave_up);
-          if (!fine) break;
-          // value rows that no row sees may hold anything: 0 x NaN is not 0
-          const int32_t key0 = u * kKeys;
-          if (key0 < keys_begin || key0 + kKeys > keys_end) {
-            uint8_t* const tile = smem + M::kRing + v_slot * M::kTileBytes;
-            for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
-              const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
-              if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
-            }
-            shared_to_async();
-            __syncwarp();
+        const uint32_t slot = step % kPairs;
+        const uint32_t k_at = ring + slot * 2u * M::kTileBytes, v_at = k_at + M::kTileBytes;
+        fine = barrier_wait_warp(smem_address(&C.full[slot]), (step / kPairs) & 1u, &C.gave_up);
+        if (!fine) break;
+        ++step;
+        // value rows that no row sees may hold anything: 0 x NaN is not 0
+        const int32_t key0 = u * kKeys;
+        if (u >= first && (key0 < keys_begin || key0 + kKeys > keys_end)) {
+          uint8_t* const tile = smem + (v_at - base);
+          for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
+            const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
+            if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
           }
+          shared_to_async();
+          __syncwarp();
         }
-        if (u + 1 < end) {
-          fine = barrier_wait_warp(smem_address(&C.full[k_slot]), (k_fill / kPairs) & 1u, &C.gave_up);
-          if (!fine) break;
-        }
+        auto weigh = [&](int t) {  // O += P V of unit u; false after a wait that gave up
+          if (u < from[t] || u >= to[t]) return true;
+          if (!barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up)) return false;
+          probability_phase[t] ^= 1u;
+          after_sync();
+          if (issuer) {
+            const uint64_t v = operand(v_at, kKeys * 128 / 16);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t s = tmem + t * 128, o = tmem + 256 + t * 128;
-          if (u >= from[t] && u < to[t]) {
-            fine = fine && barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up);
-            if (!fine) break;
-            probability_phase[t] ^= 1u;
-            after_sync();
-            if (issuer) {
-              const uint64_t v = operand(ring + v_slot * M::kTileBytes, kKeys * 128 / 16);
-#pragma unroll
-              for (int k = 0; k < kKeys / 16; ++k)
-                product_tensor(o, s + k * 8, v + k * (16 * 128 / 16), kOutput, k > 0 || u > from[t]);
-              if (u + 1 == to[t]) commit(smem_address(&C.outputs[t]));
-            }
-            __syncwarp();
+            for (int k = 0; k < kKeys / 16; ++k)
+              product_tensor(tmem + M::output_column(t), tmem + M::probability_column(t) + k * 8, v + k * (16 * 128 / 16),
+                             kOutput, k > 0 || u > from[t]);
+            if (kApart || u + 1 == to[t]) commit(smem_address(&C.outputs[t]));
           }
-          if (u + 1 >= from[t] && u + 1 < to[t]) {
-            if (u + 1 == from[t]) {
-              fine = fine && barrier_wait_warp(smem_address(&C.queries[t]), query_phase[t], &C.gave_up);
-              if (!fine) break;
-              query_phase[t] ^= 1u;
-              after_sync();
-            }
-            if (issuer) {
-              const uint64_t q = operand(base + t * M::kTileBytes, 1);
-              const uint64_t k_tile = operand(ring + k_slot * M::kTileBytes, 1);
-#pragma unroll
-              for (int k = 0; k < DIM / 16; ++k) {
-                const uint32_t at = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
-                product_shared(s, q + at, k_tile + at, kScores, k > 0);
-              }
-              commit(smem_address(&C.scores[t]));
-              if (u + 2 == to[t]) commit(smem_address(&C.queries_free[t]));
-            }
-            __syncwarp();
+          return true;
+        };
+        auto score = [&](int t) {  // S of unit u + 1
+          if (u + 1 < from[t] || u + 1 >= to[t]) return true;
+          if (kApart) {
+            if (!barrier_wait_warp(smem_address(&C.scores_read[t]), read_phase[t], &C.gave_up)) return false;
+            read_phase[t] ^= 1u;
           }
-        }
-        if (issuer && fine) {
-          if (u >= first) commit(smem_address(&C.empty[v_slot]));
-          if (u + 1 < end) commit(smem_address(&C.empty[k_slot]));
-        }
-        __syncwarp();
+          if (u + 1 == from[t]) {
+            if (!barrier_wait_warp(smem_address(&C.queries[t]), query_phase[t], &C.gave_up)) return false;
+            query_phase[t] ^= 1u;
+          }
+          if (kApart || u + 1 == from[t]) after_sync();
+          if (issuer) {
+            const uint64_t q = operand(base + t * M::kTileBytes, 1);
+            const uint64_t k_tile = operand(k_at, 1);
+#pragma unroll
+            for (int k = 0; k < DIM / 16; ++k) {
+              const uint32_t part = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
+              product_shared(tmem + M::score_column(t), q + part, k_tile + part, kScores, k > 0);
+            }
+            commit(smem_address(&C.scores[t]));
+            if (u + 2 == to[t]) commit(smem_address(&C.queries_free[t]));
+          }
+          return true;
+        };
+        // Where scores and probabilities have places of their own the next scores come first, as soon as the last
+        // ones have been read; otherwise behind the product that reads the probabilities in their place.
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          fine = fine && (kApart ? score(t) && weigh(t) : weigh(t) && score(t));
+        if (issuer && fine) commit(smem_address(&C.empty[slot]));
       }
-      used += static_cast<uint32_t>(end - first);
       if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
     if (!fine) {
@@ -464,7 +478,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   {
     const uint32_t t = (warp - kSoftmaxWarp) >> 2, thread = threadIdx.x & 127u;
     const uint32_t lanes = (warp & 3u) << 21;  // this warp's rows of tensor memory: lane 32 x (warp & 3), bits 16 up
-    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
+    const uint32_t s_at = tmem + M::score_column(t) + lanes, p_at = tmem + M::probability_column(t) + lanes,
+                   o_at = tmem + M::output_column(t) + lanes;
     const float ninf = __int_as_float(0xff800000);
     uint32_t score_phase = 0, output_phase = 0;
     const uint32_t half = P.item_rows / 2;
@@ -527,6 +542,12 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             highest_32(rest + 32, part);
           }
           const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
+          if (kApart && u != from) {  // the last unit's probabilities have been used
+            fine = barrier_wait_warp(smem_address(&C.outputs[t]), output_phase, &C.gave_up);
+            if (!fine) break;
+            output_phase ^= 1u;
+            after_sync();
+          }
           if (u == from) {
             m = top;
           } else {
@@ -554,10 +575,16 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 #pragma unroll 1
           for (int i = 0; i < kKeys; i += 64) {
             load_columns(s_at + i + 32, other);
-            probabilities<T>(s, s_at + i / 2, scales, shifts, sum);
+            probabilities<T>(s, p_at + i / 2, scales, shifts, sum);
             loads_done(other);
-            if (i == 0) load_columns(s_at + 64, s);
-            probabilities<T>(other, s_at + i / 2 + 16, scales, shifts, sum);
+            if (i == 0) {
+              load_columns(s_at + 64, s);
+            } else if (kApart) {  // the next scores may come
+              before_sync();
+              __syncwarp();
+              if (lane == 0) barrier_arrive(smem_address(&C.scores_read[t]));
+            }
+            probabilities<T>(other, p_at + i / 2 + 16, scales, shifts, sum);
             loads_done(s);
           }
           const float2 sums = apart(add_two(sum[0], sum[1]));
@@ -640,9 +667,9 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   before_sync();
   __syncthreads();
   after_sync();
-  if (C.gave_up && (warp == kKeyWarp || warp == kValueWarp)) {
+  if (C.gave_up && warp == kKeyWarp) {
     for (uint32_t f = fills > kPairs ? fills - kPairs : 0u; f < fills; ++f)
-      barrier_wait_out(smem_address(&C.full[f % kPairs * 2u + (warp - kKeyWarp)]), (f / kPairs) & 1u);
+      barrier_wait_out(smem_address(&C.full[f % kPairs]), (f / kPairs) & 1u);
     if (lane == 0) atomicExch(P.status, 1u);
   }
   if (warp == kMmaWarp)
