@@ -243,22 +243,23 @@ int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_arg
   constexpr uint64_t kMostUnits = 1ull << 31;
   const uint64_t rows = std::min<uint64_t>(new_tokens * group, most_rows);
   p->padded_dim = c.head_dim <= 64 ? 64 : 128;
-  const uint32_t few_rows = kFewRows * static_cast<uint32_t>(std::min<uint64_t>((rows + kFewRows - 1) / kFewRows, kFewTilesMost));
+  const uint32_t few = few_keys(p->padded_dim);
   const uint32_t whole_tokens = group <= kTileRows ? kTileRows / group * group : 0;  // rows of a row tile of the other
-  p->many = rows > kFewTilesMost * kFewRows || items(few_rows) * (tiles(kFewKeys) + 2) >= kMostUnits;
-  if (whole_tokens == 0) p->many = false;
-  p->rows = p->many ? kManyRows : few_rows;
-  p->item_rows = p->many ? 2 * whole_tokens : few_rows;
-  p->keys = p->many ? kManyKeys : kFewKeys;
+  // More than 16 rows: the other kernel, which takes 57 to 61 us whatever the rows for 16 sequences of 3350 keys
+  // (8 key heads of 128), where this one takes 44 us for 16 rows, 66 for 32 and 94 for 48 (keys read again).
+  p->many = whole_tokens && (rows > kFewRows || items(kFewRows) * (tiles(few) + 2) >= kMostUnits);
+  p->rows = p->many ? kManyRows : kFewRows;
+  p->item_rows = p->many ? 2 * whole_tokens : kFewRows;
+  p->keys = p->many ? kManyKeys : few;
   p->least_units = (p->many ? kManyLeastKeys : kFewLeastKeys) / p->keys;
   p->box = std::gcd(c.page_size, p->keys);
-  p->item_cost = p->many ? 1 : p->padded_dim == 64 ? 2 : 1;
+  p->item_cost = 1;
   const uint64_t most_units = items(p->item_rows) * (tiles(p->keys) + p->item_cost);
   if (most_units >= kMostUnits)
     return fail(MONONN_ERR_TOO_LARGE, "attention: so many new tokens over so many keys count 2^31 units of work or more");
   const bool whole = capacity <= kWholeKeys;
   const uint64_t wanted = whole ? items(p->item_rows) : (most_units + p->least_units - 1) / p->least_units;
-  const uint64_t most = static_cast<uint64_t>(p->many || p->rows > kFewRows ? 1 : 2) * static_cast<unsigned>(sm_count);
+  const uint64_t most = static_cast<uint64_t>(p->many ? 1 : 2) * static_cast<unsigned>(sm_count);
   p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, most)));
   p->joins = !whole && p->ctas > 1;
   p->workspace = 0;

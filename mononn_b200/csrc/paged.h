@@ -36,9 +36,10 @@ struct RowsParams {
 cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int sm_count, cudaStream_t stream);
 
 // ------------------------------------------------------------------------ attention
-// The kernel for few rows takes items of 16, 32 or 48 rows, and 64 keys a unit; the one for many rows
-// two tiles of up to 128 rows (whole tokens), and 128 keys.
-constexpr uint32_t kFewRows = 16, kFewTilesMost = 3, kFewKeys = 64;
+// The kernel for few rows takes items of 16 rows, and as many keys a unit as fill 16 KB; the one for many rows two
+// tiles of up to 128 rows (whole tokens), and 128 keys.
+constexpr uint32_t kFewRows = 16;
+constexpr uint32_t few_keys(uint32_t padded_dim) { return 8192 / padded_dim; }
 constexpr uint32_t kTileRows = 128, kManyRows = 2 * kTileRows, kManyKeys = 128;
 
 struct AttentionHeader {  // one per CTA: the item that begins in it and goes on in the next `more` CTAs

@@ -9,38 +9,33 @@
 namespace mononn {
 namespace paged {
 
-constexpr int kKeyGroups = 4;  // warps that share a row tile
-constexpr int kPieces = 2;     // told ahead
+constexpr int kWarps = 4;   // that compute
+constexpr int kThreadsFew = (kWarps + 2) * 32;  // one more that loads keys, one that loads values
+constexpr int kPieces = 2;  // told ahead
+constexpr int kRows = static_cast<int>(kFewRows);
 
-template <int DIM, int TILES>
+template <int DIM>
 struct FewShape {
-  static constexpr int kRows = static_cast<int>(kFewRows) * TILES;
-  static constexpr int kWarps = kKeyGroups * TILES;  // that compute
-  static constexpr int kThreads = (kWarps + 2) * 32;  // one more that loads keys, one that loads values
-  static constexpr int kCtas = TILES == 1 ? 2 : 1;   // of an SM
-  static constexpr int kSlotBytes = static_cast<int>(kFewKeys) * DIM * 2;
-  // keys or values of one tile each
-  static constexpr int kSlots = (TILES == 1 ? 4 : TILES == 2 ? 8 : 6) * (128 / DIM);
+  static constexpr int kKeys = static_cast<int>(few_keys(DIM));  // of a unit; 16 KB of keys
+  static constexpr int kEach = kKeys / kWarps;                   // of a warp
+  static constexpr int kSlotBytes = kKeys * DIM * 2;
+  static constexpr int kSlots = 4;        // 0, 2: keys, 1, 3: values of a unit
   static constexpr int kPitch = DIM + 8;  // floats between rows of the warps' outputs: no bank conflicts
   static constexpr int kQueries = kSlots * kSlotBytes, kQueryBytes = kRows * DIM * 2;
   static constexpr int kOutputs = kQueries + kPieces * kQueryBytes;
-  static constexpr int kControl = kOutputs + kKeyGroups * kRows * kPitch * 4;
-  static constexpr int kSmem = 1024 + kControl + 2304;
+  static constexpr int kControl = kOutputs + kWarps * kRows * kPitch * 4;
+  static constexpr int kSmem = 1024 + kControl + 1280;
 };
-template <int DIM, int TILES>
 struct FewControl {
-  using S = FewShape<DIM, TILES>;
-  uint64_t full[S::kSlots], empty[S::kSlots], told[kPieces], taken[kPieces], meeting;
+  uint64_t full[4], empty[4], told[kPieces], taken[kPieces], meeting;
   alignas(16) Piece pieces[kPieces];
   Share share;
-  uint32_t sums[S::kWarps + 2];
+  uint32_t sums[kWarps + 2];
   uint32_t gave_up;
-  float maxima[kKeyGroups][S::kRows], totals[kKeyGroups][S::kRows];
+  float maxima[kWarps][kRows], totals[kWarps][kRows];
 };
-static_assert(sizeof(FewControl<64, 1>) <= 2304 && sizeof(FewControl<64, 2>) <= 2304 && sizeof(FewControl<64, 3>) <= 2304 &&
-                  sizeof(FewControl<128, 3>) <= 2304, "control block");
-static_assert(FewShape<128, 1>::kSmem <= 113 * 1024 && FewShape<128, 2>::kSmem <= 227 * 1024 &&
-                  FewShape<128, 3>::kSmem <= 227 * 1024 && FewShape<64, 1>::kSmem <= 113 * 1024, "shared memory");
+static_assert(sizeof(FewControl) <= 1280, "control block");
+static_assert(FewShape<128>::kSmem <= 113 * 1024 && FewShape<64>::kSmem <= 113 * 1024, "two CTAs share an SM");
 
 __device__ __forceinline__ void matrices_4(uint32_t address, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -82,16 +77,13 @@ __device__ __forceinline__ bool warps_meet(uint32_t bar, uint32_t& phase, volati
   return fine;
 }
 
-template <typename T, int DIM, int TILES>
-__global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, TILES>::kCtas)
-    few_rows_kernel(const __grid_constant__ AttentionParams P) {
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t raw[];
-  using S = FewShape<DIM, TILES>;
-  constexpr int kHalves = DIM / 64, kSteps = DIM / 16, kSlots = S::kSlots, kWarps = S::kWarps, kRows = S::kRows;
-  // 13 warps leave 128 registers a thread: queries are read again for every tile of keys then
-  constexpr bool kHoldQueries = TILES < 3 || DIM == 64;
+  using S = FewShape<DIM>;
+  constexpr int kHalves = DIM / 64, kSteps = DIM / 16, kSlots = S::kSlots, kKeys = S::kKeys, kEach = S::kEach;
   uint8_t* smem = raw + ((1024u - (smem_address(raw) & 1023u)) & 1023u);
-  auto& C = *reinterpret_cast<FewControl<DIM, TILES>*>(smem + S::kControl);
+  FewControl& C = *reinterpret_cast<FewControl*>(smem + S::kControl);
   const uint32_t slots = smem_address(smem);
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -112,14 +104,14 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
   }
   let_next_begin();
   earlier_done();
-  find_share<kFewKeys, S::kThreads>(P, C.sums, &C.share);  // barriers of the CTA within
+  find_share<kKeys, kThreadsFew>(P, C.sums, &C.share);  // barriers of the CTA within
   // Slots 0, 2, .. hold keys, 1, 3, .. values.
   constexpr uint32_t kPairs = kSlots / 2;
   uint32_t fills = 0;  // of this loading warp
 
   if (warp == kWarps) {
-    TileLoader<kFewKeys, kHalves> loader(P);
-    Walker<kFewKeys> walk(P, C.share);
+    TileLoader<kKeys, kHalves> loader(P);
+    Walker<kKeys> walk(P, C.share);
     bool fine = true;
     for (uint32_t i = 0; fine; ++i) {
       const bool some = walk.next();
@@ -155,7 +147,7 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
     }
     if (lane == 0 && P.headers) walk.write_header();
   } else if (warp == kWarps + 1) {
-    TileLoader<kFewKeys, kHalves> loader(P);
+    TileLoader<kKeys, kHalves> loader(P);
     bool fine = true;
     for (uint32_t i = 0; fine; ++i) {
       const uint32_t at = i % kPieces;
@@ -179,11 +171,10 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
     const float ninf = __int_as_float(0xff800000);
     uint32_t slot = 0, parity = 0, meetings = 0;
     float* const outputs = reinterpret_cast<float*>(smem + S::kOutputs);
-    const uint32_t group = warp % kKeyGroups, row_tile = warp / kKeyGroups;
     // ldmatrix addresses: lanes 0-7, 8-15, .. point at the rows of the four 8 x 8 matrices
-    const uint32_t key_row = group * 16 + (lane & 7u) + ((lane >> 4) << 3), key_chunk = (lane >> 3) & 1u;
-    const uint32_t val_row = group * 16 + (lane & 15u), val_chunk = lane >> 4;
-    const uint32_t query_row = row_tile * 16 + (lane & 15u), query_chunk = lane >> 4;
+    const uint32_t key_row = warp * kEach + (lane & 7u) + ((lane >> 4) << 3), key_chunk = (lane >> 3) & 1u;
+    const uint32_t val_row = warp * kEach + (lane & 15u), val_chunk = lane >> 4;
+    const uint32_t query_row = lane & 15u, query_chunk = lane >> 4;
     for (uint32_t n = 0;; ++n) {
       const uint32_t at = n % kPieces;
       if (!barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up)) break;
@@ -191,18 +182,14 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
       if (piece.valid == 0) break;
       const int32_t count = piece.count, tile0 = piece.tile, keys_begin = piece.keys_begin, keys_end = piece.keys_end;
       const uint32_t queries = slots + S::kQueries + at * S::kQueryBytes + query_row * 128;
-      auto query = [&](int k, uint32_t (&r)[4]) {
-        matrices_4(queries + (k >> 2) * (kRows * 128) + ((((k & 3) * 2 + query_chunk) ^ (query_row & 7u)) << 4), r);
-      };
-      uint32_t held[kHoldQueries ? kSteps : 1][4];
-      if constexpr (kHoldQueries) {
+      uint32_t q[kSteps][4];
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) query(k, held[k]);
-      }
+      for (int k = 0; k < kSteps; ++k)
+        matrices_4(queries + (k >> 2) * (kRows * 128) + ((((k & 3) * 2 + query_chunk) ^ (query_row & 7u)) << 4), q[k]);
       int32_t see_from[2], see_to[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t r = row_tile * 16 + (lane >> 2) + 8 * i;
+        const uint32_t r = (lane >> 2) + 8 * i;
         const bool valid = r < piece.rows;
         const int32_t position = piece.length - piece.n + static_cast<int32_t>((piece.first_row + r) / P.group);
         see_to[i] = valid ? (P.causal ? max(position + 1, 0) : piece.length) : 0x7fffffff;
@@ -213,7 +200,6 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
       // keys that every row sees need no test
       const int32_t all_from = __reduce_max_sync(0xffffffffu, max(see_from[0], see_from[1]));
       const int32_t all_to = __reduce_min_sync(0xffffffffu, min(see_to[0], see_to[1]));
-      const bool idle = row_tile * 16 >= piece.rows;
 
       float acc[kSteps * 2][4];
 #pragma unroll
@@ -223,38 +209,37 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
       float m[2] = {ninf, ninf}, l[2] = {0.f, 0.f};
 
       for (int32_t u = 0; u < count; ++u) {
-        const int32_t key0 = (tile0 + u) * static_cast<int32_t>(kFewKeys) + static_cast<int32_t>(group) * 16;
-        const bool any = !idle && key0 < keys_end && key0 + 16 > keys_begin;
-        const bool tested = key0 < all_from || key0 + 16 > all_to;
-        float s[2][4];
+        const int32_t key0 = (tile0 + u) * kKeys + static_cast<int32_t>(warp) * kEach;
+        const bool any = key0 < keys_end && key0 + kEach > keys_begin;
+        const bool tested = key0 < all_from || key0 + kEach > all_to;
+        float s[kEach / 8][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < kEach / 8; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
         if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
         if (any) {
           const uint32_t base = slots + slot * S::kSlotBytes + key_row * 128;
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            uint32_t b[4];
-            const uint32_t chunk = (k & 3) * 2 + key_chunk;
-            matrices_4(base + (k >> 2) * kFewKeys * 128 + ((chunk ^ (key_row & 7u)) << 4), b);
-            uint32_t fresh[4];
-            if constexpr (!kHoldQueries) query(k, fresh);
-            const uint32_t(&q)[4] = kHoldQueries ? held[kHoldQueries ? k : 0] : fresh;
-            multiply<T>(s[0], q, b[0], b[1]);
-            multiply<T>(s[1], q, b[2], b[3]);
-          }
+          for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int i = 0; i < kEach / 16; ++i) {
+              uint32_t b[4];
+              const uint32_t chunk = (k & 3) * 2 + key_chunk;
+              matrices_4(base + (k >> 2) * kKeys * 128 + i * 16 * 128 + ((chunk ^ (key_row & 7u)) << 4), b);
+              multiply<T>(s[2 * i], q[k], b[0], b[1]);
+              multiply<T>(s[2 * i + 1], q[k], b[2], b[3]);
+            }
         }
         __syncwarp();
         if (lane == 0) barrier_arrive(smem_address(&C.empty[slot]));
         if (++slot == kSlots) slot = 0, parity ^= 1u;
 
-        uint32_t p[4];
+        uint32_t p[kEach / 16][4];
         if (any) {
           if (tested) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kEach / 8; ++i)
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int32_t key = key0 + i * 8 + (lane & 3u) * 2 + (j & 1);
@@ -264,10 +249,11 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
           float top[2];
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            top[r] = fmaxf(fmaxf(s[0][r * 2], s[0][r * 2 + 1]), fmaxf(s[1][r * 2], s[1][r * 2 + 1]));
+            top[r] = m[r];
+#pragma unroll
+            for (int i = 0; i < kEach / 8; ++i) top[r] = fmaxf(top[r], fmaxf(s[i][r * 2], s[i][r * 2 + 1]));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            top[r] = fmaxf(top[r], m[r]);
           }
           if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
             float f[2];
@@ -288,40 +274,42 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
           // a row that has seen nothing yet: exp2(-inf - 0) = 0
           const float shift[2] = {m[0] == ninf ? 0.f : m[0] * P.scale_log2, m[1] == ninf ? 0.f : m[1] * P.scale_log2};
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < kEach / 8; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               s[i][j] = exp2_fast(fmaf(s[i][j], P.scale_log2, -shift[j >> 1]));
               l[j >> 1] += s[i][j];
             }
-          // the probabilities take the values' type for the product: one rounding of half a step each
-          p[0] = Pair<T>::pack(s[0][0], s[0][1]);
-          p[1] = Pair<T>::pack(s[0][2], s[0][3]);
-          p[2] = Pair<T>::pack(s[1][0], s[1][1]);
-          p[3] = Pair<T>::pack(s[1][2], s[1][3]);
+            // the probabilities take the values' type for the product: one rounding of half a step each
+            p[i / 2][(i & 1) * 2] = Pair<T>::pack(s[i][0], s[i][1]);
+            p[i / 2][(i & 1) * 2 + 1] = Pair<T>::pack(s[i][2], s[i][3]);
+          }
         }
         if (!barrier_wait_warp(smem_address(&C.full[slot]), parity, &C.gave_up)) break;
         if (any) {
           const uint32_t base = slots + slot * S::kSlotBytes + val_row * 128;
           // value rows that no row of the item sees may hold anything: 0 x NaN is not 0
-          const bool clear = key0 < keys_begin || key0 + 16 > keys_end;
-          uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-          if (clear) {
+          const bool clear = key0 < keys_begin || key0 + kEach > keys_end;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int32_t key = key0 + i * 8 + (lane & 3u) * 2;
-              const bool a = key >= keys_begin && key < keys_end;
-              const bool b = key + 1 >= keys_begin && key + 1 < keys_end;
-              keep[i] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
+          for (int i = 0; i < kEach / 16; ++i) {
+            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+            if (clear) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int32_t key = key0 + i * 16 + j * 8 + (lane & 3u) * 2;
+                const bool a = key >= keys_begin && key < keys_end;
+                const bool b = key + 1 >= keys_begin && key + 1 < keys_end;
+                keep[j] = (a ? 0xffffu : 0u) | (b ? 0xffff0000u : 0u);
+              }
             }
-          }
 #pragma unroll
-          for (int k = 0; k < kSteps; ++k) {
-            uint32_t b[4];
-            const uint32_t chunk = (k & 3) * 2 + val_chunk;
-            matrices_4_transposed(base + (k >> 2) * kFewKeys * 128 + ((chunk ^ (val_row & 7u)) << 4), b);
-            multiply<T>(acc[k * 2], p, b[0] & keep[0], b[1] & keep[1]);
-            multiply<T>(acc[k * 2 + 1], p, b[2] & keep[0], b[3] & keep[1]);
+            for (int k = 0; k < kSteps; ++k) {
+              uint32_t b[4];
+              const uint32_t chunk = (k & 3) * 2 + val_chunk;
+              matrices_4_transposed(base + (k >> 2) * kKeys * 128 + i * 16 * 128 + ((chunk ^ (val_row & 7u)) << 4), b);
+              multiply<T>(acc[k * 2], p[i], b[0] & keep[0], b[1] & keep[1]);
+              multiply<T>(acc[k * 2 + 1], p[i], b[2] & keep[0], b[3] & keep[1]);
+            }
           }
         }
         __syncwarp();
@@ -329,7 +317,7 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
         if (++slot == kSlots) slot = 0, parity ^= 1u;
       }
 
-      // the results of the warps that share a row tile
+      // the four warps' results
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -339,13 +327,13 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
       if (!warps_meet(smem_address(&C.meeting), meetings, &C.gave_up)) break;  // the last piece's have been read
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t row = row_tile * 16 + (lane >> 2) + 8 * r;
+        const uint32_t row = (lane >> 2) + 8 * r;
         if (row < rows) {
           if ((lane & 3u) == 0) {
-            C.maxima[group][row] = m[r];
-            C.totals[group][row] = l[r];
+            C.maxima[warp][row] = m[r];
+            C.totals[warp][row] = l[r];
           }
-          float* to = outputs + (group * kRows + row) * S::kPitch + (lane & 3u) * 2;
+          float* to = outputs + (warp * kRows + row) * S::kPitch + (lane & 3u) * 2;
 #pragma unroll
           for (int i = 0; i < kSteps * 2; ++i)
             *reinterpret_cast<float2*>(to + i * 8) = make_float2(acc[i][r * 2], acc[i][r * 2 + 1]);
@@ -360,10 +348,10 @@ __global__ void __launch_bounds__(FewShape<DIM, TILES>::kThreads, FewShape<DIM, 
         const uint32_t row = i / (DIM / 8), d = (i % (DIM / 8)) * 8;
         float top = C.maxima[0][row];
 #pragma unroll
-        for (int w = 1; w < kKeyGroups; ++w) top = fmaxf(top, C.maxima[w][row]);
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, C.maxima[w][row]);
         float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kKeyGroups; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
           const float mw = C.maxima[w][row];
           const float f = mw == ninf ? 0.f : exp2_fast((mw - top) * P.scale_log2);
           sum += f * C.totals[w][row];
@@ -497,47 +485,36 @@ static __device__ uint32_t g_status;
 cudaError_t paged_status_word(uint32_t** out) { return cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_status); }
 
 namespace {
-// f(kernel, its shape) for the type, the padded head size and the row tiles of a call
-template <typename T, int DIM, typename F>
-cudaError_t with_tiles(uint32_t tiles, F&& f) {
-  if (tiles == 1) return f(paged::few_rows_kernel<T, DIM, 1>, paged::FewShape<DIM, 1>());
-  if (tiles == 2) return f(paged::few_rows_kernel<T, DIM, 2>, paged::FewShape<DIM, 2>());
-  return f(paged::few_rows_kernel<T, DIM, 3>, paged::FewShape<DIM, 3>());
+template <typename T, int DIM>
+cudaError_t prepare() {
+  return cudaFuncSetAttribute(paged::few_rows_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              paged::FewShape<DIM>::kSmem);
 }
-template <typename F>
-cudaError_t with_kernel(bool bf16, uint32_t dim, uint32_t tiles, F&& f) {
-  if (bf16) return dim == 64 ? with_tiles<__nv_bfloat16, 64>(tiles, f) : with_tiles<__nv_bfloat16, 128>(tiles, f);
-  return dim == 64 ? with_tiles<__half, 64>(tiles, f) : with_tiles<__half, 128>(tiles, f);
+template <typename T, int DIM>
+cudaError_t launch(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
+  return launch_dependent(paged::few_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsFew, paged::FewShape<DIM>::kSmem, p,
+                          stream);
 }
 template <typename T, int DIM>
 cudaError_t join(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
-  auto go = [&](auto kernel, uint32_t rows, uint32_t parts) {
-    return launch_dependent(kernel, dim3(plan.ctas, rows * parts / paged::kJoinWarps), paged::kJoinWarps * 32, 0, p, stream);
-  };
-  switch (plan.rows) {
-    case 16: return go(paged::join_kernel<T, DIM, 16, 8>, 16, 8);
-    case 32: return go(paged::join_kernel<T, DIM, 32, 4>, 32, 4);
-    case 48: return go(paged::join_kernel<T, DIM, 48, 4>, 48, 4);
-    default: return go(paged::join_kernel<T, DIM, static_cast<int>(kManyRows), 1>, kManyRows, 1);
-  }
+  if (plan.many)
+    return launch_dependent(paged::join_kernel<T, DIM, static_cast<int>(kManyRows), 1>,
+                            dim3(plan.ctas, kManyRows / paged::kJoinWarps), paged::kJoinWarps * 32, 0, p, stream);
+  return launch_dependent(paged::join_kernel<T, DIM, static_cast<int>(kFewRows), paged::kJoinWarps>,
+                          dim3(plan.ctas, kFewRows), paged::kJoinWarps * 32, 0, p, stream);
 }
 }  // namespace
 
 cudaError_t prepare_few_rows() {
-  for (int bf16 = 0; bf16 < 2; ++bf16)
-    for (uint32_t dim : {64u, 128u})
-      for (uint32_t tiles = 1; tiles <= kFewTilesMost; ++tiles) {
-        const cudaError_t e = with_kernel(bf16 != 0, dim, tiles, [](auto kernel, auto shape) {
-          return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decltype(shape)::kSmem);
-        });
-        if (e != cudaSuccess) return e;
-      }
+  for (cudaError_t e : {prepare<__half, 64>(), prepare<__half, 128>(), prepare<__nv_bfloat16, 64>(),
+                        prepare<__nv_bfloat16, 128>()})
+    if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
 cudaError_t launch_few_rows(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
-  return with_kernel(bf16, plan.padded_dim, plan.rows / kFewRows, [&](auto kernel, auto shape) {
-    return launch_dependent(kernel, dim3(plan.ctas), decltype(shape)::kThreads, decltype(shape)::kSmem, p, stream);
-  });
+  if (bf16)
+    return plan.padded_dim == 64 ? launch<__nv_bfloat16, 64>(p, plan, stream) : launch<__nv_bfloat16, 128>(p, plan, stream);
+  return plan.padded_dim == 64 ? launch<__half, 64>(p, plan, stream) : launch<__half, 128>(p, plan, stream);
 }
 cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, bool bf16, cudaStream_t stream) {
   if (bf16) return plan.padded_dim == 64 ? join<__nv_bfloat16, 64>(p, plan, stream) : join<__nv_bfloat16, 128>(p, plan, stream);
