@@ -179,6 +179,7 @@ __device__ __forceinline__ uint32_t head_units_warp(const AttentionParams& P, co
 struct Share {
   uint32_t units, begin, ctas, each, longer;
   uint32_t sequence, head, row_tile, skip;  // the item that holds the first unit, and its units before that
+  Sequence s;
   __device__ __forceinline__ uint32_t cta_of(uint32_t unit) const {
     const uint32_t in_longer = (each + 1u) * longer;
     return unit < in_longer ? unit / (each + 1u) : longer + (unit - in_longer) / each;
@@ -239,6 +240,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
       const int from = __ffs(here) - 1;
       at = __shfl_sync(0xffffffffu, at, from);
       uint32_t b = __shfl_sync(0xffffffffu, b0, from);
+      s.token = __shfl_sync(0xffffffffu, s.token, from);
       s.n = __shfl_sync(0xffffffffu, s.n, from);
       s.length = __shfl_sync(0xffffffffu, s.length, from);
       uint32_t per_head = 0;
@@ -272,7 +274,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
         left -= __shfl_sync(0xffffffffu, sum, 31);
       }
       if (lane == 0)
-        *share = Share{share_each + (blockIdx.x < longer ? 1u : 0u), u0, ctas, share_each, longer, b, head, tile, left};
+        *share = Share{share_each + (blockIdx.x < longer ? 1u : 0u), u0, ctas, share_each, longer, b, head, tile, left, s};
     }
   }
   __syncthreads();
@@ -299,12 +301,9 @@ struct Walker {
   uint32_t b, head, tile, skip, left, tiles, at, whole, goes_on;  // goes_on: tiles of the item behind the piece
   Piece piece;
   __device__ __forceinline__ Walker(const AttentionParams& params, const Share& sh)
-      : P(params), share(sh), s{0, 0, 0}, b(sh.sequence), head(sh.head), tile(sh.row_tile), skip(sh.skip),
+      : P(params), share(sh), s(sh.s), b(sh.sequence), head(sh.head), tile(sh.row_tile), skip(sh.skip),
         left(sh.units), tiles(0), at(sh.begin), whole(0), goes_on(0), piece{} {
-    if (left) {
-      s = load_sequence(P, b);
-      tiles = row_tiles(P, s);
-    }
+    if (left) tiles = row_tiles(P, s);
   }
   __device__ __forceinline__ bool next() {
     uint32_t units = 0, done = 0;
@@ -406,7 +405,6 @@ struct TileLoader {
     keys_end = min(piece.keys_end, (piece.tile + piece.count) * KEYS);
     first = static_cast<uint32_t>(piece.tile);
     look_up(first, page, row);
-    look_up(first + window, next_page, next_row);
   }
   // Loads a tile, the next one of the piece, into `dst` (HALVES blocks of KEYS rows of 128 bytes, swizzled).
   // Boxes without a visible key are left out: what the slot holds there is from earlier.
@@ -415,7 +413,6 @@ struct TileLoader {
       first = tile;
       page = next_page;
       row = next_row;
-      look_up(first + window, next_page, next_row);
     }
     const uint32_t from = (tile - first) * boxes + (lane & (boxes - 1u));
     const int32_t p = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, row, from);
@@ -428,6 +425,7 @@ struct TileLoader {
       for (int h = 0; h < HALVES; ++h)
         load_box(dst + h * KEYS * 128 + lane * P.box * 128u, map, h * 64, r, static_cast<int32_t>(head), p, bar);
     }
+    if (tile == first) look_up(first + window, next_page, next_row);
   }
 };
 

@@ -27,7 +27,7 @@ struct FewShape {
   static constexpr int kSmem = 1024 + kControl + 1280;
 };
 struct FewControl {
-  uint64_t full[4], empty[4], told[kPieces], taken[kPieces], meeting;
+  uint64_t full[4], empty[4], told[kPieces], queries[kPieces], taken[kPieces], meeting;
   alignas(16) Piece pieces[kPieces];
   Share share;
   uint32_t sums[kWarps + 2];
@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
       barrier_init(smem_address(&C.empty[i]), kWarps);
     }
     for (int i = 0; i < kPieces; ++i) {
-      barrier_init(smem_address(&C.told[i]), 33);
+      barrier_init(smem_address(&C.told[i]), 1);
+      barrier_init(smem_address(&C.queries[i]), 32);
       barrier_init(smem_address(&C.taken[i]), kWarps + 1);
     }
     barrier_init(smem_address(&C.meeting), kWarps);
@@ -116,26 +117,12 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
     for (uint32_t i = 0; fine; ++i) {
       const bool some = walk.next();
       if (some) loader.begin(walk.piece);
-      const uint32_t at = i % kPieces, told = smem_address(&C.told[at]);
+      const uint32_t at = i % kPieces;
       fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
       if (!fine) break;
       put_piece(&C.pieces[at], walk.piece, lane);
-      if (some) {  // the queries of the piece, consecutive lanes along a row
-        constexpr uint32_t kParts = DIM / 8;
-        const uint32_t tile = slots + S::kQueries + at * S::kQueryBytes;
-#pragma unroll 4
-        for (uint32_t j = lane; j < kRows * kParts; j += 32) {
-          const uint32_t row = j / kParts, part = j % kParts, g = walk.piece.first_row + row, token = g / P.group;
-          const bool wanted = row < walk.piece.rows && part * 8 < P.head_dim;
-          const T* src = static_cast<const T*>(P.q);
-          if (wanted)
-            src += (walk.piece.token + static_cast<int64_t>(token)) * P.q_token +
-                   static_cast<int64_t>(walk.piece.head * P.group + g - token * P.group) * P.q_head + part * 8;
-          copy_16(tile + (part >> 3) * (kRows * 128) + row * 128 + (((part & 7u) ^ (row & 7u)) << 4), src, wanted);
-        }
-      }
-      arrive_after_copies(told);
-      if (lane == 0) barrier_arrive(told);
+      if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
+      __syncwarp();
       if (!some) break;
       for (int32_t u = 0; u < walk.piece.count; ++u) {
         const uint32_t slot = fills % kPairs * 2u;
@@ -143,6 +130,21 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
         if (!fine) break;
         loader.load(&P.k_map, walk.piece.tile + u, slots + slot * S::kSlotBytes, walk.piece.head, smem_address(&C.full[slot]));
         ++fills;
+        if (u == 0) {  // the queries, behind the first keys: consecutive lanes along a row
+          constexpr uint32_t kParts = DIM / 8;
+          const uint32_t tile = slots + S::kQueries + at * S::kQueryBytes;
+#pragma unroll 4
+          for (uint32_t j = lane; j < kRows * kParts; j += 32) {
+            const uint32_t row = j / kParts, part = j % kParts, g = walk.piece.first_row + row, token = g / P.group;
+            const bool wanted = row < walk.piece.rows && part * 8 < P.head_dim;
+            const T* src = static_cast<const T*>(P.q);
+            if (wanted)
+              src += (walk.piece.token + static_cast<int64_t>(token)) * P.q_token +
+                     static_cast<int64_t>(walk.piece.head * P.group + g - token * P.group) * P.q_head + part * 8;
+            copy_16(tile + (part >> 3) * (kRows * 128) + row * 128 + (((part & 7u) ^ (row & 7u)) << 4), src, wanted);
+          }
+          arrive_after_copies(smem_address(&C.queries[at]));
+        }
       }
     }
     if (lane == 0 && P.headers) walk.write_header();
@@ -181,6 +183,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
       const Piece& piece = C.pieces[at];
       if (piece.valid == 0) break;
       const int32_t count = piece.count, tile0 = piece.tile, keys_begin = piece.keys_begin, keys_end = piece.keys_end;
+      if (!barrier_wait_warp(smem_address(&C.queries[at]), (n / kPieces) & 1u, &C.gave_up)) break;
       const uint32_t queries = slots + S::kQueries + at * S::kQueryBytes + query_row * 128;
       uint32_t q[kSteps][4];
 #pragma unroll
