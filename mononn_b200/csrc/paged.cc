@@ -230,8 +230,8 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
 
 // Which kernel, how many CTAs, and whether an item may span them. Only sizes count that the host knows.
 constexpr uint32_t kWholeKeys = 512;      // caches of at most so many keys: no item is split
-constexpr uint32_t kFewLeastKeys = 256;   // of a CTA's share
-constexpr uint32_t kManyLeastKeys = 512;
+constexpr uint32_t kFewLeastKeys = 512;   // of a CTA's share
+constexpr uint32_t kManyLeastKeys = 1024;
 int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
   const uint32_t group = a.q_heads / c.kv_heads;
   const uint64_t capacity = static_cast<uint64_t>(c.max_pages) * c.page_size;
@@ -253,7 +253,7 @@ int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_arg
   p->keys = p->many ? kManyKeys : few;
   p->least_units = (p->many ? kManyLeastKeys : kFewLeastKeys) / p->keys;
   p->box = std::gcd(c.page_size, p->keys);
-  p->item_cost = 1;
+  p->item_cost = p->many ? 2 : 1;
   const uint64_t most_units = items(p->item_rows) * (tiles(p->keys) + p->item_cost);
   if (most_units >= kMostUnits)
     return fail(MONONN_ERR_TOO_LARGE, "attention: so many new tokens over so many keys count 2^31 units of work or more");

@@ -311,171 +311,170 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   bool fine = true;
   // Each group of warps within its own branch: code behind a meeting of both is held to the fewer registers.
   if (warp < kSoftmaxWarp) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-  if (warp == kKeyWarp) {
-    TileLoader<kKeys, kHalves> loader(P);
-    Walker<kKeys> walk(P, C.share);
-    const uint32_t half = P.item_rows / 2, half_tokens = half / P.group;
-    uint32_t query_loads[2] = {0, 0};
-    for (uint32_t i = 0; fine; ++i) {
-      const bool some = walk.next();
-      if (some) {
-        loader.begin(walk.piece);
-        set_ranges(P, walk.piece);
-      }
-      const uint32_t at = i % kPieces;
-      fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
-      if (!fine) break;
-      put_piece(&C.pieces[at], walk.piece, lane);
-      if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
-      __syncwarp();
-      if (!some) break;
-      for (int32_t u = 0; u <= walk.piece.count; ++u) {
-        const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
-        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
-        if (!fine) break;
-        ++fills;
-        if (u == walk.piece.count) {  // the last values come alone
-          if (lane == 0) barrier_arrive(full);
-          __syncwarp();
-          break;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (warp == kKeyWarp) {
+      TileLoader<kKeys, kHalves> loader(P);
+      Walker<kKeys> walk(P, C.share);
+      const uint32_t half = P.item_rows / 2, half_tokens = half / P.group;
+      uint32_t query_loads[2] = {0, 0};
+      for (uint32_t i = 0; fine; ++i) {
+        const bool some = walk.next();
+        if (some) {
+          loader.begin(walk.piece);
+          set_ranges(P, walk.piece);
         }
-        loader.load(&P.k_map, walk.piece.tile + u, ring + slot * 2u * M::kTileBytes, walk.piece.head, full);
-        if (u == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
+        const uint32_t at = i % kPieces;
+        fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
+        if (!fine) break;
+        put_piece(&C.pieces[at], walk.piece, lane);
+        if (lane == 0) barrier_arrive(smem_address(&C.told[at]));
+        __syncwarp();
+        if (!some) break;
+        for (int32_t u = 0; u <= walk.piece.count; ++u) {
+          const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
+          fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+          if (!fine) break;
+          ++fills;
+          if (u == walk.piece.count) {  // the last values come alone
+            if (lane == 0) barrier_arrive(full);
+            __syncwarp();
+            break;
+          }
+          loader.load(&P.k_map, walk.piece.tile + u, ring + slot * 2u * M::kTileBytes, walk.piece.head, full);
+          if (u == 0) {  // the queries, behind the first keys: whole tokens, some of the next sequence perhaps
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (walk.piece.to[t] <= walk.piece.from[t]) continue;
-            fine = fine && barrier_wait_warp(smem_address(&C.queries_free[t]), (query_loads[t] & 1u) ^ 1u, &C.gave_up);
-            if (!fine) break;
-            ++query_loads[t];
-            if (lane == 0) {
-              const uint32_t bar = smem_address(&C.queries[t]);
-              barrier_arrive_bytes(bar, half * 128u * kHalves);
-              const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
+            for (int t = 0; t < 2; ++t) {
+              if (walk.piece.to[t] <= walk.piece.from[t]) continue;
+              fine = fine && barrier_wait_warp(smem_address(&C.queries_free[t]), (query_loads[t] & 1u) ^ 1u, &C.gave_up);
+              if (!fine) break;
+              ++query_loads[t];
+              if (lane == 0) {
+                const uint32_t bar = smem_address(&C.queries[t]);
+                barrier_arrive_bytes(bar, half * 128u * kHalves);
+                const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
 #pragma unroll
-              for (int h = 0; h < kHalves; ++h)
-                load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
-                             static_cast<int32_t>(walk.piece.head * P.group), token, bar);
+                for (int h = 0; h < kHalves; ++h)
+                  load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
+                               static_cast<int32_t>(walk.piece.head * P.group), token, bar);
+              }
+              __syncwarp();
             }
+            if (!fine) break;
+          }
+        }
+      }
+      if (lane == 0 && P.headers) walk.write_header();
+    } else if (warp == kValueWarp) {
+      TileLoader<kKeys, kHalves> loader(P);
+      for (uint32_t i = 0; fine; ++i) {
+        const uint32_t at = i % kPieces;
+        fine = barrier_wait_warp(smem_address(&C.told[at]), (i / kPieces) & 1u, &C.gave_up);
+        const Piece& piece = C.pieces[at];
+        if (!fine || piece.valid == 0) break;
+        const int32_t tile = piece.tile, count = piece.count;
+        const uint32_t head = piece.head;
+        loader.begin(piece);
+        __syncwarp();
+        if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
+        for (int32_t u = -1; u < count; ++u) {
+          const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
+          fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
+          if (!fine) break;
+          ++fills;
+          if (u < 0) {  // the first keys come alone
+            if (lane == 0) barrier_arrive(full);
+            __syncwarp();
+          } else {
+            loader.load(&P.v_map, tile + u, ring + (slot * 2u + 1u) * M::kTileBytes, head, full);
+          }
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      uint32_t step = 0;  // slots of the ring taken so far
+      uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0}, read_phase[2] = {1, 1};
+      const bool issuer = elected();
+      constexpr uint32_t kScores = instruction<T>(kKeys, false), kOutput = instruction<T>(DIM, true);
+      for (uint32_t n = 0; fine; ++n) {
+        const uint32_t at = n % kPieces;
+        fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
+        const Piece& piece = C.pieces[at];
+        if (!fine || piece.valid == 0) break;
+        const int32_t first = piece.tile, end = first + piece.count;
+        const int32_t from[2] = {piece.from[0], piece.from[1]}, to[2] = {piece.to[0], piece.to[1]};
+        const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
+        // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
+        for (int32_t u = first - 1; fine && u < end; ++u) {
+          const uint32_t slot = step % kPairs;
+          const uint32_t k_at = ring + slot * 2u * M::kTileBytes, v_at = k_at + M::kTileBytes;
+          fine = barrier_wait_warp(smem_address(&C.full[slot]), (step / kPairs) & 1u, &C.gave_up);
+          if (!fine) break;
+          ++step;
+          // value rows that no row sees may hold anything: 0 x NaN is not 0
+          const int32_t key0 = u * kKeys;
+          if (u >= first && (key0 < keys_begin || key0 + kKeys > keys_end)) {
+            uint8_t* const tile = smem + (v_at - base);
+            for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
+              const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
+              if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            shared_to_async();
             __syncwarp();
           }
-          if (!fine) break;
-        }
-      }
-    }
-    if (lane == 0 && P.headers) walk.write_header();
-  } else if (warp == kValueWarp) {
-    TileLoader<kKeys, kHalves> loader(P);
-    for (uint32_t i = 0; fine; ++i) {
-      const uint32_t at = i % kPieces;
-      fine = barrier_wait_warp(smem_address(&C.told[at]), (i / kPieces) & 1u, &C.gave_up);
-      const Piece& piece = C.pieces[at];
-      if (!fine || piece.valid == 0) break;
-      const int32_t tile = piece.tile, count = piece.count;
-      const uint32_t head = piece.head;
-      loader.begin(piece);
-      __syncwarp();
-      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
-      for (int32_t u = -1; u < count; ++u) {
-        const uint32_t slot = fills % kPairs, full = smem_address(&C.full[slot]);
-        fine = barrier_wait_warp(smem_address(&C.empty[slot]), ((fills / kPairs) & 1u) ^ 1u, &C.gave_up);
-        if (!fine) break;
-        ++fills;
-        if (u < 0) {  // the first keys come alone
-          if (lane == 0) barrier_arrive(full);
-          __syncwarp();
-        } else {
-          loader.load(&P.v_map, tile + u, ring + (slot * 2u + 1u) * M::kTileBytes, head, full);
-        }
-      }
-    }
-  } else if (warp == kMmaWarp) {
-    uint32_t step = 0;  // slots of the ring taken so far
-    uint32_t query_phase[2] = {0, 0}, probability_phase[2] = {0, 0}, read_phase[2] = {1, 1};
-    const bool issuer = elected();
-    constexpr uint32_t kScores = instruction<T>(kKeys, false), kOutput = instruction<T>(DIM, true);
-    for (uint32_t n = 0; fine; ++n) {
-      const uint32_t at = n % kPieces;
-      fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
-      const Piece& piece = C.pieces[at];
-      if (!fine || piece.valid == 0) break;
-      const int32_t first = piece.tile, end = first + piece.count;
-      const int32_t from[2] = {piece.from[0], piece.from[1]}, to[2] = {piece.to[0], piece.to[1]};
-      const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
-      // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
-      for (int32_t u = first - 1; fine && u < end; ++u) {
-        const uint32_t slot = step % kPairs;
-        const uint32_t k_at = ring + slot * 2u * M::kTileBytes, v_at = k_at + M::kTileBytes;
-        fine = barrier_wait_warp(smem_address(&C.full[slot]), (step / kPairs) & 1u, &C.gave_up);
-        if (!fine) break;
-        ++step;
-        // value rows that no row sees may hold anything: 0 x NaN is not 0
-        const int32_t key0 = u * kKeys;
-        if (u >= first && (key0 < keys_begin || key0 + kKeys > keys_end)) {
-          uint8_t* const tile = smem + (v_at - base);
-          for (uint32_t i = lane; i < kKeys * DIM / 8; i += 32) {
-            const int32_t r = static_cast<int32_t>((i >> 3) % kKeys);  // a row has 128 bytes of each 64 elements
-            if (key0 + r < keys_begin || key0 + r >= keys_end) *reinterpret_cast<uint4*>(tile + i * 16) = make_uint4(0, 0, 0, 0);
-          }
-          shared_to_async();
-          __syncwarp();
-        }
-        auto weigh = [&](int t) {  // O += P V of unit u; false after a wait that gave up
-          if (u < from[t] || u >= to[t]) return true;
-          if (!barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up)) return false;
-          probability_phase[t] ^= 1u;
-          after_sync();
-          if (issuer) {
-            const uint64_t v = operand(v_at, kKeys * 128 / 16);
+          auto weigh = [&](int t) {  // O += P V of unit u; false after a wait that gave up
+            if (u < from[t] || u >= to[t]) return true;
+            if (!barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up)) return false;
+            probability_phase[t] ^= 1u;
+            after_sync();
+            if (issuer) {
+              const uint64_t v = operand(v_at, kKeys * 128 / 16);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              product_tensor(tmem + M::output_column(t), tmem + M::probability_column(t) + k * 8, v + k * (16 * 128 / 16),
-                             kOutput, k > 0 || u > from[t]);
-            if (kApart || u + 1 == to[t]) commit(smem_address(&C.outputs[t]));
-          }
-          return true;
-        };
-        auto score = [&](int t) {  // S of unit u + 1
-          if (u + 1 < from[t] || u + 1 >= to[t]) return true;
-          if (kApart) {
-            if (!barrier_wait_warp(smem_address(&C.scores_read[t]), read_phase[t], &C.gave_up)) return false;
-            read_phase[t] ^= 1u;
-          }
-          if (u + 1 == from[t]) {
-            if (!barrier_wait_warp(smem_address(&C.queries[t]), query_phase[t], &C.gave_up)) return false;
-            query_phase[t] ^= 1u;
-          }
-          if (kApart || u + 1 == from[t]) after_sync();
-          if (issuer) {
-            const uint64_t q = operand(base + t * M::kTileBytes, 1);
-            const uint64_t k_tile = operand(k_at, 1);
-#pragma unroll
-            for (int k = 0; k < DIM / 16; ++k) {
-              const uint32_t part = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
-              product_shared(tmem + M::score_column(t), q + part, k_tile + part, kScores, k > 0);
+              for (int k = 0; k < kKeys / 16; ++k)
+                product_tensor(tmem + M::output_column(t), tmem + M::probability_column(t) + k * 8, v + k * (16 * 128 / 16),
+                               kOutput, k > 0 || u > from[t]);
+              if (kApart || u + 1 == to[t]) commit(smem_address(&C.outputs[t]));
             }
-            commit(smem_address(&C.scores[t]));
-            if (u + 2 == to[t]) commit(smem_address(&C.queries_free[t]));
-          }
-          return true;
-        };
-        // Where scores and probabilities have places of their own the next scores come first, as soon as the last
-        // ones have been read; otherwise behind the product that reads the probabilities in their place.
+            return true;
+          };
+          auto score = [&](int t) {  // S of unit u + 1
+            if (u + 1 < from[t] || u + 1 >= to[t]) return true;
+            if (kApart) {
+              if (!barrier_wait_warp(smem_address(&C.scores_read[t]), read_phase[t], &C.gave_up)) return false;
+              read_phase[t] ^= 1u;
+            }
+            if (u + 1 == from[t]) {
+              if (!barrier_wait_warp(smem_address(&C.queries[t]), query_phase[t], &C.gave_up)) return false;
+              query_phase[t] ^= 1u;
+            }
+            if (kApart || u + 1 == from[t]) after_sync();
+            if (issuer) {
+              const uint64_t q = operand(base + t * M::kTileBytes, 1);
+              const uint64_t k_tile = operand(k_at, 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          fine = fine && (kApart ? score(t) && weigh(t) : weigh(t) && score(t));
-        if (issuer && fine) commit(smem_address(&C.empty[slot]));
+              for (int k = 0; k < DIM / 16; ++k) {
+                const uint32_t part = (k >> 2) * (static_cast<int>(kTileRows) * 128 / 16) + (k & 3) * 2;
+                product_shared(tmem + M::score_column(t), q + part, k_tile + part, kScores, k > 0);
+              }
+              commit(smem_address(&C.scores[t]));
+              if (u + 2 == to[t]) commit(smem_address(&C.queries_free[t]));
+            }
+            return true;
+          };
+          // Where scores and probabilities have places of their own the next scores come first, as soon as the last
+          // ones have been read; otherwise behind the product that reads the probabilities in their place.
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            fine = fine && (kApart ? score(t) && weigh(t) : weigh(t) && score(t));
+          if (issuer && fine) commit(smem_address(&C.empty[slot]));
+        }
+        if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
       }
-      if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
+      if (!fine) {
+        if (issuer) commit(smem_address(&C.drained));
+        barrier_wait_out(smem_address(&C.drained), 0);
+      }
     }
-    if (!fine) {
-      if (issuer) commit(smem_address(&C.drained));
-      barrier_wait_out(smem_address(&C.drained), 0);
-    }
-  }
   } else {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-  {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const uint32_t t = (warp - kSoftmaxWarp) >> 2, thread = threadIdx.x & 127u;
     const uint32_t lanes = (warp & 3u) << 21;  // this warp's rows of tensor memory: lane 32 x (warp & 3), bits 16 up
     const uint32_t s_at = tmem + M::score_column(t) + lanes, p_at = tmem + M::probability_column(t) + lanes,
@@ -662,7 +661,6 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       }
       if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
-  }
   }
   before_sync();
   __syncthreads();
