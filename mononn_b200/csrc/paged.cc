@@ -397,6 +397,7 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
   p.max_pages = c.max_pages;
   p.num_pages = c.num_pages;
   p.page_size = c.page_size;
+  p.by_page_size = make_divisor(c.page_size);
   if (rotary) set_rotation(&p, *rotary);
   return launched(launch_rows(p, c.dtype == MONONN_BF16, rows_by_vectors(p), dev->sm_count,
                               static_cast<cudaStream_t>(cuda_stream)));
@@ -464,6 +465,9 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.item_cost = plan.item_cost;
   p.causal = a.causal != 0;
   p.window = a.window;
+  p.by_group = make_divisor(p.group);
+  p.by_item_rows = make_divisor(p.item_rows);
+  p.by_page_size = make_divisor(c.page_size);
   p.whole_items = !plan.joins;
   p.min_units = plan.joins ? plan.least_units : 1;
   p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));

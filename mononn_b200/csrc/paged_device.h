@@ -122,6 +122,11 @@ __device__ __forceinline__ void arrive_after_copies(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+__device__ __forceinline__ uint32_t divide(uint32_t n, const Divisor& d) {
+  const uint32_t t = __umulhi(n, d.multiplier);
+  return (t + ((n - t) >> d.shift1)) >> d.shift2;
+}
+
 // ------------------------------------------------------------------ division of the work
 struct Sequence {
   int32_t token, n, length;  // first new token, new tokens, keys
@@ -140,22 +145,27 @@ __device__ __forceinline__ KeyRange key_range(const AttentionParams& P, const Se
   if (P.causal) {
     const int32_t base = s.length - s.n;
     r.end = max(0, base + static_cast<int32_t>(last) + 1);
-    if (P.window) {
-      const int64_t b = static_cast<int64_t>(base) + first + 1 - static_cast<int64_t>(P.window);
-      r.begin = static_cast<int32_t>(max(static_cast<int64_t>(0), b));
-    }
+    // keys behind position p + 1 - window, where p is the first token's (below zero: it sees nothing)
+    const int32_t upto = base + static_cast<int32_t>(first) + 1;
+    if (P.window && upto > 0 && static_cast<uint32_t>(upto) > P.window) r.begin = upto - static_cast<int32_t>(P.window);
   }
   return r;
 }
 __device__ __forceinline__ uint32_t row_tiles(const AttentionParams& P, const Sequence& s) {
-  return (static_cast<uint32_t>(s.n) * P.group + P.item_rows - 1) / P.item_rows;
+  return divide(static_cast<uint32_t>(s.n) * P.group + P.item_rows - 1u, P.by_item_rows);
 }
 __device__ __forceinline__ KeyRange item_keys(const AttentionParams& P, const Sequence& s, uint32_t tile) {
   const uint32_t first = tile * P.item_rows;
   const uint32_t last = min(first + P.item_rows, static_cast<uint32_t>(s.n) * P.group) - 1u;
-  return key_range(P, s, first / P.group, last / P.group);
+  return key_range(P, s, divide(first, P.by_group), divide(last, P.by_group));
 }
 // Tiles of an item; one that sees no key has one all the same, in which its zeros are written.
+// Keys from .. to - 1 are those that the token at `position` sees (`length`: keys of its sequence).
+__device__ __forceinline__ void seen_keys(const AttentionParams& P, int32_t position, int32_t length, int32_t& from, int32_t& to) {
+  to = P.causal ? max(position + 1, 0) : length;
+  from = P.causal && P.window && position >= 0 && static_cast<uint32_t>(position) >= P.window
+             ? position + 1 - static_cast<int32_t>(P.window) : 0;
+}
 template <int KEYS>
 __device__ __forceinline__ uint32_t item_tiles(const KeyRange& r) {
   return r.end > r.begin ? (r.end + KEYS - 1) / KEYS - r.begin / KEYS : 1u;
@@ -393,7 +403,7 @@ struct TileLoader {
     page_of = -1;
     row_of = -1;
     if (key < keys_end && key + static_cast<int32_t>(P.box) > keys_begin) {
-      const uint32_t p = static_cast<uint32_t>(key) / P.page_size;
+      const uint32_t p = divide(static_cast<uint32_t>(key), P.by_page_size);
       row_of = key - static_cast<int32_t>(p * P.page_size);
       page_of = P.table[static_cast<int64_t>(sequence) * P.table_stride + p];
     }

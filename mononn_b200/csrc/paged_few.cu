@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
           const uint32_t tile = slots + S::kQueries + at * S::kQueryBytes;
 #pragma unroll 4
           for (uint32_t j = lane; j < kRows * kParts; j += 32) {
-            const uint32_t row = j / kParts, part = j % kParts, g = walk.piece.first_row + row, token = g / P.group;
+            const uint32_t row = j / kParts, part = j % kParts, g = walk.piece.first_row + row, token = divide(g, P.by_group);
             const bool wanted = row < walk.piece.rows && part * 8 < P.head_dim;
             const T* src = static_cast<const T*>(P.q);
             if (wanted)
@@ -194,11 +194,10 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
       for (int i = 0; i < 2; ++i) {
         const uint32_t r = (lane >> 2) + 8 * i;
         const bool valid = r < piece.rows;
-        const int32_t position = piece.length - piece.n + static_cast<int32_t>((piece.first_row + r) / P.group);
-        see_to[i] = valid ? (P.causal ? max(position + 1, 0) : piece.length) : 0x7fffffff;
+        const int32_t position = piece.length - piece.n + static_cast<int32_t>(divide(piece.first_row + r, P.by_group));
         see_from[i] = 0;
-        if (valid && P.causal && P.window)
-          see_from[i] = static_cast<int32_t>(max(static_cast<int64_t>(0), position + 1 - static_cast<int64_t>(P.window)));
+        see_to[i] = 0x7fffffff;
+        if (valid) seen_keys(P, position, piece.length, see_from[i], see_to[i]);
       }
       // keys that every row sees need no test
       const int32_t all_from = __reduce_max_sync(0xffffffffu, max(see_from[0], see_from[1]));
@@ -365,8 +364,9 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
         }
         if (complete) {
           const uint32_t g = piece.first_row + row;
-          const int64_t token = piece.token + static_cast<int64_t>(g / P.group);
-          const uint32_t head = piece.head * P.group + g % P.group;
+          const uint32_t of = divide(g, P.by_group);
+          const int64_t token = piece.token + static_cast<int64_t>(of);
+          const uint32_t head = piece.head * P.group + (g - of * P.group);
           const float inverse = sum == 0.f ? 0.f : 1.f / sum;
           if (d < P.head_dim) {
             uint4 v;
@@ -478,8 +478,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     }
     if (part != 0 || !valid) continue;
     const uint32_t g = h.first_row + row;
-    const int64_t token = static_cast<int64_t>(h.token) + g / P.group;
-    const uint32_t head = h.head * P.group + g % P.group;
+    const uint32_t of = divide(g, P.by_group);
+    const int64_t token = static_cast<int64_t>(h.token) + of;
+    const uint32_t head = h.head * P.group + (g - of * P.group);
     const float inverse = total == 0.f ? 0.f : 1.f / total;
     const uint32_t d = lane * kEach;
     if (d < P.head_dim) {

@@ -254,7 +254,7 @@ __device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
     p.from[t] = p.to[t] = 0;
     if (t * half >= p.rows) continue;
     const uint32_t first = p.first_row + t * half, last = p.first_row + min((t + 1) * half, p.rows) - 1u;
-    const KeyRange k = key_range(P, Sequence{p.token, p.n, p.length}, first / P.group, last / P.group);
+    const KeyRange k = key_range(P, Sequence{p.token, p.n, p.length}, divide(first, P.by_group), divide(last, P.by_group));
     if (k.end <= k.begin) continue;
     p.from[t] = max(p.tile, k.begin / kKeys);
     p.to[t] = max(p.from[t], min(p.tile + p.count, (k.end + kKeys - 1) / kKeys));
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     if (warp == kKeyWarp) {
       TileLoader<kKeys, kHalves> loader(P);
       Walker<kKeys> walk(P, C.share);
-      const uint32_t half = P.item_rows / 2, half_tokens = half / P.group;
+      const uint32_t half = P.item_rows / 2, half_tokens = divide(half, P.by_group);
       uint32_t query_loads[2] = {0, 0};
       for (uint32_t i = 0; fine; ++i) {
         const bool some = walk.next();
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               if (lane == 0) {
                 const uint32_t bar = smem_address(&C.queries[t]);
                 barrier_arrive_bytes(bar, half * 128u * kHalves);
-                const int32_t token = walk.piece.token + static_cast<int32_t>(walk.piece.first_row / P.group + t * half_tokens);
+                const int32_t token = walk.piece.token + static_cast<int32_t>(divide(walk.piece.first_row, P.by_group) + t * half_tokens);
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
                   load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
@@ -494,13 +494,9 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       const int32_t from = piece.from[t], to = piece.to[t];
       float m = ninf, l = 0.f;
       if (to > from) {
-        const int32_t position = piece.length - piece.n + static_cast<int32_t>(g / P.group);
         int32_t see_from = 0, see_to = 0x7fffffff;
-        if (valid) {
-          see_to = P.causal ? max(position + 1, 0) : piece.length;
-          if (P.causal && P.window)
-            see_from = static_cast<int32_t>(max(static_cast<int64_t>(0), position + 1 - static_cast<int64_t>(P.window)));
-        }
+        if (valid)
+          seen_keys(P, piece.length - piece.n + static_cast<int32_t>(divide(g, P.by_group)), piece.length, see_from, see_to);
         const int32_t all_from = __reduce_max_sync(0xffffffffu, see_from);
         const int32_t all_to = __reduce_min_sync(0xffffffffu, see_to);
 
@@ -601,7 +597,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       }
       if (t * half < piece.rows) {
         const bool any = to > from, complete = piece.begins && piece.ends;
-        const uint32_t token = g / P.group, head = piece.head * P.group + (g - token * P.group);
+        const uint32_t token = divide(g, P.by_group), head = piece.head * P.group + (g - token * P.group);
         const int64_t row_of = piece.token + static_cast<int64_t>(token);
         const float inverse = !complete ? 1.f : l == 0.f ? 0.f : 1.f / l;
         uint64_t row_at;  // where this thread's row goes

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_cons
         const int64_t at = static_cast<int64_t>(length) - (static_cast<int64_t>(end) - begin) + (static_cast<int64_t>(token) - begin);
         position = static_cast<int32_t>(at);
         if (member && at >= 0 && at < static_cast<int64_t>(P.max_pages) * P.page_size) {
-          const uint32_t n = static_cast<uint32_t>(at) / P.page_size;
+          const uint32_t n = divide(static_cast<uint32_t>(at), P.by_page_size);
           const int32_t page = P.table[static_cast<int64_t>(b) * P.table_stride + n];
           if (page >= 0 && static_cast<uint32_t>(page) < P.num_pages)
             page_at = page * P.page_stride + static_cast<int64_t>(static_cast<uint32_t>(at) - n * P.page_size) * P.k.dst_token;
