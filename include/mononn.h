@@ -296,8 +296,8 @@ int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* a
 /* A cache of keys and values in pages of page_size tokens. Element (token row r, head h, d) of page p is at
  * p * page_stride + r * token_stride + h * head_stride + d in k_pages and v_pages alike, so pages may be
  * token-major or head-major. Sequence b's keys 0 .. lengths[b]-1 are in the pages page_table[b *
- * table_stride + key / page_size]; a length beyond max_pages * page_size counts as that. Sequences may
- * share pages. A page number outside of 0 .. num_pages-1 is never followed: its tokens are not
+ * table_stride + key / page_size]. Attention counts a length beyond max_pages * page_size as that; the append
+ * writes no token at a position beyond it. Sequences may share pages. A page number outside of 0 .. num_pages-1 is never followed: its tokens are not
  * written, and read as zeros. New tokens are packed: sequence b has the rows indptr[b] .. indptr[b+1]-1 of
  * the token tensors (indptr: [sequences + 1], not decreasing), and they are its LAST positions:
  * row indptr[b] + i is at position lengths[b] - (indptr[b+1] - indptr[b]) + i, so `lengths` counts them.
@@ -318,7 +318,8 @@ typedef struct {
  * (q NULL: none; q_out may be q itself). positions: what is rotated by instead of the position in
  * the cache, or NULL. A token without a place (a negative position, a page number out of range) is not
  * written; its query is rotated all the same. Two tokens that fall on one place of a
- * shared page leave one of the two there. Alignment as mononn_rotary_apply. */
+ * shared page leave one of the two there. k, v and q are not themselves in the pages. Alignment as
+ * mononn_rotary_apply. */
 typedef struct {
   const void *k, *v;
   int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
@@ -336,12 +337,17 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
  * where head h reads key head h / (q_heads / kv_heads). A token at position p sees the keys j <= p
  * (causal; otherwise all of its sequence), and with window > 0 (causal only) of those the ones with
  * j > p - window. A row that sees nothing becomes zeros (lse: minus infinity). lse: natural
- * logarithm of the sum of the exponentials, f32 [tokens, q_heads], or NULL. Keys that no row sees and
- * page rows behind a length may hold anything, NaN too.
+ * logarithm of the sum of the exponentials, f32 [tokens, q_heads], or NULL. Keys that no row
+ * of a sequence sees and page rows behind a length may hold anything, NaN too; an infinity or NaN among the values
+ * that some of a sequence's new tokens see may reach those of its new tokens that do not (its weight there is zero).
  * max_new: at most how many new tokens a sequence has, as a hint that chooses between the kernel for
  * few rows (single tokens, drafts) and the one for many; 0 = unknown. Results are right whatever it says.
- * Limits: head_dim a multiple of 8 up to 128; page_size a multiple of 8; q_heads / kv_heads whole;
- * addresses of pages, q and out, and all their strides, multiples of 16 bytes (lse, indptr: 4). */
+ * The same arguments and contents give the same bits again. No gradients.
+ * Limits: head_dim a multiple of 8 up to 128; page_size a multiple of 8; q_heads / kv_heads whole (up to 128 have
+ * a kernel for many rows; above, every 16 rows read the keys again); addresses of pages, q and out, and all their
+ * strides, multiples of 16 bytes (lse, indptr: 4); new tokens x keys such that the tiles of both, with max_pages *
+ * page_size keys for every sequence, count below 2^31. The first call of these operators on a device loads their
+ * kernels: make it before a stream is captured. */
 typedef struct {
   const void* q;
   void* out;

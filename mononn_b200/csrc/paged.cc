@@ -2,11 +2,15 @@
 // tensor maps, the division into kernels and workspaces. No device memory is read or allocated here.
 #include "paged.h"
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdio>
+#include <initializer_list>
 #include <mutex>
 #include <numeric>
 #include <string>
+#include <utility>
 
 #include "../../include/mononn.h"
 #include "runtime.h"
@@ -15,17 +19,20 @@ using namespace mononn;
 
 namespace {
 
-int fail(int code, const std::string& msg) {
-  set_last_error(msg);
+// Nothing is thrown across the C entry points: a message that finds no memory is left out.
+int fail(int code, const char* msg, const char* more = "") {
+  try {
+    set_last_error(std::string(msg) + more);
+  } catch (...) {
+  }
   return code;
 }
-int invalid(const std::string& msg) { return fail(MONONN_ERR_INVALID_ARGUMENT, msg); }
+int invalid(const char* msg) { return fail(MONONN_ERR_INVALID_ARGUMENT, msg); }
 
-#define PG_TRY(expr)                                                                     \
-  do {                                                                                   \
-    cudaError_t e__ = (expr);                                                            \
-    if (e__ != cudaSuccess)                                                              \
-      return fail(MONONN_ERR_CUDA, std::string(#expr) + ": " + cudaGetErrorString(e__)); \
+#define PG_TRY(expr)                                                                         \
+  do {                                                                                       \
+    cudaError_t e__ = (expr);                                                                \
+    if (e__ != cudaSuccess) return fail(MONONN_ERR_CUDA, #expr ": ", cudaGetErrorString(e__)); \
   } while (0)
 
 // A launch on a stream of another device than the kernel's ends in this error (the stream itself cannot be
@@ -35,7 +42,7 @@ int launched(cudaError_t e) {
   cudaGetLastError();
   if (e == cudaErrorInvalidResourceHandle)
     return invalid("the stream belongs to another device than the buffers, or to none");
-  return fail(MONONN_ERR_CUDA, std::string("kernel launch: ") + cudaGetErrorString(e));
+  return fail(MONONN_ERR_CUDA, "kernel launch: ", cudaGetErrorString(e));
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -62,6 +69,8 @@ int set_up(int dev, const Device** out) {
     if (major != 10) return fail(MONONN_ERR_NO_DEVICE, "the kernels are built for sm_100a only");
     PG_TRY(cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev));
     PG_TRY(paged_status_word(&d.status));
+    // every kernel is loaded here, none during a capture later
+    PG_TRY(prepare_rows());
     PG_TRY(prepare_few_rows());
     PG_TRY(prepare_many_rows());
     if (!g_encode) {
@@ -114,6 +123,23 @@ bool whole8(int64_t stride) { return (stride & 7) == 0; }
 // Strides that no tensor of this size can have are refused, so that the kernels' 64-bit offsets never wrap.
 bool stride_in_range(int64_t s) { return s >= 0 && s < (1ll << 39); }
 
+// Whether no two elements share a place (what is written would depend on an order): by growing stride, each
+// dimension has to reach over all that the smaller ones span.
+using Dimension = std::pair<uint32_t, int64_t>;  // size, stride
+bool apart(uint32_t head_dim, std::initializer_list<Dimension> dims) {
+  Dimension sorted[3];
+  size_t n = 0;
+  for (const Dimension& d : dims)
+    if (d.first > 1) sorted[n++] = d;
+  std::sort(sorted, sorted + n, [](const Dimension& a, const Dimension& b) { return a.second < b.second; });
+  unsigned __int128 span = head_dim;
+  for (size_t i = 0; i < n; ++i) {
+    if (static_cast<uint64_t>(sorted[i].second) < span) return false;
+    span += static_cast<unsigned __int128>(sorted[i].first - 1) * static_cast<uint64_t>(sorted[i].second);
+  }
+  return true;
+}
+
 int check_dtype(int dtype) {
   if (dtype != MONONN_F16 && dtype != MONONN_BF16)
     return fail(MONONN_ERR_UNSUPPORTED, "dtype must be MONONN_F16 or MONONN_BF16");
@@ -141,7 +167,6 @@ int check_cache(const mononn_paged_cache& c) {
     return invalid("cache: strides must be in 0 .. 2^39, table_stride at least max_pages");
   if (!aligned(c.page_table, 4) || !aligned(c.lengths, 4) || !aligned(c.k_pages, 2) || !aligned(c.v_pages, 2))
     return invalid("cache: misaligned pointer");
-  // no two elements in one place: what is written would depend on an order
   const int64_t d = c.head_dim;
   if ((c.page_size > 1 && c.token_stride < d) || (c.kv_heads > 1 && c.head_stride < d) ||
       (c.num_pages > 1 && c.page_stride < d))
@@ -165,6 +190,12 @@ void set_rotation(RowsParams* p, const mononn_rotary& r) {
   for (unsigned i = 0; i < r.rotary_dim / 2; ++i) p->turns[i] = r.turns[i];
 }
 
+int encoded(CUresult r, const char* what) {
+  if (r == CUDA_SUCCESS) return MONONN_OK;
+  char detail[64];
+  std::snprintf(detail, sizeof(detail), ": cuTensorMapEncodeTiled failed (CUresult %d)", static_cast<int>(r));
+  return fail(MONONN_ERR_CUDA, what, detail);
+}
 // Elements are 16 bits wide. One box is 64 elements of a head x `box` rows of one page; elements behind
 // head_dim, rows and pages out of range arrive as zeros.
 int encode_pages(CUtensorMap* map, const mononn_paged_cache& c, const void* base, uint32_t box, const char* what) {
@@ -178,10 +209,7 @@ int encode_pages(CUtensorMap* map, const mononn_paged_cache& c, const void* base
                               4, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(MONONN_ERR_CUDA, std::string(what) + ": cuTensorMapEncodeTiled failed (CUresult " +
-                                     std::to_string(static_cast<int>(r)) + ")");
-  return MONONN_OK;
+  return encoded(r, what);
 }
 
 // One box is 64 elements of the heads of a group x the tokens of a row tile.
@@ -195,13 +223,10 @@ int encode_queries(CUtensorMap* map, const mononn_paged_cache& c, const mononn_p
                               3, const_cast<void*>(a.q), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(MONONN_ERR_CUDA, "q: cuTensorMapEncodeTiled failed (CUresult " + std::to_string(static_cast<int>(r)) + ")");
-  return MONONN_OK;
+  return encoded(r, "q");
 }
 
 int check_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* a) {
-  if (!cache || !a) return invalid("null argument");
   if (int rc = check_cache(*cache)) return rc;
   const mononn_paged_cache& c = *cache;
   if (c.head_dim % 8 || c.head_dim > 128)
@@ -215,15 +240,16 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
       !stride_in_range(a->out_token_stride) || !stride_in_range(a->out_head_stride))
     return invalid("attention: strides must be in 0 .. 2^39");
   const int64_t d = c.head_dim;
-  if ((a->q_heads > 1 && (a->out_head_stride < d || a->q_head_stride < d)) ||
-      (a->tokens > 1 && (a->out_token_stride < d || a->q_token_stride < d)))
-    return invalid("attention: strides of q or out are smaller than the heads they hold");
+  if ((a->q_heads > 1 && a->q_head_stride < d) || (a->tokens > 1 && a->q_token_stride < d))
+    return invalid("attention: strides of q are smaller than the heads they hold");
+  if (!apart(c.head_dim, {{a->tokens, a->out_token_stride}, {a->q_heads, a->out_head_stride}}))
+    return invalid("attention: strides put elements of out into one place");
   if (!aligned(c.k_pages, 16) || !aligned(c.v_pages, 16) || !whole8(c.page_stride) || !whole8(c.token_stride) ||
       !whole8(c.head_stride) || !aligned(a->q, 16) || !whole8(a->q_token_stride) || !whole8(a->q_head_stride) ||
       !aligned(a->out, 16) || !whole8(a->out_token_stride) || !whole8(a->out_head_stride))
     return invalid("attention: addresses and strides of pages, q and out must be multiples of 16 bytes");
   if (!aligned(a->lse, 4) || !aligned(a->indptr, 4)) return invalid("attention: lse and indptr must be 4-byte aligned");
-  if (!std::isfinite(a->scale) || a->scale < 0.f) return invalid("attention: scale must be positive and finite, or 0");
+  if (!std::isfinite(a->scale * 2.f) || a->scale < 0.f) return invalid("attention: scale must be positive and finite, or 0");
   if (a->window && !a->causal) return invalid("attention: a window needs causal attention");
   return MONONN_OK;
 }
@@ -321,6 +347,7 @@ int mononn_rotary_init(const mononn_rotary_config* config, mononn_rotary* out) {
 int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* args, void* cuda_stream) {
   if (!rotary || !args) return invalid("null argument");
   const mononn_rotary_args& a = *args;
+  if (a.tokens == 0 || a.heads == 0) return MONONN_OK;
   if (int rc = check_dtype(a.dtype)) return rc;
   if (a.head_dim == 0 || a.head_dim > 256 || a.heads > 65536)
     return fail(MONONN_ERR_TOO_LARGE, "rotary: head_dim in 1 .. 256, heads <= 65536");
@@ -329,12 +356,10 @@ int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* a
       !stride_in_range(a.out_token_stride) || !stride_in_range(a.out_head_stride))
     return invalid("rotary: strides must be in 0 .. 2^39");
   if (a.tokens > INT_MAX) return fail(MONONN_ERR_TOO_LARGE, "rotary: tokens < 2^31");
-  if (a.tokens == 0 || a.heads == 0) return MONONN_OK;
   if (!a.x || !a.out || !a.positions) return invalid("rotary: null pointer");
   if (!aligned(a.x, 2) || !aligned(a.out, 2) || !aligned(a.positions, 4)) return invalid("rotary: misaligned pointer");
-  const int64_t d = a.head_dim;
-  if ((a.heads > 1 && a.out_head_stride < d) || (a.tokens > 1 && a.out_token_stride < d))
-    return invalid("rotary: strides of out are smaller than the heads they hold");
+  if (!apart(a.head_dim, {{a.tokens, a.out_token_stride}, {a.heads, a.out_head_stride}}))
+    return invalid("rotary: strides put elements of out into one place");
   if (a.x == a.out && (a.x_token_stride != a.out_token_stride || a.x_head_stride != a.out_head_stride))
     return invalid("rotary: in place, x and out have the same strides");
   OnDeviceOf guard;
@@ -353,6 +378,7 @@ int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* a
 int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* rotary,
                         const mononn_paged_append_args* args, void* cuda_stream) {
   if (!cache || !args) return invalid("null argument");
+  if (args->tokens == 0 || cache->sequences == 0) return MONONN_OK;
   if (int rc = check_cache(*cache)) return rc;
   const mononn_paged_cache& c = *cache;
   const mononn_paged_append_args& a = *args;
@@ -370,13 +396,14 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
   if (!aligned(a.k, 2) || !aligned(a.v, 2) || !aligned(a.q, 2) || !aligned(a.q_out, 2) || !aligned(a.indptr, 4) ||
       !aligned(a.positions, 4))
     return invalid("append: misaligned pointer");
-  const int64_t d = c.head_dim;
-  if (a.q && ((a.q_heads > 1 && a.q_out_head_stride < d) || (a.tokens > 1 && a.q_out_token_stride < d)))
-    return invalid("append: strides of q_out are smaller than the heads they hold");
+  if (c.k_pages == c.v_pages) return invalid("append: keys and values go to the same pages");
+  if (!apart(c.head_dim, {{c.page_size, c.token_stride}, {c.kv_heads, c.head_stride}, {c.num_pages, c.page_stride}}))
+    return invalid("append: strides put elements of pages into one place");
+  if (a.q && !apart(c.head_dim, {{a.tokens, a.q_out_token_stride}, {a.q_heads, a.q_out_head_stride}}))
+    return invalid("append: strides put elements of q_out into one place");
   if (a.q && a.q == a.q_out &&
       (a.q_token_stride != a.q_out_token_stride || a.q_head_stride != a.q_out_head_stride))
     return invalid("append: in place, q and q_out have the same strides");
-  if (a.tokens == 0 || c.sequences == 0) return MONONN_OK;
   OnDeviceOf guard;
   const Device* dev = nullptr;
   if (int rc = guard.enter(c.k_pages, &dev)) return rc;
@@ -405,10 +432,10 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
 
 int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
                                      size_t* bytes) {
-  if (!bytes) return invalid("null argument");
+  if (!bytes || !cache || !args) return invalid("null argument");
   *bytes = 0;
-  if (int rc = check_attention(cache, args)) return rc;
   if (args->tokens == 0 || cache->sequences == 0) return MONONN_OK;
+  if (int rc = check_attention(cache, args)) return rc;
   OnDeviceOf guard;
   const Device* dev = nullptr;
   if (int rc = guard.enter(cache->k_pages, &dev)) return rc;
@@ -420,17 +447,21 @@ int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mono
 
 int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
                            void* cuda_stream) {
+  if (!cache || !args) return invalid("null argument");
+  if (args->tokens == 0 || cache->sequences == 0) return MONONN_OK;
   if (int rc = check_attention(cache, args)) return rc;
   const mononn_paged_cache& c = *cache;
   const mononn_paged_attention_args& a = *args;
-  if (a.tokens == 0 || c.sequences == 0) return MONONN_OK;
   OnDeviceOf guard;
   const Device* dev = nullptr;
   if (int rc = guard.enter(c.k_pages, &dev)) return rc;
   AttentionPlan plan;
   if (int rc = plan_attention(c, a, dev->sm_count, &plan)) return rc;
-  if (plan.workspace && (!a.workspace || a.workspace_bytes < plan.workspace || !aligned(a.workspace, 16)))
-    return invalid("attention: needs a workspace of " + std::to_string(plan.workspace) + " bytes, 16-byte aligned");
+  if (plan.workspace && (!a.workspace || a.workspace_bytes < plan.workspace || !aligned(a.workspace, 16))) {
+    char detail[64];
+    std::snprintf(detail, sizeof(detail), "%zu bytes, 16-byte aligned", plan.workspace);
+    return fail(MONONN_ERR_INVALID_ARGUMENT, "attention: needs a workspace of ", detail);
+  }
   AttentionParams p{};
   if (int rc = encode_pages(&p.k_map, c, c.k_pages, plan.box, "k_pages")) return rc;
   if (int rc = encode_pages(&p.v_map, c, c.v_pages, plan.box, "v_pages")) return rc;

@@ -46,6 +46,7 @@ struct RowsParams {
   float magnitude;
   double turns[128];
 };
+cudaError_t prepare_rows();
 cudaError_t launch_rows(const RowsParams& p, bool bf16, bool vectors, int sm_count, cudaStream_t stream);
 
 // ------------------------------------------------------------------------ attention

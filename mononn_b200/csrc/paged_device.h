@@ -159,13 +159,13 @@ __device__ __forceinline__ KeyRange item_keys(const AttentionParams& P, const Se
   const uint32_t last = min(first + P.item_rows, static_cast<uint32_t>(s.n) * P.group) - 1u;
   return key_range(P, s, divide(first, P.by_group), divide(last, P.by_group));
 }
-// Tiles of an item; one that sees no key has one all the same, in which its zeros are written.
 // Keys from .. to - 1 are those that the token at `position` sees (`length`: keys of its sequence).
 __device__ __forceinline__ void seen_keys(const AttentionParams& P, int32_t position, int32_t length, int32_t& from, int32_t& to) {
   to = P.causal ? max(position + 1, 0) : length;
   from = P.causal && P.window && position >= 0 && static_cast<uint32_t>(position) >= P.window
              ? position + 1 - static_cast<int32_t>(P.window) : 0;
 }
+// Tiles of an item; one that sees no key has one all the same, in which its zeros are written.
 template <int KEYS>
 __device__ __forceinline__ uint32_t item_tiles(const KeyRange& r) {
   return r.end > r.begin ? (r.end + KEYS - 1) / KEYS - r.begin / KEYS : 1u;
@@ -254,19 +254,21 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
       s.n = __shfl_sync(0xffffffffu, s.n, from);
       s.length = __shfl_sync(0xffffffffu, s.length, from);
       uint32_t per_head = 0;
+      bool found = false;  // always, where indptr does not decrease; otherwise sums may have wrapped
 #pragma unroll 1
-      for (;;) {
+      for (; b < end; ++b) {
         if (each > 1u) s = load_sequence(P, b);
         per_head = head_units_warp<KEYS>(P, s, row_tiles(P, s));
-        if (u0 - at < per_head * P.kv_heads) break;
+        found = u0 - at < per_head * P.kv_heads;
+        if (found) break;
         at += per_head * P.kv_heads;
-        ++b;
       }
       const uint32_t head = (u0 - at) / per_head;
       uint32_t left = u0 - at - head * per_head, tile = 0;
-      const uint32_t tiles = row_tiles(P, s);
+      const uint32_t tiles = found ? row_tiles(P, s) : 0u;
+      found = false;
 #pragma unroll 1
-      for (uint32_t t0 = 0;; t0 += 32u) {
+      for (uint32_t t0 = 0; t0 < tiles; t0 += 32u) {
         const uint32_t u = t0 + lane < tiles ? item_units<KEYS>(P, s, t0 + lane) : 0u;
         uint32_t sum = u;
 #pragma unroll
@@ -275,7 +277,8 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
           if (lane >= d) sum += o;
         }
         const uint32_t past = __ballot_sync(0xffffffffu, left < sum);
-        if (past) {
+        found = past != 0u;
+        if (found) {
           const int at_lane = __ffs(past) - 1;
           tile = t0 + at_lane;
           left -= __shfl_sync(0xffffffffu, sum - u, at_lane);
@@ -283,7 +286,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
         }
         left -= __shfl_sync(0xffffffffu, sum, 31);
       }
-      if (lane == 0)
+      if (lane == 0 && found)
         *share = Share{share_each + (blockIdx.x < longer ? 1u : 0u), u0, ctas, share_each, longer, b, head, tile, left, s};
     }
   }
@@ -326,7 +329,12 @@ struct Walker {
         if (++head == P.kv_heads) {
           head = 0;
           do {
-            s = load_sequence(P, ++b);
+            if (++b == P.sequences) {  // not where indptr does not decrease
+              left = 0;
+              piece.valid = 0;
+              return false;
+            }
+            s = load_sequence(P, b);
           } while (s.n == 0);
           tiles = row_tiles(P, s);
         }
@@ -370,7 +378,7 @@ struct Walker {
     AttentionHeader h{0, 0, 0, 0, 0, {0, 0, 0}};
     if (share.units != 0 && piece.begins && !piece.ends) {
       const uint32_t last = at + goes_on - 1u;  // the item's last unit
-      h = AttentionHeader{share.cta_of(last) - blockIdx.x, piece.rows, piece.first_row, piece.head,
+      h = AttentionHeader{min(share.cta_of(last), gridDim.x - 1u) - blockIdx.x, piece.rows, piece.first_row, piece.head,
                           static_cast<uint32_t>(piece.token), {0, 0, 0}};
     }
     P.headers[blockIdx.x] = h;

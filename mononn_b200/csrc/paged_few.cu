@@ -502,6 +502,10 @@ cudaError_t paged_status_word(uint32_t** out) { return cudaGetSymbolAddress(rein
 namespace {
 template <typename T, int DIM>
 cudaError_t prepare() {
+  cudaFuncAttributes a;
+  for (cudaError_t e : {cudaFuncGetAttributes(&a, paged::join_kernel<T, DIM, static_cast<int>(kFewRows), paged::kJoinWarps>),
+                        cudaFuncGetAttributes(&a, paged::join_kernel<T, DIM, static_cast<int>(kManyRows), 1>)})
+    if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(paged::few_rows_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               paged::FewShape<DIM>::kSmem);
 }

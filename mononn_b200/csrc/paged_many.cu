@@ -364,6 +364,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         }
       }
       if (lane == 0 && P.headers) walk.write_header();
+      for (int t = 0; t < 2; ++t)  // where all goes well they landed long ago
+        if (query_loads[t]) barrier_wait_out(smem_address(&C.queries[t]), (query_loads[t] - 1u) & 1u);
     } else if (warp == kValueWarp) {
       TileLoader<kKeys, kHalves> loader(P);
       for (uint32_t i = 0; fine; ++i) {

@@ -209,6 +209,14 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_cons
 
 }  // namespace paged
 
+cudaError_t prepare_rows() {
+  cudaFuncAttributes a;
+  for (cudaError_t e : {cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 1>), cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 8>),
+                        cudaFuncGetAttributes(&a, paged::rows_kernel<__nv_bfloat16, 1>),
+                        cudaFuncGetAttributes(&a, paged::rows_kernel<__nv_bfloat16, 8>)})
+    if (e != cudaSuccess) return e;
+  return cudaSuccess;
+}
 cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int sm_count, cudaStream_t stream) {
   RowsParams p = params;
   p.block_tokens = p.tokens >= 4u * static_cast<unsigned>(sm_count) ? paged::kRowsTokens : 1u;

@@ -56,6 +56,7 @@ def _dtype(t) -> int:
 
 def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
     """A [tokens, heads, head_dim] tensor of the dtype, device and head_dim of `like`."""
+    import torch
     if t.dim() != 3 or t.shape[2] != like.shape[-1]:
         raise ValueError(f"{name} must be [tokens, heads, {like.shape[-1]}], not {list(t.shape)}")
     if heads is not None and t.shape[1] != heads:
@@ -64,6 +65,8 @@ def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
         raise ValueError(f"{name} must have {tokens} tokens, not {t.shape[0]}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} on {like.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which is not computed here: detach it or use torch.no_grad()")
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name}: elements of a head must be consecutive")
     return t
@@ -108,8 +111,7 @@ def _out_rows(name: str, out, src):
     """`out` is `src` itself, or does not touch it."""
     if out.data_ptr() == src.data_ptr() and out.stride() == src.stride():
         return out
-    if out.untyped_storage().data_ptr() == src.untyped_storage().data_ptr() and _overlap(out, src) \
-            and not _same_grid(out, src):
+    if _overlap(out, src) and not _same_grid(out, src):
         raise ValueError(f"{name} overlaps its source: pass the source itself, or other memory")
     return out
 
@@ -195,6 +197,9 @@ class PagedCache:
             _rows("q", q, self.k_pages, None, k.shape[0])
             _rows("q_out", q_out, self.k_pages, q.shape[1], k.shape[0])
             _out_rows("q_out", q_out, q)
+            for name, t in (("k", k), ("v", v)):
+                if _overlap(q_out, t) and not _same_grid(q_out, t):
+                    raise ValueError(f"q_out overlaps {name}")
         qs, os = (q.stride(), q_out.stride()) if q is not None else ((0, 0), (0, 0))
         a = capi.PagedAppendArgs(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                  q.data_ptr() if q is not None else None,
@@ -221,8 +226,15 @@ class PagedCache:
         import torch
         _rows("q", q, self.k_pages, None)
         self._indptr(indptr)
+        def made_here(*size, dtype):  # on the stream of the call: in use there, and seen by the one of the caller
+            with torch.cuda.stream(stream):
+                t = torch.empty(*size, dtype=dtype, device=q.device)
+            if stream is not None and t.is_cuda:
+                t.record_stream(torch.cuda.current_stream(q.device))
+            return t
+
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = made_here(q.shape, dtype=q.dtype)
         _rows("out", out, self.k_pages, q.shape[1], q.shape[0])
         if lse is not None:
             if lse.dtype != torch.float32 or lse.device != q.device or tuple(lse.shape) != tuple(q.shape[:2]) \
@@ -233,8 +245,7 @@ class PagedCache:
         if not 0 <= window < 2**32 or not 0 <= max_new < 2**32:
             raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
         for name, t in (("q", q), ("lse", lse), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):
-            if t is not None and _overlap(out, t) and out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() \
-                    and not (name == "q" and _same_grid(out, q)):
+            if t is not None and _overlap(out, t) and not (name == "q" and _same_grid(out, q)):
                 raise ValueError(f"out overlaps {name}")
         a = capi.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
                                     q.stride(0), q.stride(1), out.stride(0), out.stride(1), indptr.data_ptr(),
@@ -244,13 +255,13 @@ class PagedCache:
         check(lib().mononn_paged_attention_workspace(C.byref(self._args), C.byref(a), C.byref(need)))
         if need.value:
             if workspace is None:
-                workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+                workspace = made_here(need.value, dtype=torch.uint8)
             if workspace.device != q.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous on {q.device}")
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
         run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a))
-        run.out, run.workspace = out, workspace if need.value else None
+        run.out = out
         return run
 
     def attention(self, q, indptr, out=None, lse=None, scale=None, causal=True, window=0, max_new=0, workspace=None,
@@ -263,11 +274,6 @@ class PagedCache:
         workspace is allocated through torch unless given; concurrent calls need one each."""
         run = self.attention_runner(q, indptr, out, lse, scale, causal, window, max_new, workspace, stream)
         run()
-        if stream is not None:  # what this call allocated is in use on that stream
-            import torch
-            for t in (run.out if out is None else None, run.workspace if workspace is None else None):
-                if t is not None:
-                    t.record_stream(stream)
         return run.out
 
 

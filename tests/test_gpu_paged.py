@@ -414,3 +414,126 @@ def test_follows_the_prompt_of_the_stand_alone_attention():
     _, _, limit, _ = p.want()
     # the other one rounds its probabilities after the division: two such limits apart at most, by the same count
     assert ((out.double() - old.double()).abs() <= 2 * limit + 2 * u(F16) * out.double().abs()).all()
+
+
+# ------------------------------------------------------------------------------ further edges
+@pytest.mark.parametrize("max_new", [1, 500])
+@pytest.mark.parametrize("group, dim", [(200, 64), (129, 128), (128, 64), (65, 128), (64, 128), (24, 64), (7, 128), (5, 80), (3, 64)])
+def test_wide_and_odd_groups(group, dim, max_new):
+    """Groups that leave rows of a tile unused, fill it alone, or are too wide for one."""
+    p = Problem([1, 9, 0, 70], [40, 700, 3, 333], 1, group, dim, 16, BF16, seed=group)
+    p.check(*attend(p, max_new=max_new))
+
+
+@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("pages", [31, 32, 33, 64, 65])
+def test_caches_around_the_size_from_which_items_are_split(pages, max_new):
+    p = Problem([1, 40, 2, 0], [pages * 16, pages * 16 - 7, 17, 300], 2, 4, 64, 16, F16, seed=pages)
+    p.table = p.table[:, :pages].contiguous()
+    p.check(*attend(p, max_new=max_new))
+
+
+@pytest.mark.parametrize("max_new", [1, 300])
+def test_pages_that_end_inside_a_tile(max_new):
+    """Page sizes that share no large factor with a tile of keys."""
+    for page in (8, 24, 40, 56, 200, 1000):
+        p = Problem([1, 33, 5], [1013, 700, page], 2, 2, 128, page, F16, seed=page)
+        p.check(*attend(p, max_new=max_new))
+
+
+@pytest.mark.parametrize("max_new", [1, 300])
+def test_nothing_new(max_new):
+    """No sequence has a new token: nothing is written."""
+    p = Problem([0, 0, 0], [5, 900, 0], 2, 2, 64, 16, F16, spare_rows=3)
+    out, lse = attend(p, max_new=max_new)
+    assert (out == 7.0).all() and (lse == 5.0).all()
+    new = torch.ones(3, 2, 64, device="cuda", dtype=F16)
+    before = p.k.clone(), p.v.clone()
+    q = torch.randn(3, 4, 64, device="cuda").to(F16)
+    keep = q.clone()
+    p.cache().append(new, new, p.indptr, Rotary(64), q=q)
+    assert torch.equal(p.k, before[0]) and torch.equal(p.v, before[1]) and torch.equal(q, keep)
+
+
+def test_tensors_without_elements():
+    p = Problem([0, 0], [5, 9], 2, 2, 64, 16, F16)
+    cache, none = p.cache(), torch.empty(0, 2, 64, device="cuda", dtype=F16)
+    assert cache.attention(p.q, p.indptr).shape == (0, 4, 64)
+    assert cache.append(none, none, p.indptr, Rotary(64), q=p.q).shape == (0, 4, 64)
+    assert rotary(p.q, torch.empty(0, device="cuda", dtype=torch.int32), Rotary(64)).shape == (0, 4, 64)
+    empty = PagedCache(p.k, p.v, p.table[:0], p.lengths[:0])
+    start = torch.zeros(1, device="cuda", dtype=torch.int32)
+    out = torch.full((2, 4, 64), 7.0, device="cuda", dtype=F16)
+    empty.attention(torch.zeros_like(out), start, out=out)
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("max_new", [1, 300])
+def test_overlapping_sequences_stay_in_bounds(max_new):
+    """An indptr that decreases is not allowed; what it leads to stays within the tensors all the same."""
+    p = Problem([31, 0, 0], [200, 90, 900], 2, 2, 64, 16, F16, spare_rows=4)
+    p.indptr.copy_(torch.tensor([0, 31, 0, 31], dtype=torch.int32))
+    out, lse = attend(p, max_new=max_new)
+    assert (out[31:] == 7.0).all() and (lse[31:] == 5.0).all()
+    assert torch.isfinite(out[:31]).all()
+
+
+@pytest.mark.parametrize("max_new", [1, 300])
+def test_a_runner_reads_what_its_buffers_hold(max_new):
+    p = Problem([1, 30, 2], [400, 900, 77], 2, 2, 64, 16, BF16, seed=21)
+    run = p.cache().attention_runner(p.q, p.indptr, max_new=max_new)
+    run()
+    p.check(run.out)
+    p.q.copy_(torch.randn(p.q.shape, device="cuda"))
+    p.news, p.lens, p.starts = [3, 0, 30], [399, 20, 64], [0, 3, 3, 33]
+    p.indptr.copy_(torch.tensor(p.starts, dtype=torch.int32))
+    p.lengths.copy_(torch.tensor(p.lens, dtype=torch.int32))
+    run()
+    p.check(run.out)
+
+
+def test_calls_on_several_streams_at_once():
+    """Each with a workspace of its own, over one cache."""
+    p = Problem([1, 64, 1], [9000, 5000, 20000], 2, 4, 128, 16, F16, seed=23)
+    first, _ = attend(p)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    runs = []
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        runs.append(p.cache().attention_runner(p.q, p.indptr, max_new=1 if i % 2 else 300, stream=s))
+    for _ in range(20):
+        for run in runs:
+            run()
+    torch.cuda.synchronize()
+    paged_attention_status()
+    for run in runs[::2]:
+        assert torch.equal(run.out, runs[0].out)
+    for run in runs[1::2]:
+        assert torch.equal(run.out, runs[1].out)
+        p.check(run.out)
+    p.check(runs[0].out)
+    p.check(first)
+
+
+@pytest.mark.parametrize("dim, heads", [(64, 3), (128, 9), (67, 2), (80, 1)])
+@pytest.mark.parametrize("config", [dict(rotary_dim=64), dict(rotary_dim=32, interleaved=True)])
+@pytest.mark.parametrize("tokens", [591, 592, 595, 2001])
+def test_rotary_of_many_tokens(tokens, config, dim, heads):
+    """Enough tokens that a block takes several, and a last block that is not full."""
+    x = torch.randn(tokens, heads, dim, device="cuda").to(BF16)
+    pos = torch.randint(0, 5000, (tokens,), device="cuda", dtype=torch.int32)
+    want, size = rotate(x, pos, *rates_of(config))
+    out = rotary(x, pos, Rotary(**config), out=torch.full_like(x, 9.0))
+    assert_rotated(out, want, size, BF16)
+    assert torch.equal(out[..., config["rotary_dim"]:], x[..., config["rotary_dim"]:])
+
+
+def test_vectors_and_single_elements_agree():
+    """The same rows at addresses that are and are not multiples of 16 bytes."""
+    x = torch.randn(700, 5, 128, device="cuda").to(F16)
+    pos = torch.arange(700, device="cuda", dtype=torch.int32) * 31
+    odd = torch.empty(700 * 5 * 128 + 1, device="cuda", dtype=F16)[1:].view(700, 5, 128)
+    for config in (dict(rotary_dim=128), dict(rotary_dim=64, interleaved=True)):
+        odd.copy_(x)
+        rotary(odd, pos, Rotary(**config))
+        assert torch.equal(odd, rotary(x, pos, Rotary(**config), out=torch.empty_like(x)))

@@ -12,7 +12,7 @@ FAKE = 1 << 20  # an aligned address that is never followed
 
 
 def cache_args(**change):
-    base = dict(k_pages=FAKE, v_pages=FAKE, page_stride=16 * 2 * 64, token_stride=2 * 64, head_stride=64,
+    base = dict(k_pages=FAKE, v_pages=2 * FAKE, page_stride=16 * 2 * 64, token_stride=2 * 64, head_stride=64,
                 page_table=FAKE, table_stride=4, lengths=FAKE, sequences=2, max_pages=4, num_pages=9, page_size=16,
                 kv_heads=2, head_dim=64, dtype=0)
     return capi.PagedCacheArgs(**{**base, **change})
@@ -137,7 +137,18 @@ def test_nothing_to_do_is_fine(lib_built):
     assert append(args=append_args(tokens=0)) == 0
     table = Rotary(64).table()
     assert capi.lib().mononn_rotary_apply(C.byref(table), C.byref(rotary_args(tokens=0)), None) == 0
+    # tensors without elements have no addresses
+    none = dict.fromkeys(("q", "out", "indptr"))
+    assert attend(cache=cache_args(k_pages=None, v_pages=None, num_pages=0), args=attention_args(tokens=0, **none)) == 0
+    assert attend(cache=cache_args(sequences=0, page_table=None, lengths=None)) == 0
+    assert append(args=append_args(tokens=0, k=None, v=None, indptr=None)) == 0
+    assert append(cache=cache_args(sequences=0, page_table=None, lengths=None)) == 0
     lib = capi.lib()
+    assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(tokens=0, x=None, out=None, positions=None)), None) == 0
+    assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(heads=0, x=None, out=None)), None) == 0
+    need = C.c_size_t(7)
+    assert lib.mononn_paged_attention_workspace(C.byref(cache_args()), C.byref(attention_args(tokens=0, **none)), C.byref(need)) == 0
+    assert need.value == 0
     assert lib.mononn_paged_attention(None, C.byref(attention_args()), None) == -1
     assert lib.mononn_paged_append(C.byref(cache_args()), None, None, None) == -1
     assert lib.mononn_rotary_apply(None, C.byref(rotary_args()), None) == -1
@@ -211,3 +222,46 @@ def test_tensors_refused(lib_built):
             rotary_runner(*args, **kw)
     with pytest.raises(ValueError):
         Rotary(64, scaling="other").table()
+
+
+def test_places_written_twice_are_refused(lib_built):
+    """Two elements of what is written at one address: strides that are wide enough one by one, but not together."""
+    lib, table = capi.lib(), Rotary(64).table()
+    assert append(cache=cache_args(v_pages=FAKE)) == -1
+    assert append(cache=cache_args(head_stride=128)) == -1
+    assert append(cache=cache_args(page_stride=15 * 128 + 64)) == -1
+    assert append(cache=cache_args(head_stride=16 * 64, token_stride=64)) in PASSES
+    assert append(cache=cache_args(head_stride=9 * 16 * 64, page_stride=16 * 64, token_stride=64)) in PASSES
+    q = dict(q=FAKE, q_out=3 * FAKE, q_heads=4, q_token_stride=256, q_head_stride=64)
+    assert append(args=append_args(**q, q_out_token_stride=192, q_out_head_stride=64)) == -1
+    assert append(args=append_args(**q, q_out_token_stride=64, q_out_head_stride=192)) in PASSES
+    assert attend(args=attention_args(out_token_stride=192)) == -1
+    assert attend(args=attention_args(out_token_stride=64, out_head_stride=192)) in PASSES
+    assert attend(args=attention_args(tokens=1, out_token_stride=0)) in PASSES
+    out = dict(out=3 * FAKE, out_token_stride=64, out_head_stride=128)
+    assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(**out)), None) == -1
+    out["out_head_stride"] = 192
+    assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(**out)), None) in PASSES
+
+
+def test_tensors_that_want_gradients_are_refused(lib_built):
+    """No gradient is computed, so none may be lost without a word."""
+    cache = PagedCache(*small_cache())
+    new, q = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, 4, 64, dtype=torch.float16)
+    indptr, pos = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    grad = torch.zeros(3, 4, 64, dtype=torch.float16, requires_grad=True)
+    for call in (lambda: rotary_runner(grad, pos, Rotary(64)), lambda: cache.attention_runner(grad, indptr),
+                 lambda: cache.append_runner(grad[:, :2], new, indptr), lambda: cache.append_runner(new, grad[:, 2:], indptr),
+                 lambda: cache.append_runner(new, new, indptr, q=grad), lambda: cache.attention_runner(q, indptr, out=grad)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+
+
+def test_queries_may_not_overlap_what_is_appended(lib_built):
+    cache = PagedCache(*small_cache())
+    indptr = torch.zeros(3, dtype=torch.int32)
+    wide = torch.zeros(3, 8, 64, dtype=torch.float16)
+    q, k, v = wide[:, :4], wide[:, 4:6], wide[:, 6:]
+    for q_out in (wide[:, 2:6], wide[:, 4:]):
+        with pytest.raises(ValueError, match="overlaps"):
+            cache.append_runner(k, v, indptr, q=q, q_out=q_out)
