@@ -255,9 +255,6 @@ int check_attention(const mononn_paged_cache* cache, const mononn_paged_attentio
 }
 
 // Which kernel, how many CTAs, and whether an item may span them. Only sizes count that the host knows.
-constexpr uint32_t kWholeKeys = 512;      // caches of at most so many keys: no item is split
-constexpr uint32_t kFewLeastKeys = 512;   // of a CTA's share
-constexpr uint32_t kManyLeastKeys = 1024;
 int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_args& a, int sm_count, AttentionPlan* p) {
   const uint32_t group = a.q_heads / c.kv_heads;
   const uint64_t capacity = static_cast<uint64_t>(c.max_pages) * c.page_size;
@@ -271,21 +268,33 @@ int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_arg
   p->padded_dim = c.head_dim <= 64 ? 64 : 128;
   const uint32_t few = few_keys(p->padded_dim);
   const uint32_t whole_tokens = group <= kTileRows ? kTileRows / group * group : 0;  // rows of a row tile of the other
-  // More than 16 rows: the other kernel, which takes 57 to 61 us whatever the rows for 16 sequences of 3350 keys
-  // (8 key heads of 128), where this one takes 44 us for 16 rows, 66 for 32 and 94 for 48 (keys read again).
-  p->many = whole_tokens && (rows > kFewRows || items(kFewRows) * (tiles(few) + 2) >= kMostUnits);
+  // More than 16 rows: the kernel for many, which takes 57 to 61 us whatever the rows for 16 sequences of 3350 keys
+  // (8 key heads of 128), where the one for few takes 44 us for 16 rows, 66 for 32 and 94 for 48 (keys read again). But
+  // calls that leave most of the GPU idle are done sooner by the one for few, which starts and ends faster and has
+  // twice the CTAs: up to an item for each of those and seven units in all (8 key heads, 64 rows: a sequence of
+  // 2000 keys 14.9 us instead of 16.7, four 25.1 instead of 19.9; eight of 500 keys 13.8 and 14.8, of 1000 27.6 and 21.6;
+  // 128 rows, eight of 250 keys: 16.0 and 11.5).
+  const uint64_t few_ctas = 2 * static_cast<uint64_t>(static_cast<unsigned>(sm_count));
+  const uint64_t few_items = std::min<uint64_t>(c.sequences, a.tokens) * c.kv_heads * ((new_tokens * group + kFewRows - 1) / kFewRows);
+  const bool idle = few_items <= few_ctas && few_items * tiles(few) <= 7 * few_ctas;
+  p->many = whole_tokens && ((rows > kFewRows && !idle) || items(kFewRows) * (tiles(few) + 2) >= kMostUnits);
   p->rows = p->many ? kManyRows : kFewRows;
   p->item_rows = p->many ? 2 * whole_tokens : kFewRows;
   p->keys = p->many ? kManyKeys : few;
-  p->least_units = (p->many ? kManyLeastKeys : kFewLeastKeys) / p->keys;
+  // Units of a CTA's share, at least: joining takes longer than they do otherwise (many rows, 32 of them over 1000 keys,
+  // 8 key heads: 14.9 us with shares of one unit, 15.2 of two, 18.0 of four, 23.9 of eight; 400 rows: 20.9, 18.6, 20.4, 27.4;
+  // single tokens over 1000 keys: 8.6 with one unit, 9.1 with two, 13.1 with eight).
+  p->least_units = p->many ? 2 : 1;
   p->box = std::gcd(c.page_size, p->keys);
   p->item_cost = p->many ? 2 : 1;
   const uint64_t most_units = items(p->item_rows) * (tiles(p->keys) + p->item_cost);
   if (most_units >= kMostUnits)
     return fail(MONONN_ERR_TOO_LARGE, "attention: so many new tokens over so many keys count 2^31 units of work or more");
-  const bool whole = capacity <= kWholeKeys;
-  const uint64_t wanted = whole ? items(p->item_rows) : (most_units + p->least_units - 1) / p->least_units;
   const uint64_t most = static_cast<uint64_t>(p->many ? 1 : 2) * static_cast<unsigned>(sm_count);
+  // Short caches: no item is split, and the join not needed. One sequence and 8 key heads: 250 keys 7.8 us whole and 8.6
+  // split, 500 keys 10.6 and 8.0 (4 and 8 units); 64 sequences: 13.8 and 16.7, 26.7 and 29.4; a prompt of 500 tokens 16.6 and 27.8.
+  const bool whole = tiles(p->keys) <= 4 || (!p->many && tiles(p->keys) <= 8 && 2 * items(p->item_rows) >= most);
+  const uint64_t wanted = whole ? items(p->item_rows) : (most_units + p->least_units - 1) / p->least_units;
   p->ctas = static_cast<uint32_t>(std::max<uint64_t>(1, std::min(wanted, most)));
   p->joins = !whole && p->ctas > 1;
   p->workspace = 0;

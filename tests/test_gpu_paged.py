@@ -11,6 +11,7 @@ from mononn_b200 import PagedCache, Rotary, paged_attention_status, rotary  # no
 from tests.paged_reference import Problem, assert_rotated, rotary_rates, rotate, u  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
+MANY = 10 ** 6  # new tokens of a sequence, as a hint: the kernel for many rows, however small the problem
 
 
 def attend(p, **kw):
@@ -35,7 +36,7 @@ def test_single_tokens(dtype, kv_heads, group, dim, page, head_major):
     p.check(*attend(p))
 
 
-@pytest.mark.parametrize("max_new", [0, 16, 1000])
+@pytest.mark.parametrize("max_new", [0, 16, MANY])
 @pytest.mark.parametrize("dtype, kv_heads, group, dim, page", [
     (F16, 2, 1, 64, 16), (BF16, 1, 4, 128, 32), (F16, 1, 3, 96, 8), (BF16, 2, 8, 64, 128)])
 def test_ragged_batch(dtype, kv_heads, group, dim, page, max_new):
@@ -51,27 +52,27 @@ def test_ragged_batch(dtype, kv_heads, group, dim, page, max_new):
         assert (empty == 0).all()
 
 
-@pytest.mark.parametrize("max_new", [0, 500])
+@pytest.mark.parametrize("max_new", [0, MANY])
 @pytest.mark.parametrize("window", [1, 2, 31, 64, 129, 100000, 2 ** 32 - 1])
 def test_window(window, max_new):
     p = Problem([1, 5, 200, 40], [500, 300, 200, 1500], 2, 2, 64, 16, BF16, seed=window % 1000)
     p.check(*attend(p, window=window, max_new=max_new), window=window)
 
 
-@pytest.mark.parametrize("max_new", [0, 500])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_all_keys(max_new):
     p = Problem([1, 5, 200, 3, 4], [500, 300, 90, 1, 0], 2, 3, 128, 16, F16, seed=3)
     p.check(*attend(p, causal=False, max_new=max_new), causal=False)
 
 
-@pytest.mark.parametrize("max_new", [1, 64])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_long_split_sequences(max_new):
     """Items that span many CTAs, beside short ones."""
     p = Problem([1, 2, 1, 64], [20001, 70, 9000, 5000], 2, 4, 128, 16, BF16, seed=11)
     p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [1, 64])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_many_sequences(max_new):
     """More sequences than a CTA has threads, many of them without work."""
     lens = [(37 * i) % 90 for i in range(1500)]
@@ -80,7 +81,7 @@ def test_many_sequences(max_new):
     p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_what_no_row_sees_may_hold_anything(max_new):
     """NaN and infinities behind the lengths, in pages before the window (their table entries gone) and in
     pages of nobody."""
@@ -103,7 +104,7 @@ def test_what_no_row_sees_may_hold_anything(max_new):
         p.check(out, lse, window=window)
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_pages_out_of_range_read_as_zeros(max_new):
     p = Problem([1, 200], [100, 260], 1, 2, 64, 16, F16, seed=2)
     p.table[0, 2], p.table[1, 0], p.table[1, 5], p.table[1, 9] = -1, p.pages, 2 ** 31 - 1, -2 ** 31
@@ -114,7 +115,7 @@ def test_pages_out_of_range_read_as_zeros(max_new):
     p.check(out, lse)
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_lengths_and_indptr_out_of_range_stay_in_bounds(max_new):
     p = Problem([1, 30], [100, 100], 1, 2, 64, 16, F16, seed=2)
     p.lengths.copy_(torch.tensor([2 ** 31 - 1, -5], dtype=torch.int32))
@@ -123,7 +124,7 @@ def test_lengths_and_indptr_out_of_range_stay_in_bounds(max_new):
     assert (out[2:] == 0).all()  # a length below zero: no keys
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_strides_of_a_fused_projection(max_new):
     """q as a slice of one projection, out as a slice of a wider buffer, a cache with both in one page."""
     p = Problem([1, 90, 7], [300, 130, 70], 2, 2, 64, 16, BF16, seed=4)
@@ -140,7 +141,7 @@ def test_strides_of_a_fused_projection(max_new):
     assert (result == 3.0).all()
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 @pytest.mark.parametrize("scale", [1e-6, 0.5, 4.0])
 def test_scales(scale, max_new):
     """Nearly even probabilities, and ones that one key takes whole; scores far from zero."""
@@ -148,7 +149,7 @@ def test_scales(scale, max_new):
     p.check(*attend(p, scale=scale, max_new=max_new), scale=scale)
 
 
-@pytest.mark.parametrize("max_new", [0, 300])
+@pytest.mark.parametrize("max_new", [0, MANY])
 def test_rising_scores(max_new):
     """The running maximum goes up at every step."""
     p = Problem([1, 130], [2000, 1500], 1, 1, 64, 16, BF16, seed=8)
@@ -160,7 +161,7 @@ def test_rising_scores(max_new):
     p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_offsets_beyond_32_bits(max_new):
     """A cache of more than 2^32 bytes and 2^31 elements in each of its two buffers."""
     pages, page, heads, dim = 2 ** 31 // (16 * 2 * 128) + 64, 16, 2, 128
@@ -179,7 +180,7 @@ def test_offsets_beyond_32_bits(max_new):
     assert torch.equal(k[at, spot % page], new_k[0]) and torch.equal(v[at, spot % page], new_v[0])
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_same_bits_again_in_a_graph_and_on_another_stream(max_new):
     p = Problem([1, 1, 40, 1], [9000, 31, 700, 2500], 2, 4, 128, 16, BF16, seed=10)
     first, lse = attend(p, max_new=max_new)
@@ -417,7 +418,7 @@ def test_follows_the_prompt_of_the_stand_alone_attention():
 
 
 # ------------------------------------------------------------------------------ further edges
-@pytest.mark.parametrize("max_new", [1, 500])
+@pytest.mark.parametrize("max_new", [1, MANY])
 @pytest.mark.parametrize("group, dim", [(200, 64), (129, 128), (128, 64), (65, 128), (64, 128), (24, 64), (7, 128), (5, 80), (3, 64)])
 def test_wide_and_odd_groups(group, dim, max_new):
     """Groups that leave rows of a tile unused, fill it alone, or are too wide for one."""
@@ -425,7 +426,7 @@ def test_wide_and_odd_groups(group, dim, max_new):
     p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 @pytest.mark.parametrize("pages", [31, 32, 33, 64, 65])
 def test_caches_around_the_size_from_which_items_are_split(pages, max_new):
     p = Problem([1, 40, 2, 0], [pages * 16, pages * 16 - 7, 17, 300], 2, 4, 64, 16, F16, seed=pages)
@@ -433,7 +434,7 @@ def test_caches_around_the_size_from_which_items_are_split(pages, max_new):
     p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_pages_that_end_inside_a_tile(max_new):
     """Page sizes that share no large factor with a tile of keys."""
     for page in (8, 24, 40, 56, 200, 1000):
@@ -441,7 +442,7 @@ def test_pages_that_end_inside_a_tile(max_new):
         p.check(*attend(p, max_new=max_new))
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_nothing_new(max_new):
     """No sequence has a new token: nothing is written."""
     p = Problem([0, 0, 0], [5, 900, 0], 2, 2, 64, 16, F16, spare_rows=3)
@@ -468,7 +469,7 @@ def test_tensors_without_elements():
     assert (out == 7.0).all()
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_overlapping_sequences_stay_in_bounds(max_new):
     """An indptr that decreases is not allowed; what it leads to stays within the tensors all the same."""
     p = Problem([31, 0, 0], [200, 90, 900], 2, 2, 64, 16, F16, spare_rows=4)
@@ -478,7 +479,7 @@ def test_overlapping_sequences_stay_in_bounds(max_new):
     assert torch.isfinite(out[:31]).all()
 
 
-@pytest.mark.parametrize("max_new", [1, 300])
+@pytest.mark.parametrize("max_new", [1, MANY])
 def test_a_runner_reads_what_its_buffers_hold(max_new):
     p = Problem([1, 30, 2], [400, 900, 77], 2, 2, 64, 16, BF16, seed=21)
     run = p.cache().attention_runner(p.q, p.indptr, max_new=max_new)
@@ -500,7 +501,7 @@ def test_calls_on_several_streams_at_once():
     runs = []
     for i, s in enumerate(streams):
         s.wait_stream(torch.cuda.current_stream())
-        runs.append(p.cache().attention_runner(p.q, p.indptr, max_new=1 if i % 2 else 300, stream=s))
+        runs.append(p.cache().attention_runner(p.q, p.indptr, max_new=1 if i % 2 else MANY, stream=s))
     for _ in range(20):
         for run in runs:
             run()
