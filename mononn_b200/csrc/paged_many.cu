@@ -22,6 +22,11 @@ constexpr int kPieces = 4;                  // told ahead
 constexpr uint32_t kSoftmaxRegisters = 216, kOtherRegisters = 72, kLaunchRegisters = 168;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreadsMany * kLaunchRegisters, "register split");
 constexpr float kRise = 8.0f;  // in powers of two
+// Heads of 65 to 128: of the probabilities of a unit, by the reference that their row has. Above, the unit is done again by a
+// higher one. A sum is there anyway, and no probability is above it, so the maxima are left out: they are on the chain from
+// one unit's scores to the next one's (8192 x 8192 x 8 heads of 128: 236 us with them, 222 without). 64-wide heads keep them, as
+// their scores have to make room before the sum is known.
+constexpr float kMostSum = 256.0f;
 
 template <int DIM>
 struct ManySmem {
@@ -187,18 +192,24 @@ __device__ __forceinline__ float at_least(float x, float low) {  // NaN stays Na
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
   return r;
 }
+__device__ __forceinline__ float within(float x, float low, float high) {  // NaN stays NaN
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tmax.NaN.f32 t, %1, %2;\n\tmin.NaN.f32 %0, t, %3;\n\t}" : "=f"(r) : "f"(x), "f"(low), "f"(high));
+  return r;
+}
 // Kept in its order, which is that of the loop below: the exponentials of one group beside the sums of the last.
 __device__ __forceinline__ float exp2_in_order(float x) {
   float y;
   asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^x for two x of at most 127 on the arithmetic pipes: 2^n from the integer nearest to x, times a polynomial of degree
+// 2^x for two x on the arithmetic pipes: 2^n from the integer nearest to x, times a polynomial of degree
 // 4 on -1/2 .. 1/2 (smallest largest relative error, 2.6e-6, found by exchange of its extrema). Below -126.5
-// it is 0, as for a key that is hidden.
+// it is 0, as for a key that is hidden; from 127.5 on it is infinite.
+template <bool BOUNDED>
 __device__ __forceinline__ float2 exp2_polynomial(uint64_t x) {
   const float2 v = apart(x);
-  x = two(at_least(v.x, -127.f), at_least(v.y, -127.f));
+  x = BOUNDED ? two(at_least(v.x, -127.f), at_least(v.y, -127.f)) : two(within(v.x, -127.f, 128.f), within(v.y, -127.f, 128.f));
   const uint64_t moved = add_two(x, two(12582912.f, 12582912.f));  // 1.5 x 2^23: the integer is in the low bits
   const uint64_t whole = add_two(moved, two(-12582912.f, -12582912.f));
   const uint64_t f = multiply_add_two(whole, two(-1.f, -1.f), x);
@@ -214,9 +225,8 @@ __device__ __forceinline__ float2 exp2_polynomial(uint64_t x) {
 // The probabilities exp2(scale x s + shift) of 32 scores, rounded to T once and stored from column `at` on, and their sum.
 // The special-function units take 8 cycles for the exponentials of a warp and bound this loop: one of eight goes to
 // the arithmetic pipes instead, which have time left.
-template <typename T>
-__device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t at, uint64_t scales, uint64_t shifts, uint64_t (&sum)[2]) {
-  uint32_t p[16];
+template <typename T, bool BOUNDED>
+__device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t* p, uint64_t scales, uint64_t shifts, uint64_t (&sum)[2]) {
 #pragma unroll
   for (int g = 0; g <= 4; ++g) {
     if (g < 4) {
@@ -225,7 +235,7 @@ __device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t at, ui
         const uint64_t x = multiply_add_two(two(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), scales, shifts);
         float2 e = apart(x);
         if (j % 16 == 14) {
-          e = exp2_polynomial(x);
+          e = exp2_polynomial<BOUNDED>(x);
         } else {
           e.x = exp2_in_order(e.x);
           e.y = exp2_in_order(e.y);
@@ -244,7 +254,6 @@ __device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t at, ui
       }
     }
   }
-  store_columns_16(at, p);  // over scores that have been read
 }
 // The key tiles of a piece that hold keys which some row of row tile t sees.
 __device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
@@ -507,85 +516,161 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           if (!fine) break;
           score_phase ^= 1u;
           after_sync();
-          const int32_t key0 = u * kKeys;
-          const bool tested = key0 < all_from || key0 + kKeys > all_to;
-          // The code of a unit is kept small (it is run by eight warps beside four others' that differ): the scores are
-          // read twice, for the maximum and for the probabilities, and hidden ones are put back as such.
-          float part[4] = {ninf, ninf, ninf, ninf};
-          uint32_t s[32], other[32];
-          if (tested) {
-#pragma unroll 1
-            for (int i = kKeys - 32; i >= 0; i -= 32) {
-              load_columns(s_at + i, s);
+          if constexpr (!kApart) {
+            const int32_t key0 = u * kKeys;
+            const bool tested = key0 < all_from || key0 + kKeys > all_to;
+            uint32_t s[32], other[32], p[64];
+            const uint64_t scales = two(P.scale_log2, P.scale_log2);
+            uint64_t shifts, sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+            bool again = __any_sync(0xffffffffu, valid && m == ninf);  // a row that has seen nothing has no reference
+            if (!again) {
+              const float shift = m * P.scale_log2;
+              shifts = two(-shift, -shift);
+              load_columns(s_at, s);
+              load_columns(s_at + 32, other);
               loads_done(s);
-              hide(s, see_from - key0 - i, see_to - key0 - i);
-              highest_32(s, part);
-              store_columns(s_at + i, s);
+              loaded(other);
+              if (tested) hide(s, see_from - key0, see_to - key0), hide(other, see_from - key0 - 32, see_to - key0 - 32);
+              probabilities<T, false>(s, p, scales, shifts, sum);
+              load_columns(s_at + 64, s);
+              probabilities<T, false>(other, p + 16, scales, shifts, sum);
+              loads_done(s);
+              load_columns(s_at + 96, other);
+              if (tested) hide(s, see_from - key0 - 64, see_to - key0 - 64);
+              probabilities<T, false>(s, p + 32, scales, shifts, sum);
+              loads_done(other);
+              if (tested) hide(other, see_from - key0 - 96, see_to - key0 - 96);
+              probabilities<T, false>(other, p + 48, scales, shifts, sum);
+              const float2 sums = apart(add_two(sum[0], sum[1]));
+              // no probability is above their sum
+              again = __any_sync(0xffffffffu, valid && !(sums.x + sums.y <= kMostSum));
             }
-            stores_done();
-          } else {
-            uint32_t rest[64];
-            load_columns(s_at, s);
-            load_columns(s_at + 32, other);
-            load_columns(s_at + 64, rest);
-            load_columns(s_at + 96, rest + 32);
-            loads_done(s);
-            loaded(other);
-            loaded(rest);
-            loaded(rest + 32);
-            highest_32(s, part);
-            highest_32(other, part);
-            highest_32(rest, part);
-            highest_32(rest + 32, part);
-          }
-          const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
-          if (kApart && u != from) {  // the last unit's probabilities have been used
-            fine = barrier_wait_warp(smem_address(&C.outputs[t]), output_phase, &C.gave_up);
-            if (!fine) break;
-            output_phase ^= 1u;
-            after_sync();
-          }
-          if (u == from) {
-            m = top;
-          } else {
-            // the scores of this unit are there, so the last unit's O is complete
-            const bool rise = valid && (top - m) * P.scale_log2 > kRise;
-            if (__any_sync(0xffffffffu, rise)) {
-              const float f = rise ? exp2_fast((m - top) * P.scale_log2) : 1.f;
-              if (rise) m = top;
-              l *= f;
+            if (again) {
+              float part[4] = {m, m, m, m};
 #pragma unroll 1
-              for (int i = 0; i < DIM; i += 16) {
-                uint32_t o[16];
-                load_columns_16(o_at + i, o);
-                loads_done_16(o);
+              for (int i = 0; i < kKeys; i += 32) {
+                load_columns(s_at + i, s);
+                loads_done(s);
+                if (tested) hide(s, see_from - key0 - i, see_to - key0 - i);
+                highest_32(s, part);
+              }
+              const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
+              if (u != from) {
+                // the scores of this unit are there, so the last unit's O is complete
+                const float f = top == m ? 1.f : exp2_fast((m - top) * P.scale_log2);
+                l *= f;
+#pragma unroll 1
+                for (int i = 0; i < DIM; i += 16) {
+                  uint32_t o[16];
+                  load_columns_16(o_at + i, o);
+                  loads_done_16(o);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                store_columns_16(o_at + i, o);
+                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                  store_columns_16(o_at + i, o);
+                }
+              }
+              m = top;
+              const float shift = m == ninf ? 0.f : m * P.scale_log2;
+              shifts = two(-shift, -shift);
+              sum[0] = sum[1] = two(0.f, 0.f);
+#pragma unroll 1
+              for (int i = 0; i < kKeys; i += 32) {
+                load_columns(s_at + i, s);
+                loads_done(s);
+                if (tested) hide(s, see_from - key0 - i, see_to - key0 - i);
+                probabilities<T, false>(s, p, scales, shifts, sum);
+                store_columns_16(p_at + i / 2, p);
+              }
+            } else {
+              store_columns(p_at, p);
+              store_columns(p_at + 32, p + 32);
+            }
+            const float2 sums = apart(add_two(sum[0], sum[1]));
+            l += sums.x + sums.y;
+          } else {
+            const int32_t key0 = u * kKeys;
+            const bool tested = key0 < all_from || key0 + kKeys > all_to;
+            // The code of a unit is kept small (it is run by eight warps beside four others' that differ): the scores are
+            // read twice, for the maximum and for the probabilities, and hidden ones are put back as such.
+            float part[4] = {ninf, ninf, ninf, ninf};
+            uint32_t s[32], other[32];
+            if (tested) {
+#pragma unroll 1
+              for (int i = kKeys - 32; i >= 0; i -= 32) {
+                load_columns(s_at + i, s);
+                loads_done(s);
+                hide(s, see_from - key0 - i, see_to - key0 - i);
+                highest_32(s, part);
+                store_columns(s_at + i, s);
               }
               stores_done();
+            } else {
+              uint32_t rest[64];
+              load_columns(s_at, s);
+              load_columns(s_at + 32, other);
+              load_columns(s_at + 64, rest);
+              load_columns(s_at + 96, rest + 32);
+              loads_done(s);
+              loaded(other);
+              loaded(rest);
+              loaded(rest + 32);
+              highest_32(s, part);
+              highest_32(other, part);
+              highest_32(rest, part);
+              highest_32(rest + 32, part);
             }
-          }
-          const float shift = m == ninf ? 0.f : m * P.scale_log2;
-          const uint64_t scales = two(P.scale_log2, P.scale_log2), shifts = two(-shift, -shift);
-          uint64_t sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+            const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
+            if (kApart && u != from) {  // the last unit's probabilities have been used
+              fine = barrier_wait_warp(smem_address(&C.outputs[t]), output_phase, &C.gave_up);
+              if (!fine) break;
+              output_phase ^= 1u;
+              after_sync();
+            }
+            if (u == from) {
+              m = top;
+            } else {
+              // the scores of this unit are there, so the last unit's O is complete
+              const bool rise = valid && (top - m) * P.scale_log2 > kRise;
+              if (__any_sync(0xffffffffu, rise)) {
+                const float f = rise ? exp2_fast((m - top) * P.scale_log2) : 1.f;
+                if (rise) m = top;
+                l *= f;
 #pragma unroll 1
-          for (int i = 0; i < kKeys; i += 64) {
-            load_columns(s_at + i + 32, other);
-            probabilities<T>(s, p_at + i / 2, scales, shifts, sum);
-            loads_done(other);
-            if (i == 0) {
-              load_columns(s_at + 64, s);
-            } else if (kApart) {  // the next scores may come
-              before_sync();
-              __syncwarp();
-              if (lane == 0) barrier_arrive(smem_address(&C.scores_read[t]));
+                for (int i = 0; i < DIM; i += 16) {
+                  uint32_t o[16];
+                  load_columns_16(o_at + i, o);
+                  loads_done_16(o);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                  store_columns_16(o_at + i, o);
+                }
+                stores_done();
+              }
             }
-            probabilities<T>(other, p_at + i / 2 + 16, scales, shifts, sum);
-            loads_done(s);
+            const float shift = m == ninf ? 0.f : m * P.scale_log2;
+            const uint64_t scales = two(P.scale_log2, P.scale_log2), shifts = two(-shift, -shift);
+            uint64_t sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
+#pragma unroll 1
+            for (int i = 0; i < kKeys; i += 64) {
+              load_columns(s_at + i + 32, other);
+              uint32_t p[16];
+              probabilities<T, true>(s, p, scales, shifts, sum);
+              store_columns_16(p_at + i / 2, p);  // over scores that have been read
+              loads_done(other);
+              if (i == 0) {
+                load_columns(s_at + 64, s);
+              } else if (kApart) {  // the next scores may come
+                before_sync();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(smem_address(&C.scores_read[t]));
+              }
+              probabilities<T, true>(other, p, scales, shifts, sum);
+              store_columns_16(p_at + i / 2 + 16, p);
+              loads_done(s);
+            }
+            const float2 sums = apart(add_two(sum[0], sum[1]));
+            l += sums.x + sums.y;
           }
-          const float2 sums = apart(add_two(sum[0], sum[1]));
-          l += sums.x + sums.y;
           stores_done();
           before_sync();
           __syncwarp();

@@ -104,6 +104,32 @@ def test_what_no_row_sees_may_hold_anything(max_new):
         p.check(out, lse, window=window)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("max_new", [1, MANY])
+def test_queries_of_no_sequence_may_hold_anything(max_new, dim):
+    """They share tiles with the last sequence's, and its results do not change for them."""
+    p = Problem([1, 37], [900, 1500], 2, 2, dim, 16, BF16, seed=12, spare_rows=40)
+    for bad in (math.nan, math.inf, 3e38):
+        p.q[p.starts[-1]:] = bad
+        out, lse = attend(p, max_new=max_new)
+        p.check(out, lse)
+
+
+@pytest.mark.parametrize("max_new", [1, MANY])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("jump", [3.0, 40.0, 3000.0])
+def test_scores_that_jump(jump, dim, max_new):
+    """Rows whose maximum rises little by little, then by a factor that no probability can hold, and falls again;
+    others whose highest score comes first."""
+    p = Problem([1, 140], [1100, 1400], 1, 2, dim, 16, BF16, seed=13, spread=0.5)
+    for b in range(2):
+        for i, page in enumerate(range(-(-p.lens[b] // p.page))):
+            at = p.table[b, page].item()
+            size = jump if i % 17 == 11 else 0.02 * i
+            p.k[at] = (torch.sign(p.q[p.starts[b], 0]).float() * size).to(BF16)
+    p.check(*attend(p, max_new=max_new))
+
+
 @pytest.mark.parametrize("max_new", [0, MANY])
 def test_pages_out_of_range_read_as_zeros(max_new):
     p = Problem([1, 200], [100, 260], 1, 2, 64, 16, F16, seed=2)
