@@ -297,10 +297,11 @@ int mononn_rotary_apply(const mononn_rotary* rotary, const mononn_rotary_args* a
  * p * page_stride + r * token_stride + h * head_stride + d in k_pages and v_pages alike, so pages may be
  * token-major or head-major. Sequence b's keys 0 .. lengths[b]-1 are in the pages page_table[b *
  * table_stride + key / page_size]. Attention counts a length beyond max_pages * page_size as that; the append
- * writes no token at a position beyond it. Sequences may share pages. A page number outside of 0 .. num_pages-1 is never followed: its tokens are not
- * written, and read as zeros. New tokens are packed: sequence b has the rows indptr[b] .. indptr[b+1]-1 of
- * the token tensors (indptr: [sequences + 1], not decreasing), and they are its LAST positions:
- * row indptr[b] + i is at position lengths[b] - (indptr[b+1] - indptr[b]) + i, so `lengths` counts them.
+ * writes no token at a position beyond it. Sequences may share pages. A page number outside of 0 ..
+ * num_pages-1 is never followed: its tokens are not written, and read as zeros. New tokens are packed: sequence
+ * b has the rows indptr[b] .. indptr[b+1]-1 of the token tensors (indptr: [sequences + 1], not decreasing), and
+ * they are its LAST positions: row indptr[b] + i is at position lengths[b] - (indptr[b+1] - indptr[b]) + i, so
+ * `lengths` counts them.
  * Rows outside of every sequence (behind indptr[sequences]) are left as they were. */
 typedef struct {
   void* k_pages;

@@ -1,15 +1,24 @@
 // Attention over a paged cache for many rows: prompts, chunks of prompts, drafts of wide groups.
 //
-// The same one pass over the keys as the kernel for few rows, on the fifth-generation tensor cores. An item has
-// up to 256 rows, two tiles of 128; a unit is 128 keys, loaded once for both. Roles of a CTA (one per SM):
-//   warps 4-7, 8-11 the softmax of one row tile each, a thread to a row: scores from tensor memory,
-//                   running maximum, probabilities back to tensor memory, row sums in registers
+// o = sum_j p_j v_j / sum_j p_j, p_j = exp2(c (s_j - r)), s_j = q.k_j, c = scale log2(e): any reference r of a row gives
+// the same o, so r need not be the maximum, only near enough that no p_j is too large. One pass over the keys, on
+// the fifth-generation tensor cores. An item has up to 256 rows, two tiles of 128; a unit is 128 keys, loaded once
+// for both. Roles of a CTA (one per SM):
+//   warps 4-7, 8-11 the softmax of one row tile each, a thread to a row: scores from tensor memory, probabilities
+//                   back to tensor memory, row sums in registers
 //   warp 0          issues the matrix products: S = Q K^T (both operands in shared memory), O += P V (P in
-//                   tensor memory, in the place of the scores it was made from)
+//                   tensor memory: in the place of the scores it was made from, or beside them for 64-wide heads)
 //   warps 1, 2      load keys (and queries) and values, page by page, into a ring of tiles
-// While one row tile's softmax runs, the tensor cores work on the other's products.
-// O stays in tensor memory. It is rescaled only when a row's maximum has risen by more than
-// 2^8 since its reference was set: until then probabilities are above 1, by 2^8 at most, which costs no accuracy.
+// While one row tile's softmax runs, the tensor cores work on the other's products. O stays in tensor memory. It is
+// rescaled only when a probability may be above 2^8: until then they are above 1, which costs no accuracy.
+//
+// 8192 queries x 8192 keys x 8 heads of 128: 223 us, 1230 TFLOP/s (0.76 of what a large matrix product reaches in such a
+// short run; the tensor cores are active in 0.66 of the cycles). 32 heads of 64: 680 us, 810 TFLOP/s. What bounds it is the
+// chain of a row tile: scores, softmax of 128 of them a thread (about 1600 of some 3300 cycles a unit), product with the
+// values, next scores, which have no other place with 128-wide heads (all 512 columns are used). It does not get
+// shorter by halving the units (next scores early, but products of 64 keys read 1.5 times as much shared memory: 228), by two
+// issuing warps (279), or by handing over the probabilities in halves (238); more exponentials by polynomial: 234. 64-wide
+// heads: exponentials and the 8 warps' other instructions, 0.55 of the special-function units' rate.
 #include "paged_device.h"
 
 namespace mononn {
@@ -17,11 +26,13 @@ namespace paged {
 
 constexpr int kRows = static_cast<int>(kManyRows), kKeys = static_cast<int>(kManyKeys);
 constexpr int kThreadsMany = 384;
-constexpr int kMmaWarp = 0, kKeyWarp = 1, kValueWarp = 2, kSoftmaxWarp = 4;  // 3 only makes up the group whose registers go to the others
+// The warps that issue and load come first: the scheduler prefers them, and they are on everybody's path. Warp 3 only makes
+// up the group whose registers go to the others.
+constexpr int kMmaWarp = 0, kKeyWarp = 1, kValueWarp = 2, kSoftmaxWarp = 4;
 constexpr int kPieces = 4;                  // told ahead
 constexpr uint32_t kSoftmaxRegisters = 216, kOtherRegisters = 72, kLaunchRegisters = 168;
 static_assert(256 * kSoftmaxRegisters + 128 * kOtherRegisters <= kThreadsMany * kLaunchRegisters, "register split");
-constexpr float kRise = 8.0f;  // in powers of two
+constexpr float kRise = 8.0f;  // 64-wide heads: how far a maximum may be above the reference, in powers of two
 // Heads of 65 to 128: of the probabilities of a unit, by the reference that their row has. Above, the unit is done again by a
 // higher one. A sum is there anyway, and no probability is above it, so the maxima are left out: they are on the chain from
 // one unit's scores to the next one's (8192 x 8192 x 8 heads of 128: 236 us with them, 222 without). 64-wide heads keep them, as
@@ -46,7 +57,8 @@ struct ManySmem {
 };
 struct ManyControl {
   uint64_t full[4], empty[4];  // of pairs
-  uint64_t scores[2], scores_read[2], probabilities[2], queries[2], queries_free[2], outputs[2], told[kPieces], taken[kPieces], drained;
+  uint64_t scores[2], scores_read[2], probabilities[2], outputs[2], queries[2], queries_free[2];  // of row tiles
+  uint64_t told[kPieces], taken[kPieces], drained;
   alignas(16) Piece pieces[kPieces];
   Share share;
   uint32_t sums[12];
@@ -209,7 +221,8 @@ __device__ __forceinline__ float exp2_in_order(float x) {
 template <bool BOUNDED>
 __device__ __forceinline__ float2 exp2_polynomial(uint64_t x) {
   const float2 v = apart(x);
-  x = BOUNDED ? two(at_least(v.x, -127.f), at_least(v.y, -127.f)) : two(within(v.x, -127.f, 128.f), within(v.y, -127.f, 128.f));
+  x = BOUNDED ? two(at_least(v.x, -127.f), at_least(v.y, -127.f))
+              : two(within(v.x, -127.f, 128.f), within(v.y, -127.f, 128.f));
   const uint64_t moved = add_two(x, two(12582912.f, 12582912.f));  // 1.5 x 2^23: the integer is in the low bits
   const uint64_t whole = add_two(moved, two(-12582912.f, -12582912.f));
   const uint64_t f = multiply_add_two(whole, two(-1.f, -1.f), x);
@@ -222,11 +235,13 @@ __device__ __forceinline__ float2 exp2_polynomial(uint64_t x) {
   return apart(multiply_two(y, two(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
                                    __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u))));
 }
-// The probabilities exp2(scale x s + shift) of 32 scores, rounded to T once and stored from column `at` on, and their sum.
+// The probabilities exp2(scale x s + shift) of 32 scores, rounded to T once, in pairs, and their sum.
 // The special-function units take 8 cycles for the exponentials of a warp and bound this loop: one of eight goes to
 // the arithmetic pipes instead, which have time left.
+// BOUNDED: none of them is above 2^127.
 template <typename T, bool BOUNDED>
-__device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t* p, uint64_t scales, uint64_t shifts, uint64_t (&sum)[2]) {
+__device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t* p, uint64_t scales, uint64_t shifts,
+                                              uint64_t (&sum)[2]) {
 #pragma unroll
   for (int g = 0; g <= 4; ++g) {
     if (g < 4) {
@@ -360,7 +375,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               if (lane == 0) {
                 const uint32_t bar = smem_address(&C.queries[t]);
                 barrier_arrive_bytes(bar, half * 128u * kHalves);
-                const int32_t token = walk.piece.token + static_cast<int32_t>(divide(walk.piece.first_row, P.by_group) + t * half_tokens);
+                const uint32_t from_token = divide(walk.piece.first_row, P.by_group) + t * half_tokens;
+                const int32_t token = walk.piece.token + static_cast<int32_t>(from_token);
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
                   load_queries(base + t * M::kTileBytes + h * (kTileRows * 128), &P.q_map, h * 64,
@@ -620,7 +636,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               highest_32(rest + 32, part);
             }
             const float top = fmaxf(max3(part[0], part[1], part[2]), part[3]);
-            if (kApart && u != from) {  // the last unit's probabilities have been used
+            if (u != from) {  // the last unit's probabilities have been used
               fine = barrier_wait_warp(smem_address(&C.outputs[t]), output_phase, &C.gave_up);
               if (!fine) break;
               output_phase ^= 1u;
@@ -659,7 +675,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               loads_done(other);
               if (i == 0) {
                 load_columns(s_at + 64, s);
-              } else if (kApart) {  // the next scores may come
+              } else {  // the next scores may come
                 before_sync();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(smem_address(&C.scores_read[t]));
@@ -689,7 +705,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         const float inverse = !complete ? 1.f : l == 0.f ? 0.f : 1.f / l;
         uint64_t row_at;  // where this thread's row goes
         if (complete) {
-          row_at = reinterpret_cast<uint64_t>(static_cast<T*>(P.out) + row_of * P.out_token + static_cast<int64_t>(head) * P.out_head);
+          row_at = reinterpret_cast<uint64_t>(static_cast<T*>(P.out) + row_of * P.out_token +
+                                              static_cast<int64_t>(head) * P.out_head);
           if (valid && P.lse) P.lse[row_of * P.kv_heads * P.group + head] = l == 0.f ? ninf : m * P.scale + logf(l);
         } else {
           float* slot = P.partial + (2u * blockIdx.x + (piece.begins ? 1u : 0u)) * static_cast<size_t>(kRows * (2 + DIM));
@@ -772,8 +789,8 @@ cudaError_t prepare() {
 }
 template <typename T, int DIM>
 cudaError_t launch(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
-  return launch_dependent(paged::many_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsMany, 1024 + paged::ManySmem<DIM>::kBytes, p,
-                          stream);
+  return launch_dependent(paged::many_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsMany,
+                          1024 + paged::ManySmem<DIM>::kBytes, p, stream);
 }
 }  // namespace
 cudaError_t prepare_many_rows() {

@@ -4,6 +4,9 @@
 // a head, t = position x f_i. The angle is taken in 64 bits as a share of a full turn (position x f_i / 2 pi, of
 // which only the fraction matters), so that positions of any size keep it to 32 bits; sine and
 // cosine of that share, and the products, are 32-bit. Bound by memory: every element is read once and written once.
+// 8192 tokens x 40 heads of 128 in place (168 MB): 34 us, 4.9 TB/s; append of 11.6k tokens x 32 heads of 64 (191 MB):
+// 34 us, 5.6 TB/s, 0.86 of what a copy reaches. One token: 3.0 us, the launch. A block takes a few tokens, so that
+// the angles and places, worked out once for all of their heads, are few beside the elements.
 #include "paged_device.h"
 
 namespace mononn {
@@ -161,7 +164,8 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_cons
       if (member) {
         const int32_t begin = P.indptr[b], end = P.indptr[b + 1], length = P.lengths[b];
         member = begin <= static_cast<int32_t>(token);
-        const int64_t at = static_cast<int64_t>(length) - (static_cast<int64_t>(end) - begin) + (static_cast<int64_t>(token) - begin);
+        const int64_t at = static_cast<int64_t>(length) - (static_cast<int64_t>(end) - begin) +
+                           (static_cast<int64_t>(token) - begin);
         position = static_cast<int32_t>(at);
         if (member && at >= 0 && at < static_cast<int64_t>(P.max_pages) * P.page_size) {
           const uint32_t n = divide(static_cast<uint32_t>(at), P.by_page_size);
@@ -211,12 +215,17 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_cons
 
 cudaError_t prepare_rows() {
   cudaFuncAttributes a;
-  for (cudaError_t e : {cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 1>), cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 8>),
+  for (cudaError_t e : {cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 1>),
+                        cudaFuncGetAttributes(&a, paged::rows_kernel<__half, 8>),
                         cudaFuncGetAttributes(&a, paged::rows_kernel<__nv_bfloat16, 1>),
                         cudaFuncGetAttributes(&a, paged::rows_kernel<__nv_bfloat16, 8>)})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
+// One token a block until there are four blocks for each SM, then four tokens a block (one and four, 32 heads of 128: 100 tokens
+// 3.7 and 5.2 us, 300 4.5 and 5.3, 592 5.6 and 4.7, 4000 16.0 and 12.7; two and eight for all of 8192: 35.5 and 38.0, four 34.5).
+// 16-byte vectors where everything is aligned to them, otherwise single elements: 2.7 and 4.2 us for one token, 9.5 and 21.4
+// for 2048, 26 and 55 for 8192 x 40 heads (in L2).
 cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int sm_count, cudaStream_t stream) {
   RowsParams p = params;
   p.block_tokens = p.tokens >= 4u * static_cast<unsigned>(sm_count) ? paged::kRowsTokens : 1u;

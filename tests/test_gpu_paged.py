@@ -445,7 +445,8 @@ def test_follows_the_prompt_of_the_stand_alone_attention():
 
 # ------------------------------------------------------------------------------ further edges
 @pytest.mark.parametrize("max_new", [1, MANY])
-@pytest.mark.parametrize("group, dim", [(200, 64), (129, 128), (128, 64), (65, 128), (64, 128), (24, 64), (7, 128), (5, 80), (3, 64)])
+@pytest.mark.parametrize("group, dim", [(200, 64), (129, 128), (128, 64), (65, 128), (64, 128), (24, 64), (7, 128),
+                                        (5, 80), (3, 64)])
 def test_wide_and_odd_groups(group, dim, max_new):
     """Groups that leave rows of a tile unused, fill it alone, or are too wide for one."""
     p = Problem([1, 9, 0, 70], [40, 700, 3, 333], 1, group, dim, 16, BF16, seed=group)

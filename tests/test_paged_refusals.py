@@ -147,8 +147,8 @@ def test_nothing_to_do_is_fine(lib_built):
     assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(tokens=0, x=None, out=None, positions=None)), None) == 0
     assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args(heads=0, x=None, out=None)), None) == 0
     need = C.c_size_t(7)
-    assert lib.mononn_paged_attention_workspace(C.byref(cache_args()), C.byref(attention_args(tokens=0, **none)), C.byref(need)) == 0
-    assert need.value == 0
+    rc = lib.mononn_paged_attention_workspace(C.byref(cache_args()), C.byref(attention_args(tokens=0, **none)), C.byref(need))
+    assert rc == 0 and need.value == 0
     assert lib.mononn_paged_attention(None, C.byref(attention_args()), None) == -1
     assert lib.mononn_paged_append(C.byref(cache_args()), None, None, None) == -1
     assert lib.mononn_rotary_apply(None, C.byref(rotary_args()), None) == -1
