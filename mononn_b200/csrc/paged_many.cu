@@ -748,13 +748,18 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           const uint32_t part = lane & 7u;
           const uint32_t element = complete ? static_cast<uint32_t>(i - 32) + part * 8 : static_cast<uint32_t>(i) + part * 4;
           const uint32_t offset = complete ? element * 2 : element * 4;
+          uint64_t to_row[8];
+          uint4 v[8];
 #pragma unroll
           for (uint32_t j = 0; j < 8; ++j) {
             const uint32_t row = j * 4 + (lane >> 3);
-            const uint64_t to_row = __shfl_sync(0xffffffffu, row_at, row);
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((part ^ (row & 7u)) << 4));
-            if (row < rows_here && (!complete || element < P.head_dim)) *reinterpret_cast<uint4*>(to_row + offset) = v;
+            to_row[j] = __shfl_sync(0xffffffffu, row_at, row);
+            v[j] = *reinterpret_cast<const uint4*>(stage + row * 128 + ((part ^ (row & 7u)) << 4));
           }
+          const bool wanted = !complete || element < P.head_dim;
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j)
+            if (wanted && j * 4 + (lane >> 3) < rows_here) *reinterpret_cast<uint4*>(to_row[j] + offset) = v[j];
           __syncwarp();
         }
         before_sync();
