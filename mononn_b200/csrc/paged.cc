@@ -512,7 +512,7 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.by_item_rows = make_divisor(p.item_rows);
   p.by_page_size = make_divisor(c.page_size);
   p.whole_items = !plan.joins;
-  p.min_units = plan.joins ? plan.least_units : 1;
+  p.least_shift = plan.joins && plan.least_units == 2 ? 1 : 0;
   p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
   p.scale_log2 = p.scale * 1.4426950408889634f;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);

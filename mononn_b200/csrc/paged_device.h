@@ -240,7 +240,7 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
     if (w < warp) before += x;
     total += x;
   }
-  const uint32_t ctas = min(gridDim.x, (total + P.min_units - 1u) / P.min_units);
+  const uint32_t ctas = min(gridDim.x, (total + (1u << P.least_shift) - 1u) >> P.least_shift);
   if (blockIdx.x < ctas) {
     const uint32_t share_each = total / ctas, longer = total - share_each * ctas;
     const uint32_t u0 = share_each * blockIdx.x + min(blockIdx.x, longer);
@@ -258,17 +258,18 @@ __device__ __forceinline__ void find_share(const AttentionParams& P, uint32_t* s
 #pragma unroll 1
       for (; b < end; ++b) {
         if (each > 1u) s = load_sequence(P, b);
-        per_head = head_units_warp<KEYS>(P, s, row_tiles(P, s));
+        const uint32_t tiles = row_tiles(P, s);
+        per_head = tiles == 1u ? item_units<KEYS>(P, s, 0) : head_units_warp<KEYS>(P, s, tiles);
         found = u0 - at < per_head * P.kv_heads;
         if (found) break;
         at += per_head * P.kv_heads;
       }
-      const uint32_t head = (u0 - at) / per_head;
+      const uint32_t head = per_head == 1u ? u0 - at : (u0 - at) / per_head;
       uint32_t left = u0 - at - head * per_head, tile = 0;
       const uint32_t tiles = found ? row_tiles(P, s) : 0u;
-      found = false;
+      found = found && tiles == 1u;  // nothing to look for then
 #pragma unroll 1
-      for (uint32_t t0 = 0; t0 < tiles; t0 += 32u) {
+      for (uint32_t t0 = 0; !found && t0 < tiles; t0 += 32u) {
         const uint32_t u = t0 + lane < tiles ? item_units<KEYS>(P, s, t0 + lane) : 0u;
         uint32_t sum = u;
 #pragma unroll
