@@ -503,7 +503,7 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.head_dim = c.head_dim;
   p.page_size = c.page_size;
   p.capacity = c.max_pages * c.page_size;
-  p.box = plan.box;
+  while ((1u << p.box_shift) < plan.box) ++p.box_shift;  // a power of two, as the keys of a unit are
   p.item_rows = plan.item_rows;
   p.item_cost = plan.item_cost;
   p.causal = a.causal != 0;

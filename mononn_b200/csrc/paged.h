@@ -76,7 +76,7 @@ struct AttentionParams {
   AttentionHeader* headers;
   float* partial;           // slots 2 * CTA (an item begun earlier) and 2 * CTA + 1 (one that goes on)
   uint32_t* status;
-  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box, item_rows, item_cost;
+  uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box_shift, item_rows, item_cost;
   uint32_t causal, window, least_shift, whole_items;
   Divisor by_group, by_item_rows, by_page_size;
   float scale, scale_log2;  // of the scores; scale * log2(e)

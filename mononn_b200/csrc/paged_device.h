@@ -405,13 +405,13 @@ struct TileLoader {
   int32_t keys_begin, keys_end;
   int32_t page, row, next_page, next_row;  // row below 0: not wanted
   __device__ __forceinline__ TileLoader(const AttentionParams& params)
-      : P(params), lane(threadIdx.x & 31u), boxes(KEYS / params.box), window(32u / boxes), sequence(0), first(0),
+      : P(params), lane(threadIdx.x & 31u), boxes(KEYS >> params.box_shift), window((32u << params.box_shift) / KEYS), sequence(0), first(0),
         keys_begin(0), keys_end(0), page(-1), row(-1), next_page(-1), next_row(-1) {}
   __device__ __forceinline__ void look_up(uint32_t tile0, int32_t& page_of, int32_t& row_of) const {
-    const int32_t key = static_cast<int32_t>(tile0 * KEYS + lane * P.box);
+    const int32_t key = static_cast<int32_t>(tile0 * KEYS + (lane << P.box_shift));
     page_of = -1;
     row_of = -1;
-    if (key < keys_end && key + static_cast<int32_t>(P.box) > keys_begin) {
+    if (key < keys_end && key + (1 << P.box_shift) > keys_begin) {
       const uint32_t p = divide(static_cast<uint32_t>(key), P.by_page_size);
       row_of = key - static_cast<int32_t>(p * P.page_size);
       page_of = P.table[static_cast<int64_t>(sequence) * P.table_stride + p];
@@ -437,12 +437,12 @@ struct TileLoader {
     const int32_t p = __shfl_sync(0xffffffffu, page, from), r = __shfl_sync(0xffffffffu, row, from);
     const bool wanted = lane < boxes && r >= 0;
     const uint32_t count = __popc(__ballot_sync(0xffffffffu, wanted));
-    if (lane == 0) barrier_arrive_bytes(bar, count * P.box * 128u * HALVES);
+    if (lane == 0) barrier_arrive_bytes(bar, (count << P.box_shift) * 128u * HALVES);
     __syncwarp();
     if (wanted) {
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
-        load_box(dst + h * KEYS * 128 + lane * P.box * 128u, map, h * 64, r, static_cast<int32_t>(head), p, bar);
+        load_box(dst + h * KEYS * 128 + ((lane << P.box_shift) * 128u), map, h * 64, r, static_cast<int32_t>(head), p, bar);
     }
     if (tile == first) look_up(first + window, next_page, next_row);
   }
