@@ -82,7 +82,7 @@ struct AttentionParams {
   float scale, scale_log2;  // of the scores; scale * log2(e)
 };
 struct AttentionPlan {  // how a call is launched: the same for every content of its device arrays
-  bool many;            // the kernel for many rows
+  bool many, turns;     // the kernel for many rows; with row tiles that may take turns
   uint32_t rows, keys, padded_dim, ctas, least_units;  // rows: of a slot of the workspace
   uint32_t item_rows;   // rows of an item, at most `rows`
   uint32_t item_cost;   // units that stand for an item's work beside its keys

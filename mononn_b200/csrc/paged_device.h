@@ -303,7 +303,7 @@ struct Piece {
   uint32_t begins, ends;           // whether the item begins and ends in it
   uint32_t valid;                  // 0: no more pieces
   uint32_t sequence;
-  int32_t pad[2];
+  uint32_t shared, pad;            // many rows: 1 when the two row tiles hold the same rows, for every other key tile each
   int32_t from[2], to[2];          // many rows: the key tiles from .. to - 1 that concern each of the two row tiles
 };
 // Walks through the pieces of a share; all lanes of the loading warp alike.
@@ -391,7 +391,7 @@ __device__ __forceinline__ void put_piece(Piece* to, const Piece& p, uint32_t la
   d[0] = make_int4(p.token, p.n, p.length, static_cast<int>(p.head));
   d[1] = make_int4(static_cast<int>(p.first_row), static_cast<int>(p.rows), p.tile, p.count);
   d[2] = make_int4(p.keys_begin, p.keys_end, static_cast<int>(p.begins), static_cast<int>(p.ends));
-  d[3] = make_int4(static_cast<int>(p.valid), static_cast<int>(p.sequence), 0, 0);
+  d[3] = make_int4(static_cast<int>(p.valid), static_cast<int>(p.sequence), static_cast<int>(p.shared), 0);
   d[4] = make_int4(p.from[0], p.from[1], p.to[0], p.to[1]);
 }
 

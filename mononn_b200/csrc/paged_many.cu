@@ -59,6 +59,7 @@ struct ManyControl {
   uint64_t full[4], empty[4];  // of pairs
   uint64_t scores[2], scores_read[2], probabilities[2], outputs[2], queries[2], queries_free[2];  // of row tiles
   uint64_t told[kPieces], taken[kPieces], drained;
+  uint64_t other_done, other_read;  // of two row tiles that hold the same rows, the second
   alignas(16) Piece pieces[kPieces];
   Share share;
   uint32_t sums[12];
@@ -270,7 +271,9 @@ __device__ __forceinline__ void probabilities(uint32_t (&s)[32], uint32_t* p, ui
     }
   }
 }
-// The key tiles of a piece that hold keys which some row of row tile t sees.
+// The key tiles of a piece that hold keys which some row of row tile t sees. Where the rows fill no more than one tile, both
+// hold them, and take turns with the key tiles: the chain of a row tile (see above) is then half as long.
+template <bool TURNS>
 __device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
   const uint32_t half = P.item_rows / 2;
 #pragma unroll
@@ -283,9 +286,16 @@ __device__ __forceinline__ void set_ranges(const AttentionParams& P, Piece& p) {
     p.from[t] = max(p.tile, k.begin / kKeys);
     p.to[t] = max(p.from[t], min(p.tile + p.count, (k.end + kKeys - 1) / kKeys));
   }
+  p.shared = TURNS && p.rows <= half && p.to[0] > p.from[0] + 1 ? 1u : 0u;
+  if (p.shared) {  // `to` is one behind the last tile of a turn
+    p.from[1] = p.from[0] + 1;
+    p.to[1] = p.from[1] + ((p.to[0] - p.from[1] - 1) & ~1) + 1;
+    p.to[0] = p.from[0] + ((p.to[0] - p.from[0] - 1) & ~1) + 1;
+  }
 }
 
-template <typename T, int DIM>
+// TURNS: whether row tiles may take turns, which costs the issuing warp some code.
+template <typename T, int DIM, bool TURNS>
 __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid_constant__ AttentionParams P) {
   extern __shared__ uint8_t raw[];
   using M = ManySmem<DIM>;
@@ -314,6 +324,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       barrier_init(smem_address(&C.taken[i]), 10);  // all but the warp that tells
     }
     barrier_init(smem_address(&C.drained), 1);
+    barrier_init(smem_address(&C.other_done), 4);
+    barrier_init(smem_address(&C.other_read), 4);
     C.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));
@@ -345,7 +357,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         const bool some = walk.next();
         if (some) {
           loader.begin(walk.piece);
-          set_ranges(P, walk.piece);
+          set_ranges<TURNS>(P, walk.piece);
         }
         const uint32_t at = i % kPieces;
         fine = barrier_wait_warp(smem_address(&C.taken[at]), ((i / kPieces) & 1u) ^ 1u, &C.gave_up);
@@ -375,7 +387,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               if (lane == 0) {
                 const uint32_t bar = smem_address(&C.queries[t]);
                 barrier_arrive_bytes(bar, half * 128u * kHalves);
-                const uint32_t from_token = divide(walk.piece.first_row, P.by_group) + t * half_tokens;
+                const uint32_t from_token = divide(walk.piece.first_row, P.by_group) + (TURNS && walk.piece.shared ? 0u : t * half_tokens);
                 const int32_t token = walk.piece.token + static_cast<int32_t>(from_token);
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
@@ -429,6 +441,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         const int32_t first = piece.tile, end = first + piece.count;
         const int32_t from[2] = {piece.from[0], piece.from[1]}, to[2] = {piece.to[0], piece.to[1]};
         const int32_t keys_begin = piece.keys_begin, keys_end = piece.keys_end;
+        const int32_t turns = TURNS ? static_cast<int32_t>(piece.shared) : 0;
         // step u: O += P V of unit u, then the scores of unit u + 1, for one row tile after the other
         for (int32_t u = first - 1; fine && u < end; ++u) {
           const uint32_t slot = step % kPairs;
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             __syncwarp();
           }
           auto weigh = [&](int t) {  // O += P V of unit u; false after a wait that gave up
-            if (u < from[t] || u >= to[t]) return true;
+            if (u < from[t] || u >= to[t] || ((u - from[t]) & turns)) return true;
             if (!barrier_wait_warp(smem_address(&C.probabilities[t]), probability_phase[t], &C.gave_up)) return false;
             probability_phase[t] ^= 1u;
             after_sync();
@@ -463,7 +476,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
             return true;
           };
           auto score = [&](int t) {  // S of unit u + 1
-            if (u + 1 < from[t] || u + 1 >= to[t]) return true;
+            if (u + 1 < from[t] || u + 1 >= to[t] || ((u + 1 - from[t]) & turns)) return true;
             if (kApart) {
               if (!barrier_wait_warp(smem_address(&C.scores_read[t]), read_phase[t], &C.gave_up)) return false;
               read_phase[t] ^= 1u;
@@ -488,9 +501,13 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           };
           // Where scores and probabilities have places of their own the next scores come first, as soon as the last
           // ones have been read; otherwise behind the product that reads the probabilities in their place.
+          // Tiles that take turns: the second one's scores need not wait for the first one's probabilities.
+          if (turns) fine = score(1);
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            fine = fine && (kApart ? score(t) && weigh(t) : weigh(t) && score(t));
+          for (int t = 0; t < 2; ++t) {
+            const bool scored = t == 1 && turns;
+            fine = fine && (kApart ? (scored || score(t)) && weigh(t) : weigh(t) && (scored || score(t)));
+          }
           if (issuer && fine) commit(smem_address(&C.empty[slot]));
         }
         if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
@@ -507,7 +524,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
     const uint32_t s_at = tmem + M::score_column(t) + lanes, p_at = tmem + M::probability_column(t) + lanes,
                    o_at = tmem + M::output_column(t) + lanes;
     const float ninf = __int_as_float(0xff800000);
-    uint32_t score_phase = 0, output_phase = 0;
+    uint32_t score_phase = 0, output_phase = 0, other_phase = 0;
     const uint32_t half = P.item_rows / 2;
     uint8_t* const stage = smem + M::kStage + (warp - kSoftmaxWarp) * 4096;
     for (uint32_t n = 0;; ++n) {
@@ -515,7 +532,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       fine = barrier_wait_warp(smem_address(&C.told[at]), (n / kPieces) & 1u, &C.gave_up);
       const Piece& piece = C.pieces[at];
       if (!fine || piece.valid == 0) break;
-      const uint32_t r = t * half + thread;  // row of the item
+      const bool shared = TURNS && piece.shared != 0;
+      const uint32_t r = (shared ? 0u : t * half) + thread;  // row of the item
       const bool valid = thread < half && r < piece.rows;
       const uint32_t g = piece.first_row + r;
       const int32_t from = piece.from[t], to = piece.to[t];
@@ -527,7 +545,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         const int32_t all_from = __reduce_max_sync(0xffffffffu, see_from);
         const int32_t all_to = __reduce_min_sync(0xffffffffu, see_to);
 
-        for (int32_t u = from; u < to; ++u) {
+        for (int32_t u = from; u < to; u += shared ? 2 : 1) {
           fine = barrier_wait_warp(smem_address(&C.scores[t]), score_phase, &C.gave_up);
           if (!fine) break;
           score_phase ^= 1u;
@@ -698,7 +716,31 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         output_phase ^= 1u;
         after_sync();
       }
-      if (t * half < piece.rows) {
+      // Two tiles of the same rows: the second leaves its references and sums in its stage, the first takes these and
+      // the second's O, which is in its own lanes of tensor memory.
+      float keep = 1.f, take = 0.f;
+      if (shared) {
+        float2* const other = reinterpret_cast<float2*>(smem + M::kStage + ((warp - kSoftmaxWarp) | 4u) * 4096);
+        if (t == 1) {
+          other[lane] = make_float2(m, l);
+          before_sync();
+          __syncwarp();
+          if (lane == 0) barrier_arrive(smem_address(&C.other_done));
+          fine = barrier_wait_warp(smem_address(&C.other_read), other_phase, &C.gave_up);
+        } else {
+          fine = barrier_wait_warp(smem_address(&C.other_done), other_phase, &C.gave_up);
+          after_sync();
+          const float2 o = other[lane];
+          const float top = fmaxf(m, o.x);
+          keep = m == top ? 1.f : exp2_fast((m - top) * P.scale_log2);
+          take = o.x == top ? 1.f : exp2_fast((o.x - top) * P.scale_log2);
+          m = top;
+          l = l * keep + o.y * take;
+        }
+        if (!fine) break;
+        other_phase ^= 1u;
+      }
+      if (shared ? t == 0 : t * half < piece.rows) {
         const bool any = to > from, complete = piece.begins && piece.ends;
         const uint32_t token = divide(g, P.by_group), head = piece.head * P.group + (g - token * P.group);
         const int64_t row_of = piece.token + static_cast<int64_t>(token);
@@ -718,7 +760,16 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 #pragma unroll 1
         for (int i = 0; i < DIM; i += 32) {
           uint32_t o[32];
-          if (any) {
+          if (shared) {
+            uint32_t other[32];
+            load_columns(o_at + i, o);
+            load_columns(tmem + M::output_column(1) + lanes + i, other);
+            loads_done(o);
+            loaded(other);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              o[j] = __float_as_uint(__uint_as_float(o[j]) * keep + __uint_as_float(other[j]) * take);
+          } else if (any) {
             load_columns(o_at + i, o);
             loads_done(o);
           } else {
@@ -763,6 +814,10 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           __syncwarp();
         }
         before_sync();
+        if (shared) {
+          __syncwarp();
+          if (lane == 0) barrier_arrive(smem_address(&C.other_read));
+        }
       }
       if (lane == 0) barrier_arrive(smem_address(&C.taken[at]));
     }
@@ -782,25 +837,26 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 }  // namespace paged
 
 namespace {
-template <typename T, int DIM>
+template <typename T, int DIM, bool TURNS>
 cudaError_t prepare() {
   // setmaxnreg.inc would wait for good if the launch brought fewer registers than its warps share out
   cudaFuncAttributes a;
-  const cudaError_t e = cudaFuncGetAttributes(&a, paged::many_rows_kernel<T, DIM>);
+  const cudaError_t e = cudaFuncGetAttributes(&a, paged::many_rows_kernel<T, DIM, TURNS>);
   if (e != cudaSuccess) return e;
   if (a.numRegs < static_cast<int>(paged::kLaunchRegisters)) return cudaErrorInvalidDeviceFunction;
-  return cudaFuncSetAttribute(paged::many_rows_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  return cudaFuncSetAttribute(paged::many_rows_kernel<T, DIM, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               1024 + paged::ManySmem<DIM>::kBytes);
 }
 template <typename T, int DIM>
 cudaError_t launch(const AttentionParams& p, const AttentionPlan& plan, cudaStream_t stream) {
-  return launch_dependent(paged::many_rows_kernel<T, DIM>, dim3(plan.ctas), paged::kThreadsMany,
-                          1024 + paged::ManySmem<DIM>::kBytes, p, stream);
+  return launch_dependent(plan.turns ? paged::many_rows_kernel<T, DIM, true> : paged::many_rows_kernel<T, DIM, false>,
+                          dim3(plan.ctas), paged::kThreadsMany, 1024 + paged::ManySmem<DIM>::kBytes, p, stream);
 }
 }  // namespace
 cudaError_t prepare_many_rows() {
-  for (cudaError_t e : {prepare<__half, 64>(), prepare<__half, 128>(), prepare<__nv_bfloat16, 64>(),
-                        prepare<__nv_bfloat16, 128>()})
+  for (cudaError_t e : {prepare<__half, 64, false>(), prepare<__half, 128, false>(), prepare<__nv_bfloat16, 64, false>(),
+                        prepare<__nv_bfloat16, 128, false>(), prepare<__half, 64, true>(), prepare<__half, 128, true>(),
+                        prepare<__nv_bfloat16, 64, true>(), prepare<__nv_bfloat16, 128, true>()})
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }

@@ -453,6 +453,19 @@ def test_wide_and_odd_groups(group, dim, max_new):
     p.check(*attend(p, max_new=max_new))
 
 
+@pytest.mark.parametrize("mask", [{}, dict(window=200), dict(window=3), dict(causal=False)])
+@pytest.mark.parametrize("dtype, group, dim", [(F16, 4, 64), (BF16, 4, 128), (F16, 1, 128), (BF16, 3, 96), (BF16, 5, 48)])
+def test_drafts_of_many_sequences(dtype, group, dim, mask):
+    """Row tiles that are not full, where both of a CTA take turns with the keys; and sequences beyond the hint, whose
+    rows fill one tile, or more than both."""
+    g = torch.Generator().manual_seed(dim)
+    news = torch.randint(0, 25, (48,), generator=g).tolist()
+    lens = (torch.randint(0, 1800, (48,), generator=g) + torch.tensor(news)).tolist()
+    news[7], lens[7], news[20], lens[20], news[21], lens[21], news[30], lens[30] = 128 // group, 4000, 300, 700, 33, 40, 25, 1
+    p = Problem(news, lens, 2, group, dim, 16, dtype, seed=dim)
+    p.check(*attend(p, max_new=24, **mask), **mask)
+
+
 @pytest.mark.parametrize("max_new", [1, MANY])
 @pytest.mark.parametrize("pages", [31, 32, 33, 64, 65])
 def test_caches_around_the_size_from_which_items_are_split(pages, max_new):
