@@ -12,13 +12,14 @@
 // While one row tile's softmax runs, the tensor cores work on the other's products. O stays in tensor memory. It is
 // rescaled only when a probability may be above 2^8: until then they are above 1, which costs no accuracy.
 //
-// 8192 queries x 8192 keys x 8 heads of 128: 223 us, 1230 TFLOP/s (0.76 of what a large matrix product reaches in such a
+// 8192 queries x 8192 keys x 8 heads of 128: 222 us, 1240 TFLOP/s (0.76 of what a large matrix product reaches in such a
 // short run; the tensor cores are active in 0.66 of the cycles). 32 heads of 64: 680 us, 810 TFLOP/s. What bounds it is the
 // chain of a row tile: scores, softmax of 128 of them a thread (about 1600 of some 3300 cycles a unit), product with the
 // values, next scores, which have no other place with 128-wide heads (all 512 columns are used). It does not get
 // shorter by halving the units (next scores early, but products of 64 keys read 1.5 times as much shared memory: 228), by two
 // issuing warps (279), or by handing over the probabilities in halves (238); more exponentials by polynomial: 234. 64-wide
-// heads: exponentials and the 8 warps' other instructions, 0.55 of the special-function units' rate.
+// heads: exponentials and the 8 warps' other instructions, 0.55 of the special-function units' rate. Drafts: the keys, read at
+// 5.5 to 6 TB/s; 16 of 3 to 8 tokens over 700 to 6000 keys 52 us.
 #include "paged_device.h"
 
 namespace mononn {
