@@ -442,7 +442,7 @@ struct TileLoader {
     if (wanted) {
 #pragma unroll
       for (int h = 0; h < HALVES; ++h)
-        load_box(dst + h * KEYS * 128 + ((lane << P.box_shift) * 128u), map, h * 64, r, static_cast<int32_t>(head), p, bar);
+        load_box(dst + h * KEYS * 128 + (lane << P.box_shift) * 128u, map, h * 64, r, static_cast<int32_t>(head), p, bar);
     }
     if (tile == first) look_up(first + window, next_page, next_row);
   }

@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
               if (lane == 0) {
                 const uint32_t bar = smem_address(&C.queries[t]);
                 barrier_arrive_bytes(bar, half * 128u * kHalves);
-                const uint32_t from_token = divide(walk.piece.first_row, P.by_group) + (TURNS && walk.piece.shared ? 0u : t * half_tokens);
+                const uint32_t from_token =
+                    divide(walk.piece.first_row, P.by_group) + (TURNS && walk.piece.shared ? 0u : t * half_tokens);
                 const int32_t token = walk.piece.token + static_cast<int32_t>(from_token);
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)

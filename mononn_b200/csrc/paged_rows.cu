@@ -222,13 +222,32 @@ cudaError_t prepare_rows() {
     if (e != cudaSuccess) return e;
   return cudaSuccess;
 }
-// One token a block until there are four blocks for each SM, then four tokens a block (one and four, 32 heads of 128: 100 tokens
-// 3.7 and 5.2 us, 300 4.5 and 5.3, 592 5.6 and 4.7, 4000 16.0 and 12.7; two and eight for all of 8192: 35.5 and 38.0, four 34.5).
+// One token a block until there are four blocks for each SM, then up to four tokens a block (one and four, 32 heads of 128: 100
+// tokens 3.7 and 5.2 us, 300 4.5 and 5.3, 592 5.6 and 4.7, 4000 16.0 and 12.7): as many as take the fewest turns of move_rows
+// a token, so that few threads stay idle in a last turn (8192 tokens of 40 heads, half of each turned: three tokens 32.0 us, four, in
+// two turns of which the second is a quarter full, 34.6, two 35.5; append of 32 heads of 64, no turn: 35.1, 34.4, 39.6).
 // 16-byte vectors where everything is aligned to them, otherwise single elements: 2.7 and 4.2 us for one token, 9.5 and 21.4
 // for 2048, 26 and 55 for 8192 x 40 heads (in L2).
 cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int sm_count, cudaStream_t stream) {
   RowsParams p = params;
-  p.block_tokens = p.tokens >= 4u * static_cast<unsigned>(sm_count) ? paged::kRowsTokens : 1u;
+  p.block_tokens = 1;
+  if (p.tokens >= 4u * static_cast<unsigned>(sm_count)) {
+    const uint32_t v = vectors ? 8 : 1, rest = (p.head_dim - p.rotary_dim) / v;
+    const bool two = !p.interleaved || v == 1;  // a thread turns two vectors
+    const uint32_t turned = p.interleaved && !two ? p.rotary_dim / 8 : p.rotary_dim / 2 / (p.interleaved ? 1 : v);
+    auto turns = [&](uint32_t tokens, uint32_t vectors_each, uint32_t heads, uint32_t at_once) {
+      const uint64_t each = static_cast<uint64_t>(paged::kRowsThreads) * at_once;
+      return (static_cast<uint64_t>(tokens) * heads * vectors_each + each - 1) / each;
+    };
+    auto all_turns = [&](uint32_t t) {
+      uint64_t sum = turns(t, p.head_dim / v, p.v.heads, 4);
+      for (uint32_t heads : {p.q.heads, p.k.heads}) sum += turns(t, turned, heads, two ? 2 : 4) + turns(t, rest, heads, 4);
+      return sum;
+    };
+    p.block_tokens = paged::kRowsTokens;
+    for (uint32_t t = paged::kRowsTokens - 1; t > 1; --t)  // fewer turns a token
+      if (all_turns(t) * p.block_tokens < all_turns(p.block_tokens) * t) p.block_tokens = t;
+  }
   const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens);
   auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, paged::kRowsThreads, 0, p, stream); };
   if (bf16) return vectors ? launch(paged::rows_kernel<__nv_bfloat16, 8>) : launch(paged::rows_kernel<__nv_bfloat16, 1>);
