@@ -4,7 +4,7 @@
 // a head, t = position x f_i. The angle is taken in 64 bits as a share of a full turn (position x f_i / 2 pi, of
 // which only the fraction matters), so that positions of any size keep it to 32 bits; sine and
 // cosine of that share, and the products, are 32-bit. Bound by memory: every element is read once and written once.
-// 8192 tokens x 40 heads of 128 in place (168 MB): 34 us, 4.9 TB/s; append of 11.6k tokens x 32 heads of 64 (191 MB):
+// 8192 tokens x 40 heads of 128 in place (168 MB): 32 us, 5.2 TB/s; append of 11.6k tokens x 32 heads of 64 (191 MB):
 // 34 us, 5.6 TB/s, 0.86 of what a copy reaches. One token: 3.0 us, the launch. A block takes a few tokens, so that
 // the angles and places, worked out once for all of their heads, are few beside the elements.
 #include "paged_device.h"
@@ -13,7 +13,7 @@ namespace mononn {
 namespace paged {
 
 constexpr int kRowsThreads = 256;
-constexpr uint32_t kRowsTokens = 4;  // of a block, at most
+constexpr uint32_t kRowsTokens = 8, kRowsAngles = 512;  // of a block, at most
 
 // V elements at once, of type T
 template <typename T, int V>
@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t sequence_of(const int32_t* indptr, uint32_t 
 
 // What a block knows of its tokens.
 struct RowsShared {
-  float cosines[kRowsTokens][128], sines[kRowsTokens][128];
+  alignas(16) float cosines[kRowsAngles], sines[kRowsAngles];  // token by token
   int64_t page_at[kRowsTokens];  // of the token's row in the pages, in elements; below 0: none
   int32_t position[kRowsTokens];
   bool member[kRowsTokens];      // of some sequence
@@ -113,8 +113,8 @@ __device__ __forceinline__ void move_rows(const RowsSource& s, const RowsShared&
 #pragma unroll
       for (int u = 0; u < kAtOnce; ++u) {
         if (to[u] == nullptr) continue;
-        const float* cosines = S.cosines[of[u]];
-        const float* sines = S.sines[of[u]];
+        const float* cosines = S.cosines + of[u] * (rd / 2);
+        const float* sines = S.sines + of[u] * (rd / 2);
         if constexpr (MODE == kNeighbours && V == 8) {
           float x[V], y[V];
           a[u].get(x);
@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(kRowsThreads, 6) rows_kernel(const __grid_cons
       const double turns = S.position[t] * P.turns[p];
       float s, c;
       sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
-      S.cosines[t][p] = c * P.magnitude;
-      S.sines[t][p] = s * P.magnitude;
+      S.cosines[t * pairs + p] = c * P.magnitude;
+      S.sines[t * pairs + p] = s * P.magnitude;
     }
     __syncthreads();
     if (P.interleaved) {
@@ -226,6 +226,7 @@ cudaError_t prepare_rows() {
 // tokens 3.7 and 5.2 us, 300 4.5 and 5.3, 592 5.6 and 4.7, 4000 16.0 and 12.7): as many as take the fewest turns of move_rows
 // a token, so that few threads stay idle in a last turn (8192 tokens of 40 heads, half of each turned: three tokens 32.0 us, four, in
 // two turns of which the second is a quarter full, 34.6, two 35.5; append of 32 heads of 64, no turn: 35.1, 34.4, 39.6).
+// With few heads up to eight (12 heads of the same bytes in all: 36 us instead of 46 with four).
 // 16-byte vectors where everything is aligned to them, otherwise single elements: 2.7 and 4.2 us for one token, 9.5 and 21.4
 // for 2048, 26 and 55 for 8192 x 40 heads (in L2).
 cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int sm_count, cudaStream_t stream) {
@@ -244,9 +245,12 @@ cudaError_t launch_rows(const RowsParams& params, bool bf16, bool vectors, int s
       for (uint32_t heads : {p.q.heads, p.k.heads}) sum += turns(t, turned, heads, two ? 2 : 4) + turns(t, rest, heads, 4);
       return sum;
     };
-    p.block_tokens = paged::kRowsTokens;
-    for (uint32_t t = paged::kRowsTokens - 1; t > 1; --t)  // fewer turns a token
+    p.block_tokens = 4;
+    for (uint32_t t : {3, 2})  // fewer turns a token
       if (all_turns(t) * p.block_tokens < all_turns(p.block_tokens) * t) p.block_tokens = t;
+    while (p.block_tokens >= 4 && p.block_tokens < paged::kRowsTokens && all_turns(p.block_tokens + 1) == all_turns(1) &&
+           (p.block_tokens + 1) * (p.rotary_dim / 2) <= paged::kRowsAngles)
+      ++p.block_tokens;  // as long as one turn is enough
   }
   const dim3 grid((p.tokens + p.block_tokens - 1) / p.block_tokens);
   auto launch = [&](auto kernel) { return launch_dependent(kernel, grid, paged::kRowsThreads, 0, p, stream); };

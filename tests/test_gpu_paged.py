@@ -556,7 +556,7 @@ def test_calls_on_several_streams_at_once():
     p.check(first)
 
 
-@pytest.mark.parametrize("dim, heads", [(64, 3), (128, 9), (67, 2), (80, 1), (128, 40), (128, 70)])
+@pytest.mark.parametrize("dim, heads", [(64, 3), (128, 9), (67, 2), (80, 1), (128, 12), (128, 40), (128, 70)])
 @pytest.mark.parametrize("config", [dict(rotary_dim=64), dict(rotary_dim=32, interleaved=True)])
 @pytest.mark.parametrize("tokens", [591, 592, 595, 2001])
 def test_rotary_of_many_tokens(tokens, config, dim, heads):
