@@ -61,7 +61,7 @@ struct ManyControl {
   uint64_t scores[2], scores_read[2], probabilities[2], outputs[2], queries[2], queries_free[2];  // of row tiles
   uint64_t told[kPieces], taken[kPieces], drained;
   uint64_t other_done, other_read;  // of two row tiles that hold the same rows, the second
-  alignas(16) Piece pieces[kPieces];
+  alignas(16) Piece pieces[kPieces], deferred;
   Share share;
   uint32_t sums[12];
   uint32_t gave_up, tmem;
@@ -354,8 +354,25 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
       Walker<kKeys> walk(P, C.share);
       const uint32_t half = P.item_rows / 2, half_tokens = divide(half, P.by_group);
       uint32_t query_loads[2] = {0, 0};
+      // A share that begins within an item takes that item's rest last: CTAs whose items see the same keys then go through
+      // them at about the same time, and most reads find them in L2.
+      bool deferred = false, last = false;
       for (uint32_t i = 0; fine; ++i) {
-        const bool some = walk.next();
+        bool some = walk.next();
+        if (i == 0 && some && !walk.piece.begins && walk.left != 0u) {
+          if (lane == 0) C.deferred = walk.piece;
+          __syncwarp();
+          deferred = true;
+          some = walk.next();
+        }
+        if (!some && !last) {  // behind the last piece in order
+          last = true;
+          if (lane == 0 && P.headers) walk.write_header();
+          if (deferred) {
+            walk.piece = C.deferred;
+            some = true;
+          }
+        }
         if (some) {
           loader.begin(walk.piece);
           set_ranges<TURNS>(P, walk.piece);
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
           }
         }
       }
-      if (lane == 0 && P.headers) walk.write_header();
+      if (!last && lane == 0 && P.headers) walk.write_header();  // on the way out after a wait that gave up
       for (int t = 0; t < 2; ++t)  // where all goes well they landed long ago
         if (query_loads[t]) barrier_wait_out(smem_address(&C.queries[t]), (query_loads[t] - 1u) & 1u);
     } else if (warp == kValueWarp) {
