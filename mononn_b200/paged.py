@@ -117,13 +117,33 @@ def _out_rows(name: str, out, src):
 
 
 def _same_grid(a, b) -> bool:
-    """Head slices of one projection: the same rows, other columns (never the same elements)."""
-    if a.stride() != b.stride() or a.stride(0) == 0 or a.dim() != 3:
+    """Slices of one projection (other heads of the same rows, or others of the parts that a head has there): the
+    same strides, and never the same element."""
+    if a.dim() != 3 or b.dim() != 3 or a.element_size() != b.element_size():
         return False
-    off = abs(a.data_ptr() - b.data_ptr()) // a.element_size()
-    width = max(a.shape[1], b.shape[1])
-    return a.stride(1) >= a.shape[2] and a.stride(0) >= off + (width - 1) * a.stride(1) + a.shape[2] \
-        and off >= (min(a.shape[1], b.shape[1]) - 1) * a.stride(1) + a.shape[2]
+    low, high = sorted((a, b), key=lambda t: t.data_ptr())
+    off, rest = divmod(high.data_ptr() - low.data_ptr(), a.element_size())
+    if rest:
+        return False
+    steps = [(off, 0, 0)]  # stride, and how often each of the two takes it
+    for i in range(2):
+        strides = {t.stride(i) for t in (low, high) if t.shape[i] > 1}
+        if len(strides) > 1:
+            return False
+        steps += [(n, low.shape[i], high.shape[i]) for n in strides]
+    # by growing stride, each step has to reach over all that the smaller ones span
+    below, above = low.shape[2], high.shape[2]
+    for stride, of_low, of_high in sorted(steps):
+        if of_low == 0:  # from the one to the other: from here on both are one block
+            if stride < below:
+                return False
+            below = above = stride + above
+        else:
+            if stride < max(below, above):
+                return False
+            below += (of_low - 1) * stride
+            above += (of_high - 1) * stride
+    return True
 
 
 def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):

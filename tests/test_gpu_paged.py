@@ -578,3 +578,25 @@ def test_vectors_and_single_elements_agree():
         odd.copy_(x)
         rotary(odd, pos, Rotary(**config))
         assert torch.equal(odd, rotary(x, pos, Rotary(**config), out=torch.empty_like(x)))
+
+
+@pytest.mark.parametrize("heads, kv_heads, order", [(4, 2, "qkv"), (32, 8, "qkv"), (5, 1, "kvq"), (6, 3, "kqv"), (2, 2, "qkv")])
+def test_queries_of_a_fused_projection_turned_in_place(heads, kv_heads, order):
+    """Grouped heads as slices of one projection: the queries turn in place beside the keys and values that are stored."""
+    p = Problem([1, 40, 7], [300, 130, 7], kv_heads, heads // kv_heads, 64, 16, F16, seed=heads)
+    t = p.starts[-1]
+    wide = torch.randn(t, heads + 2 * kv_heads, 64, device="cuda").to(F16)
+    parts, at = {}, 0
+    for name in order:
+        n = heads if name == "q" else kv_heads
+        parts[name] = wide[:, at:at + n]
+        at += n
+    config = Rotary(64)
+    apart = {name: x.clone() for name, x in parts.items()}
+    pages = p.k.clone(), p.v.clone()
+    want = PagedCache(*pages, p.table, p.lengths).append(apart["k"], apart["v"], p.indptr, config, q=apart["q"])
+    keep = {name: parts[name].clone() for name in "kv"}
+    assert p.cache().append(parts["k"], parts["v"], p.indptr, config, q=parts["q"]) is parts["q"]
+    assert torch.equal(parts["q"], want)
+    assert torch.equal(p.k, pages[0]) and torch.equal(p.v, pages[1])
+    assert all(torch.equal(parts[name], keep[name]) for name in "kv")

@@ -265,3 +265,54 @@ def test_queries_may_not_overlap_what_is_appended(lib_built):
     for q_out in (wide[:, 2:6], wide[:, 4:]):
         with pytest.raises(ValueError, match="overlaps"):
             cache.append_runner(k, v, indptr, q=q, q_out=q_out)
+
+
+def test_queries_in_place_beside_what_is_appended(lib_built):
+    """Slices of one projection: whether q turned in place is taken goes by the elements alone, whichever has more heads
+    and comes first. What is taken gets as far as the library call, and is refused there for want of a GPU."""
+    cache = PagedCache(*small_cache())
+    indptr = torch.zeros(3, dtype=torch.int32)
+
+    class OfHost:
+        cuda_stream = 0
+
+    def parts(wide, q, k, v):
+        return lambda: cache.append_runner(wide[:, k:k + 2], wide[:, v:v + 2], indptr, q=wide[:, q:q + 4], stream=OfHost)
+
+    wide = torch.zeros(3, 16, 64, dtype=torch.float16)
+    for q, k, v in ((0, 4, 6), (4, 0, 2), (2, 0, 6), (12, 10, 8)):
+        parts(wide, q, k, v)()
+    for q, k, v in ((0, 2, 8), (0, 8, 3), (4, 3, 0), (4, 0, 7), (4, 5, 12)):
+        with pytest.raises(ValueError, match="overlaps"):
+            parts(wide, q, k, v)()
+    heads = torch.zeros(3, 2, 3, 64, dtype=torch.float16)  # the parts of a head side by side
+    cache.append_runner(heads[:, :, 1], heads[:, :, 2], indptr, q=heads[:, :, 0], stream=OfHost)
+    cache.append_runner(heads[:, :, 0], heads[:, :, 1], indptr, q=heads[:, :, 2], stream=OfHost)
+    major = torch.zeros(2, 3, 3, 64, dtype=torch.float16).transpose(0, 1)  # heads apart, then tokens, then parts
+    cache.append_runner(major[:, :, 0], major[:, :, 2], indptr, q=major[:, :, 1], stream=OfHost)
+    with pytest.raises(ValueError, match="overlaps"):
+        cache.append_runner(heads[:, :, 0], heads[:, :, 2], indptr, q=heads[:, :, 0], stream=OfHost)
+
+
+def test_slices_that_share_an_element_are_never_taken(lib_built):
+    """Every two small slices of a buffer that the check takes for disjoint have no element in common."""
+    import itertools
+    import random
+
+    from mononn_b200.paged import _overlap, _same_grid
+    rng = random.Random(5)
+    flat = torch.zeros(400, dtype=torch.float16)
+
+    def places(t):
+        o = t.storage_offset()
+        return {o + sum(i * s for i, s in zip(at, t.stride())) for at in itertools.product(*map(range, t.shape))}
+
+    taken = 0
+    for _ in range(6000):
+        strides = rng.choice(((8, 2), (12, 4), (2, 9), (6, 3), (24, 6), (4, 2), (0, 2), (3, 3), (5, 2)))
+        tokens, dim = rng.randint(1, 3), rng.randint(1, 3)
+        a, b = (flat.as_strided((tokens, rng.randint(1, 4), dim), (*strides, 1), rng.randint(0, 30)) for _ in range(2))
+        if _same_grid(a, b) or not _overlap(a, b):
+            taken += 1
+            assert not places(a) & places(b)
+    assert taken > 500
