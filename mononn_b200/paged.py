@@ -54,9 +54,14 @@ def _dtype(t) -> int:
     return int(t.dtype == torch.bfloat16)
 
 
+def _no_gradient(name: str, t) -> None:
+    import torch
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which is not computed here: detach it or use torch.no_grad()")
+
+
 def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
     """A [tokens, heads, head_dim] tensor of the dtype, device and head_dim of `like`."""
-    import torch
     if t.dim() != 3 or t.shape[2] != like.shape[-1]:
         raise ValueError(f"{name} must be [tokens, heads, {like.shape[-1]}], not {list(t.shape)}")
     if heads is not None and t.shape[1] != heads:
@@ -65,8 +70,7 @@ def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
         raise ValueError(f"{name} must have {tokens} tokens, not {t.shape[0]}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} on {like.device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient, which is not computed here: detach it or use torch.no_grad()")
+    _no_gradient(name, t)
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name}: elements of a head must be consecutive")
     return t
@@ -200,11 +204,16 @@ class PagedCache:
     def kv_heads(self) -> int:
         return self.k_pages.shape[2]
 
+    def _pages_without_gradient(self):  # asked at each call: whether gradients are on may change behind the constructor
+        _no_gradient("k_pages", self.k_pages)
+        _no_gradient("v_pages", self.v_pages)
+
     def _indptr(self, indptr):
         return _ints("indptr", indptr, self.k_pages, (self.page_table.shape[0] + 1,))
 
     def append_runner(self, k, v, indptr, rotary: Rotary | None = None, positions=None, q=None, q_out=None, stream=None):
         """A prepared `append`."""
+        self._pages_without_gradient()
         _rows("k", k, self.k_pages, self.kv_heads)
         _rows("v", v, self.k_pages, self.kv_heads, k.shape[0])
         self._indptr(indptr)
@@ -244,8 +253,10 @@ class PagedCache:
                          workspace=None, stream=None):
         """A prepared `attention`; what it returns is in `out` (made here when none is given: `.out`)."""
         import torch
+        self._pages_without_gradient()
         _rows("q", q, self.k_pages, None)
         self._indptr(indptr)
+
         def made_here(*size, dtype):  # on the stream of the call: in use there, and seen by the one of the caller
             with torch.cuda.stream(stream):
                 t = torch.empty(*size, dtype=dtype, device=q.device)

@@ -316,3 +316,22 @@ def test_slices_that_share_an_element_are_never_taken(lib_built):
             taken += 1
             assert not places(a) & places(b)
     assert taken > 500
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_pages_that_want_gradients_are_refused(lib_built, which):
+    """A learned prefix among the keys or the values: neither reading nor writing it loses a gradient without a word."""
+    tensors = list(small_cache())
+    tensors[which].requires_grad_()
+    cache = PagedCache(*tensors)
+    new, q = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, 4, 64, dtype=torch.float16)
+    indptr = torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: cache.attention_runner(q, indptr), lambda: cache.append_runner(new, new, indptr)):
+        with pytest.raises(ValueError, match="_pages requires a gradient"):
+            call()
+
+    class OfHost:
+        cuda_stream = 0
+
+    with torch.no_grad():
+        cache.append_runner(new, new, indptr, stream=OfHost)
