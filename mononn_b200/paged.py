@@ -58,6 +58,8 @@ def _no_gradient(name: str, t) -> None:
     import torch
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which is not computed here: detach it or use torch.no_grad()")
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a forward gradient, which is not computed here")
 
 
 def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):

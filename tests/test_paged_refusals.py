@@ -335,3 +335,21 @@ def test_pages_that_want_gradients_are_refused(lib_built, which):
 
     with torch.no_grad():
         cache.append_runner(new, new, indptr, stream=OfHost)
+
+
+def test_forward_gradients_are_refused(lib_built):
+    from torch.autograd import forward_ad
+    k, v, table, lengths = small_cache()
+    new, q = torch.zeros(3, 2, 64, dtype=torch.float16), torch.zeros(3, 4, 64, dtype=torch.float16)
+    indptr, pos = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    cache = PagedCache(k, v, table, lengths)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: rotary_runner(dual(q), pos, Rotary(64)), lambda: cache.attention_runner(dual(q), indptr),
+                     lambda: cache.append_runner(dual(new), new, indptr), lambda: cache.append_runner(new, dual(new), indptr),
+                     lambda: PagedCache(dual(k), v, table, lengths).attention_runner(q, indptr),
+                     lambda: PagedCache(k, dual(v), table, lengths).append_runner(new, new, indptr)):
+            with pytest.raises(ValueError, match="forward gradient"):
+                call()
