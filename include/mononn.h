@@ -371,7 +371,7 @@ int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mono
                                      size_t* bytes);
 /* Waits for `cuda_stream`, then reports and clears the status word that the attention kernels of its
  * device share: MONONN_OK, or MONONN_ERR_BARRIER_TIMEOUT when a bounded wait expired in one of them
- * since the last report (its output is incomplete). */
+ * since the last report (its output is incomplete). A null stream is the default one of the current device. */
 int mononn_paged_attention_status(void* cuda_stream);
 
 void mononn_destroy(mononn_module* m);

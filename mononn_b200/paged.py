@@ -315,4 +315,5 @@ def paged_attention_status(stream=None) -> None:
     kernel of its device since the last call (the output of that attention is incomplete)."""
     import torch
     st = stream if stream is not None else torch.cuda.current_stream()
-    check(lib().mononn_paged_attention_status(C.c_void_p(st.cuda_stream)))
+    with torch.cuda.device(st.device):  # the handle of a default stream is null on every device
+        check(lib().mononn_paged_attention_status(C.c_void_p(st.cuda_stream)))

@@ -353,3 +353,31 @@ def test_forward_gradients_are_refused(lib_built):
                      lambda: PagedCache(k, dual(v), table, lengths).append_runner(new, new, indptr)):
             with pytest.raises(ValueError, match="forward gradient"):
                 call()
+
+
+def test_status_is_read_on_the_device_of_the_stream(lib_built, monkeypatch):
+    """Default streams have the same handle on every device: the one of the stream has to be current."""
+    import contextlib
+
+    from mononn_b200 import paged
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d
+        yield
+        current[0] = before
+
+    class Library:
+        @staticmethod
+        def mononn_paged_attention_status(handle):
+            asked.append((current[0], handle.value))
+            return 0
+
+    class DefaultStream:
+        device, cuda_stream = 1, 0
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(paged, "lib", Library)
+    paged.paged_attention_status(DefaultStream)
+    assert asked == [(1, None)] and current == [0]
