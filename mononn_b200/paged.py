@@ -92,6 +92,9 @@ def _ints(name: str, t, like, shape):
 def _stream(device, stream) -> C.c_void_p:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream(device)
+    # the handle of a default stream is null on every device, so the library cannot tell
+    if device.type == "cuda" and s.device != device:
+        raise ValueError(f"the stream belongs to {s.device}, the tensors to {device}")
     return C.c_void_p(s.cuda_stream)
 
 

@@ -381,3 +381,14 @@ def test_status_is_read_on_the_device_of_the_stream(lib_built, monkeypatch):
     monkeypatch.setattr(paged, "lib", Library)
     paged.paged_attention_status(DefaultStream)
     assert asked == [(1, None)] and current == [0]
+
+
+def test_streams_of_other_devices_are_refused(lib_built):
+    from mononn_b200 import paged
+
+    class DefaultStream:
+        device, cuda_stream = torch.device("cuda", 1), 0
+
+    with pytest.raises(ValueError, match="stream belongs to cuda:1"):
+        paged._stream(torch.device("cuda", 0), DefaultStream)
+    assert paged._stream(torch.device("cuda", 1), DefaultStream).value is None
