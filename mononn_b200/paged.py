@@ -26,13 +26,13 @@ class Rotary:
     those of mononn_rotary_config; None or 0 stands for the default)."""
     rotary_dim: int
     interleaved: bool = False
-    theta: float = 10000.0
+    theta: float | None = 10000.0
     scaling: str = "none"  # none, linear, base, ramp, bands
-    factor: float = 1.0
-    original_length: float = 0.0
-    low: float = 0.0
-    high: float = 0.0
-    magnitude: float = 0.0
+    factor: float | None = 1.0           # has no default where a scaling uses it
+    original_length: float | None = 0.0  # has none, either
+    low: float | None = 0.0
+    high: float | None = 0.0
+    magnitude: float | None = 0.0
 
     def table(self) -> capi.RotaryTable:
         """Turning rates (shares of a full turn per position) as the kernels take them."""
@@ -40,8 +40,9 @@ class Rotary:
             raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}")
         if not 0 <= self.rotary_dim < 2**32:
             raise ValueError("rotary_dim out of range")
-        c = capi.RotaryConfigArgs(self.rotary_dim, int(self.interleaved), _SCALINGS[self.scaling], self.theta,
-                                  self.factor, self.original_length, self.low, self.high, self.magnitude)
+        c = capi.RotaryConfigArgs(self.rotary_dim, int(self.interleaved), _SCALINGS[self.scaling], *(
+            0.0 if x is None else x
+            for x in (self.theta, self.factor, self.original_length, self.low, self.high, self.magnitude)))
         t = capi.RotaryTable()
         check(lib().mononn_rotary_init(C.byref(c), C.byref(t)))
         return t

@@ -392,3 +392,19 @@ def test_streams_of_other_devices_are_refused(lib_built):
     with pytest.raises(ValueError, match="stream belongs to cuda:1"):
         paged._stream(torch.device("cuda", 0), DefaultStream)
     assert paged._stream(torch.device("cuda", 1), DefaultStream).value is None
+
+
+@pytest.mark.parametrize("scaling", ["none", "linear", "base", "ramp", "bands"])
+def test_entries_that_a_configuration_leaves_open(lib_built, scaling):
+    """None stands for the default, as 0 does."""
+    given = dict(scaling=scaling, factor=4.0, original_length=4096.0)
+    want = Rotary(64, **given).table()
+    got = Rotary(64, **given, theta=None, low=None, high=None, magnitude=None).table()
+    assert bytes(got) == bytes(want)
+    assert bytes(Rotary(64, factor=None, original_length=None).table()) == bytes(Rotary(64).table())
+    if scaling != "none":
+        with pytest.raises(capi.MononnError, match="factor"):
+            Rotary(64, **{**given, "factor": None}).table()
+    if scaling in ("ramp", "bands"):
+        with pytest.raises(capi.MononnError, match="original_length"):
+            Rotary(64, **{**given, "original_length": None}).table()
