@@ -185,6 +185,9 @@ class PagedCache:
                       [pages, kv_heads, page_size, head_dim])
     page_table        int32 [sequences, most pages of a sequence]
     lengths           int32 [sequences]: tokens of each sequence, the new ones of a call among them
+
+    What these hold may change from call to call, the tensors themselves may not: a step writes
+    `cache.lengths.add_(1)` or copies into them.
     """
 
     def __init__(self, k_pages, v_pages, page_table, lengths):
@@ -199,12 +202,18 @@ class PagedCache:
         n, most = page_table.shape
         _ints("page_table", page_table, k_pages, (n, most))
         _ints("lengths", lengths, k_pages, (n,))
-        self.k_pages, self.v_pages, self.page_table, self.lengths = k_pages, v_pages, page_table, lengths
+        self._tensors = k_pages, v_pages, page_table, lengths
         pages, size, heads, dim = k_pages.shape
         ps, ts, hs, _ = k_pages.stride()
         self._args = capi.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, hs, page_table.data_ptr(),
                                          page_table.stride(0) if n > 1 else most, lengths.data_ptr(), n, most, pages,
                                          size, heads, dim, _dtype(k_pages))
+
+    # Read only: the addresses are taken once, so another tensor would not be seen. New contents are copied into these.
+    k_pages = property(lambda self: self._tensors[0])
+    v_pages = property(lambda self: self._tensors[1])
+    page_table = property(lambda self: self._tensors[2])
+    lengths = property(lambda self: self._tensors[3])
 
     @property
     def kv_heads(self) -> int:

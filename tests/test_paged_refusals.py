@@ -408,3 +408,15 @@ def test_entries_that_a_configuration_leaves_open(lib_built, scaling):
     if scaling in ("ramp", "bands"):
         with pytest.raises(capi.MononnError, match="original_length"):
             Rotary(64, **{**given, "original_length": None}).table()
+
+
+@pytest.mark.parametrize("name", ["k_pages", "v_pages", "page_table", "lengths"])
+def test_tensors_of_a_cache_are_not_replaced(lib_built, name):
+    """Calls would go on with the address of the old one, which may be somebody else's memory by then."""
+    tensors = small_cache()
+    cache = PagedCache(*tensors)
+    before = bytes(cache._args)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, getattr(cache, name) + 1)
+    cache.lengths.add_(1)
+    assert bytes(cache._args) == before and cache.lengths is tensors[3] and cache.lengths.tolist() == [1, 1]
