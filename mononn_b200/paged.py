@@ -286,8 +286,8 @@ class PagedCache:
             if lse.dtype != torch.float32 or lse.device != q.device or tuple(lse.shape) != tuple(q.shape[:2]) \
                     or not lse.is_contiguous():
                 raise ValueError(f"lse must be contiguous float32 {list(q.shape[:2])} on {q.device}")
-        if scale is not None and not scale > 0:
-            raise ValueError("scale must be positive")
+        if scale is not None and not C.c_float(scale).value > 0:  # 0 in 32 bits would stand for the default
+            raise ValueError("scale must be positive, in 32 bits too")
         if not 0 <= window < 2**32 or not 0 <= max_new < 2**32:
             raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
         for name, t in (("q", q), ("lse", lse), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):

@@ -420,3 +420,12 @@ def test_tensors_of_a_cache_are_not_replaced(lib_built, name):
         setattr(cache, name, getattr(cache, name) + 1)
     cache.lengths.add_(1)
     assert bytes(cache._args) == before and cache.lengths is tensors[3] and cache.lengths.tolist() == [1, 1]
+
+
+def test_scales_that_vanish_in_32_bits_are_refused(lib_built):
+    """They would become 0, which stands for 1 / sqrt(head_dim)."""
+    cache = PagedCache(*small_cache())
+    q, indptr = torch.zeros(3, 4, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+    for scale in (1e-46, 0.0, -1.0, math.nan):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            cache.attention_runner(q, indptr, scale=scale)
