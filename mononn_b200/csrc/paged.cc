@@ -3,6 +3,7 @@
 #include "paged.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -148,9 +149,11 @@ int check_dtype(int dtype) {
 int check_rotary(const mononn_rotary& r, unsigned head_dim) {
   if (r.rotary_dim == 0 || (r.rotary_dim & 1u) || r.rotary_dim > 2 * MONONN_MAX_ROTARY_PAIRS || r.rotary_dim > head_dim)
     return invalid("rotary_dim must be even, at least 2 and at most head_dim");
-  if (!std::isfinite(r.magnitude)) return invalid("rotary magnitude must be finite");
+  // the kernel takes the magnitude in 32 bits, and the angle of the farthest position in 64
+  if (!(std::fabs(r.magnitude) <= FLT_MAX)) return invalid("rotary magnitude must be finite in 32 bits");
   for (unsigned i = 0; i < r.rotary_dim / 2; ++i)
-    if (!std::isfinite(r.turns[i])) return invalid("rotary rates must be finite");
+    if (!std::isfinite(r.turns[i] * 2147483648.0))
+      return invalid("rotary rates must be finite, and so the angles of all 32-bit positions");
   return MONONN_OK;
 }
 int check_cache(const mononn_paged_cache& c) {
@@ -356,6 +359,7 @@ int mononn_rotary_init(const mononn_rotary_config* config, mononn_rotary* out) {
     if (c.scaling == MONONN_ROTARY_BANDS) blend(1.0 - clamp((c.original_length * f / two_pi - low) / (high - low)));
     made.turns[i] = f / two_pi;
   }
+  if (int rc = check_rotary(made, r)) return rc;
   *out = made;
   return MONONN_OK;
 }

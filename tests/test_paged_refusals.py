@@ -429,3 +429,24 @@ def test_scales_that_vanish_in_32_bits_are_refused(lib_built):
     for scale in (1e-46, 0.0, -1.0, math.nan):
         with pytest.raises(ValueError, match="scale must be positive"):
             cache.attention_runner(q, indptr, scale=scale)
+
+
+def test_rotations_that_leave_the_kernels_numbers_are_refused(lib_built):
+    """A magnitude that is infinite in 32 bits, rates whose angle at a far position is infinite: NaN would come out."""
+    lib = capi.lib()
+    for change in (dict(magnitude=1e39), dict(magnitude=-1e300), dict(turns=1e300), dict(turns=-math.inf), dict(turns=math.nan)):
+        table = Rotary(64).table()
+        if "turns" in change:
+            table.turns[31] = change["turns"]
+        else:
+            table.magnitude = change["magnitude"]
+        assert lib.mononn_rotary_apply(C.byref(table), C.byref(rotary_args()), None) == -1
+        assert b"rotary" in lib.mononn_last_error()
+        assert append(table=table) == -1
+        assert b"rotary" in lib.mononn_last_error()
+    for change in (dict(magnitude=1e39), dict(scaling="linear", factor=1e-305),
+                   dict(scaling="bands", factor=1e-305, original_length=10.0)):
+        with pytest.raises(capi.MononnError, match="rotary"):
+            Rotary(64, **change).table()
+    table = Rotary(64, magnitude=1e38, scaling="linear", factor=1e-30).table()
+    assert append(table=table) in PASSES
