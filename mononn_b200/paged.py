@@ -63,6 +63,12 @@ def _no_gradient(name: str, t) -> None:
         raise ValueError(f"{name} carries a forward gradient, which is not computed here")
 
 
+def _sizes(name: str, t) -> None:
+    """The library counts in 32 bits; ctypes would drop the higher ones."""
+    if max(t.shape) >= 2**32:
+        raise ValueError(f"{name} has a size of 2^32 or more: {list(t.shape)}")
+
+
 def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
     """A [tokens, heads, head_dim] tensor of the dtype, device and head_dim of `like`."""
     if t.dim() != 3 or t.shape[2] != like.shape[-1]:
@@ -74,6 +80,7 @@ def _rows(name: str, t, like, heads: int | None, tokens: int | None = None):
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must be {like.dtype} on {like.device}")
     _no_gradient(name, t)
+    _sizes(name, t)
     if t.shape[2] > 1 and t.stride(2) != 1:
         raise ValueError(f"{name}: elements of a head must be consecutive")
     return t
@@ -199,6 +206,8 @@ class PagedCache:
             raise ValueError("k_pages: elements of a head must be consecutive")
         if page_table.dim() != 2:
             raise ValueError("page_table must be [sequences, pages]")
+        _sizes("k_pages", k_pages)
+        _sizes("page_table", page_table)
         n, most = page_table.shape
         _ints("page_table", page_table, k_pages, (n, most))
         _ints("lengths", lengths, k_pages, (n,))

@@ -450,3 +450,18 @@ def test_rotations_that_leave_the_kernels_numbers_are_refused(lib_built):
             Rotary(64, **change).table()
     table = Rotary(64, magnitude=1e38, scaling="linear", factor=1e-30).table()
     assert append(table=table) in PASSES
+
+
+def test_sizes_beyond_32_bits_are_refused(lib_built):
+    """2^32 tokens would be counted as none, 2^32 + 3 pages as three."""
+    cache = PagedCache(*small_cache())
+    k, v, table, lengths = small_cache()
+    many = torch.zeros(1, 2, 64, dtype=torch.float16).expand(2 ** 32, 2, 64)
+    wide = torch.zeros(3, 1, 64, dtype=torch.float16).expand(3, 2 ** 32 + 1, 64)
+    indptr, pos = torch.zeros(3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: cache.append_runner(many, many, indptr), lambda: cache.attention_runner(wide, indptr, out=wide),
+                 lambda: rotary_runner(wide, pos, Rotary(64)),
+                 lambda: PagedCache(*[t[:1].expand(2 ** 32 + 3, 16, 2, 64) for t in (k, v)], table, lengths),
+                 lambda: PagedCache(k, v, table[:, :1].expand(2, 2 ** 32), lengths)):
+        with pytest.raises(ValueError, match="2\\^32 or more"):
+            call()
