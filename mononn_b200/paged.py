@@ -4,9 +4,9 @@ include/mononn.h; the reference has no counterpart (its decoder graphs end with 
 
 Each operator comes as a function, and as a runner (`rotary_runner`, `PagedCache.append_runner`,
 `PagedCache.attention_runner`): the arguments are checked and their addresses and sizes taken once, and
-the returned zero-argument callable does nothing but the library call, for serving loops that reuse
-their buffers (what page tables, lengths, indptr and positions hold is read on the device at each
-call).  A runner keeps its tensors alive; its stream is the one given, or torch's current stream of
+the returned zero-argument callable does nothing but the library call (and tells autograd what was
+written), for serving loops that reuse their buffers (what page tables, lengths, indptr and positions
+hold is read on the device at each call).  A runner keeps its tensors alive; its stream is the one given, or torch's current stream of
 the tensors' device when it was made.
 """
 from __future__ import annotations
@@ -106,11 +106,14 @@ def _stream(device, stream) -> C.c_void_p:
     return C.c_void_p(s.cuda_stream)
 
 
-def _runner(fn, args, keep):
+def _runner(fn, args, keep, written):
+    from torch.autograd.graph import increment_version
+
     def run(_keep=keep):
         rc = fn(*args)
         if rc:
             check(rc)
+        increment_version(written)  # a graph that saved one of them says so, as behind torch's own writes
     return run
 
 
@@ -174,7 +177,7 @@ def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):
                         positions.data_ptr(), x.shape[0], x.shape[1], x.shape[2], _dtype(x))
     table = rotary.table()
     args = (C.byref(table), C.byref(a), _stream(x.device, stream))
-    return _runner(lib().mononn_rotary_apply, args, (x, out, positions, table, a))
+    return _runner(lib().mononn_rotary_apply, args, (x, out, positions, table, a), (out,))
 
 
 def rotary(x, positions, rotary: Rotary, out=None, stream=None):
@@ -262,7 +265,8 @@ class PagedCache:
         table = rotary.table() if rotary is not None else None
         args = (C.byref(self._args), C.byref(table) if table is not None else None, C.byref(a),
                 _stream(k.device, stream))
-        return _runner(lib().mononn_paged_append, args, (self, k, v, q, q_out, indptr, positions, table, a))
+        return _runner(lib().mononn_paged_append, args, (self, k, v, q, q_out, indptr, positions, table, a),
+                       (self.k_pages, self.v_pages) + ((q_out,) if q is not None else ()))
 
     def append(self, k, v, indptr, rotary: Rotary | None = None, positions=None, q=None, q_out=None, stream=None):
         """Writes the new tokens' keys and values [tokens, kv_heads, head_dim] to their places, the last
@@ -315,7 +319,8 @@ class PagedCache:
                 raise ValueError(f"workspace must be contiguous on {q.device}")
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
-        run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a))
+        run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a),
+                      (out,) + ((lse,) if lse is not None else ()))
         run.out = out
         return run
 

@@ -465,3 +465,33 @@ def test_sizes_beyond_32_bits_are_refused(lib_built):
                  lambda: PagedCache(k, v, table[:, :1].expand(2, 2 ** 32), lengths)):
         with pytest.raises(ValueError, match="2\\^32 or more"):
             call()
+
+
+def test_autograd_is_told_what_is_written(lib_built):
+    """A graph that saved a tensor does not go on with what a call wrote over it. Without tokens a call needs no GPU."""
+    class OfHost:
+        cuda_stream = 0
+
+    cache = PagedCache(*small_cache())
+    indptr, none = torch.zeros(3, dtype=torch.int32), torch.zeros(0, dtype=torch.int32)
+
+    def rows(heads=2):
+        return torch.zeros(0, heads, 64, dtype=torch.float16)
+
+    x, y, q, q2, out, lse = rows(), rows(), rows(4), rows(4), rows(4), torch.zeros(0, 4)
+    k, v = rows(), rows()
+    for written, kept, call in (
+            ((x,), (), lambda: rotary_runner(x, none, Rotary(64), stream=OfHost)()),
+            ((y,), (x,), lambda: rotary_runner(x, none, Rotary(64), out=y, stream=OfHost)()),
+            ((cache.k_pages, cache.v_pages, q), (k, v), lambda: cache.append(k, v, indptr, q=q, stream=OfHost)),
+            ((q2,), (q,), lambda: cache.append(k, v, indptr, q=q, q_out=q2, stream=OfHost)),
+            ((out, lse), (q, cache.k_pages), lambda: cache.attention_runner(q, indptr, out=out, lse=lse, stream=OfHost)())):
+        weight = torch.ones(1, dtype=torch.float16, requires_grad=True)
+        saved = [(weight * t).sum() for t in written]
+        fine = [(weight * t).sum() for t in kept]
+        call()
+        for s in saved:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                s.backward()
+        for s in fine:
+            s.backward()
