@@ -237,6 +237,7 @@ int mononn_attention_noalloc_status(void* cuda_stream);
  * and may be captured into a CUDA graph; pointers and sizes are those of the call, what indptr,
  * lengths, page_table and positions hold is read on the device at each launch. Every call runs on the device that owns
  * its first buffer (a stream of another device is refused) and restores the caller's current device.
+ * What a call writes may not overlap what it reads or writes otherwise, but for what an entry point allows.
  * dtype: MONONN_F16 or MONONN_BF16 for every tensor of a call; sums, softmax and rotations are
  * computed in 32 bits (angles in 64). Strides count elements. */
 enum { MONONN_F16 = 0, MONONN_BF16 = 1 };

@@ -117,14 +117,29 @@ def _runner(fn, args, keep, written):
     return run
 
 
+def _span(t):
+    """Addresses from the first element to behind the last; None without elements."""
+    if t.numel() == 0:
+        return None
+    n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
 def _overlap(a, b) -> bool:
-    def span(t):
-        n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    a, b = _span(a), _span(b)
+    return a is not None and b is not None and a[0] < b[1] and b[0] < a[1]
+
+
+def _apart(written: dict, read: dict) -> None:
+    """Nothing that a call writes is read by it, or written twice."""
+    spans = [(name, _span(t)) for name, t in (*written.items(), *read.items()) if t is not None]
+    spans = [(name, s) for name, s in spans if s is not None]
+    for i, (name, a) in enumerate(spans):
+        if name not in written:
+            break
+        for other, b in spans[i + 1:]:
+            if a[0] < b[1] and b[0] < a[1]:
+                raise ValueError(f"{name} overlaps {other}")
 
 
 def _out_rows(name: str, out, src):
@@ -173,6 +188,7 @@ def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):
     _rows("out", out, x, x.shape[1], x.shape[0])
     _out_rows("out", out, x)
     _ints("positions", positions, x, (x.shape[0],))
+    _apart(dict(out=out), dict(positions=positions))
     a = capi.RotaryArgs(x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1),
                         positions.data_ptr(), x.shape[0], x.shape[1], x.shape[2], _dtype(x))
     table = rotary.table()
@@ -256,6 +272,10 @@ class PagedCache:
             for name, t in (("k", k), ("v", v)):
                 if _overlap(q_out, t) and not _same_grid(q_out, t):
                     raise ValueError(f"q_out overlaps {name}")
+        tables = dict(page_table=self.page_table, lengths=self.lengths, indptr=indptr, positions=positions)
+        _apart(dict(q_out=q_out), dict(k_pages=self.k_pages, v_pages=self.v_pages, **tables))
+        for name, pages in (("k_pages", self.k_pages), ("v_pages", self.v_pages)):
+            _apart({name: pages}, dict(k=k, v=v, q=q, **tables))
         qs, os = (q.stride(), q_out.stride()) if q is not None else ((0, 0), (0, 0))
         a = capi.PagedAppendArgs(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                  q.data_ptr() if q is not None else None,
@@ -303,9 +323,11 @@ class PagedCache:
             raise ValueError("scale must be positive, in 32 bits too")
         if not 0 <= window < 2**32 or not 0 <= max_new < 2**32:
             raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
-        for name, t in (("q", q), ("lse", lse), ("k_pages", self.k_pages), ("v_pages", self.v_pages)):
-            if t is not None and _overlap(out, t) and not (name == "q" and _same_grid(out, q)):
-                raise ValueError(f"out overlaps {name}")
+        if _overlap(out, q) and not _same_grid(out, q):
+            raise ValueError("out overlaps q")
+        read = dict(k_pages=self.k_pages, v_pages=self.v_pages, page_table=self.page_table, lengths=self.lengths, indptr=indptr)
+        _apart(dict(out=out, lse=lse), read)
+        _apart(dict(lse=lse), dict(q=q))
         a = capi.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
                                     q.stride(0), q.stride(1), out.stride(0), out.stride(1), indptr.data_ptr(),
                                     q.shape[0], q.shape[1], 0.0 if scale is None else scale, int(causal), window,
@@ -317,6 +339,7 @@ class PagedCache:
                 workspace = made_here(need.value, dtype=torch.uint8)
             if workspace.device != q.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous on {q.device}")
+            _apart(dict(workspace=workspace), dict(q=q, out=out, lse=lse, **read))
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
         run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a),

@@ -600,3 +600,13 @@ def test_queries_of_a_fused_projection_turned_in_place(heads, kv_heads, order):
     assert torch.equal(parts["q"], want)
     assert torch.equal(p.k, pages[0]) and torch.equal(p.v, pages[1])
     assert all(torch.equal(parts[name], keep[name]) for name in "kv")
+
+
+def test_workspaces_that_overlap_are_refused():
+    p = Problem([1], [5000], 1, 1, 64, 16, F16)
+    need = p.cache().attention_runner(p.q, p.indptr)
+    room = torch.empty(1 << 23, dtype=torch.uint8, device="cuda")
+    out = room[4096:4096 + 128].view(F16).view(1, 1, 64)
+    with pytest.raises(ValueError, match="workspace overlaps out"):
+        p.cache().attention_runner(p.q, p.indptr, out=out, workspace=room)
+    assert torch.equal(p.cache().attention(p.q, p.indptr, workspace=room), (need(), need.out)[1])

@@ -495,3 +495,53 @@ def test_autograd_is_told_what_is_written(lib_built):
                 s.backward()
         for s in fine:
             s.backward()
+
+
+def test_what_is_written_may_not_be_read(lib_built):
+    """Tensors of any kind that a call writes and reads at one address, or writes twice."""
+    halves = torch.zeros(1 << 16, dtype=torch.float16)
+
+    def at(offset, *shape, dtype=torch.float16):
+        return halves[offset:].view(dtype).flatten()[:math.prod(shape)].view(*shape)
+
+    def cache(k=0, v=8192, table=16384, lengths=16512):
+        return PagedCache(at(k, 4, 16, 2, 64), at(v, 4, 16, 2, 64), at(table, 2, 3, dtype=torch.int32),
+                          at(lengths, 2, dtype=torch.int32))
+
+    indptr, pos = at(16640, 3, dtype=torch.int32), at(16768, 3, dtype=torch.int32)
+    free = 20480
+
+    class OfHost:
+        cuda_stream = 0
+
+    def append(c, q_out=None, **kw):
+        q = at(free + 2048, 3, 4, 64)
+        given = dict(k=at(free, 3, 2, 64), v=at(free + 1024, 3, 2, 64), indptr=indptr, positions=pos, q=q, stream=OfHost)
+        given.update(kw)
+        return c.append_runner(q_out=q if q_out is None else q_out, **given)
+
+    append(cache())
+    for call, names in ((lambda: append(cache(), q_out=at(4096, 3, 4, 64)), "q_out overlaps k_pages"),
+                        (lambda: append(cache(), q_out=at(12288, 3, 4, 64)), "q_out overlaps v_pages"),
+                        (lambda: append(cache(), q_out=at(16640 - 64, 3, 4, 64)), "q_out overlaps indptr"),
+                        (lambda: append(cache(), q_out=at(16768, 3, 4, 64)), "q_out overlaps positions"),
+                        (lambda: append(cache(), k=at(64, 3, 2, 64)), "k_pages overlaps k"),
+                        (lambda: append(cache(), v=at(8192, 3, 2, 64)), "v_pages overlaps v"),
+                        (lambda: append(cache(table=128)), "k_pages overlaps page_table"),
+                        (lambda: append(cache(lengths=8192 + 128)), "v_pages overlaps lengths"),
+                        (lambda: rotary_runner(at(16768 - 128, 3, 2, 64), pos, Rotary(64)), "out overlaps positions")):
+        with pytest.raises(ValueError, match=names):
+            call()
+
+    def attend(c, out, lse):
+        return c.attention_runner(at(free, 3, 4, 64), indptr, out=out, lse=lse)
+
+    out, lse = at(free + 1024, 3, 4, 64), at(free + 2048, 3, 4, dtype=torch.float32)
+    for call, names in ((lambda: attend(cache(), at(16384, 3, 4, 64), lse), "out overlaps page_table"),
+                        (lambda: attend(cache(), at(16512, 3, 4, 64), lse), "out overlaps lengths"),
+                        (lambda: attend(cache(), out, at(free + 1024, 3, 4, dtype=torch.float32)), "out overlaps lse"),
+                        (lambda: attend(cache(), out, at(free, 3, 4, dtype=torch.float32)), "lse overlaps q"),
+                        (lambda: attend(cache(), out, at(0, 3, 4, dtype=torch.float32)), "lse overlaps k_pages"),
+                        (lambda: attend(cache(), out, at(16640, 3, 4, dtype=torch.float32)), "lse overlaps indptr")):
+        with pytest.raises(ValueError, match=names):
+            call()
