@@ -128,7 +128,7 @@ bool stride_in_range(int64_t s) { return s >= 0 && s < (1ll << 39); }
 // dimension has to reach over all that the smaller ones span.
 using Dimension = std::pair<uint32_t, int64_t>;  // size, stride
 bool apart(uint32_t head_dim, std::initializer_list<Dimension> dims) {
-  Dimension sorted[3];
+  Dimension sorted[3];  // as many as any caller has
   size_t n = 0;
   for (const Dimension& d : dims)
     if (d.first > 1) sorted[n++] = d;
@@ -416,7 +416,11 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
   if (!aligned(a.k, 2) || !aligned(a.v, 2) || !aligned(a.q, 2) || !aligned(a.q_out, 2) || !aligned(a.indptr, 4) ||
       !aligned(a.positions, 4))
     return invalid("append: misaligned pointer");
-  if (c.k_pages == c.v_pages) return invalid("append: keys and values go to the same pages");
+  const uintptr_t k_at = reinterpret_cast<uintptr_t>(c.k_pages), v_at = reinterpret_cast<uintptr_t>(c.v_pages);
+  const uint64_t between = (k_at < v_at ? v_at - k_at : k_at - v_at) / 2;
+  if (between > INT64_MAX / 2 || !apart(c.head_dim, {{c.page_size, c.token_stride}, {c.kv_heads, c.head_stride},
+                                                     {2, static_cast<int64_t>(between)}}))
+    return invalid("append: keys and values of a page go to the same places");
   if (!apart(c.head_dim, {{c.page_size, c.token_stride}, {c.kv_heads, c.head_stride}, {c.num_pages, c.page_stride}}))
     return invalid("append: strides put elements of pages into one place");
   if (a.q && !apart(c.head_dim, {{a.tokens, a.q_out_token_stride}, {a.q_heads, a.q_out_head_stride}}))

@@ -545,3 +545,16 @@ def test_what_is_written_may_not_be_read(lib_built):
                         (lambda: attend(cache(), out, at(16640, 3, 4, dtype=torch.float32)), "lse overlaps indptr")):
         with pytest.raises(ValueError, match=names):
             call()
+
+
+def test_keys_and_values_of_a_page_share_no_place(lib_built):
+    for off in (0, 2, 64, 128, 16 * 128 - 2):  # bytes; a page has 16 tokens x 2 heads x 64 elements
+        for change in (dict(v_pages=FAKE + off), dict(k_pages=FAKE + off, v_pages=FAKE)):
+            assert append(cache=cache_args(**change)) == -1
+            assert b"same places" in capi.lib().mononn_last_error()
+    page = 16 * 2 * 64
+    assert append(cache=cache_args(v_pages=FAKE + 2 * page, page_stride=2 * page)) in PASSES
+    assert append(cache=cache_args(v_pages=FAKE + 2 * 64, head_stride=128, token_stride=256, page_stride=2 * page)) in PASSES
+    assert append(cache=cache_args(v_pages=FAKE + 2 * 128, token_stride=256, page_stride=2 * page)) in PASSES
+    assert append(cache=cache_args(v_pages=FAKE + 2 * 64, token_stride=256, page_stride=2 * page)) == -1
+    assert append(cache=cache_args(v_pages=FAKE + 2 * page, num_pages=4, page_stride=page)) in PASSES  # of other pages
