@@ -844,7 +844,7 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
   before_sync();
   __syncthreads();
   after_sync();
-  if (C.gave_up && warp == kKeyWarp) {
+  if (C.gave_up && (warp == kKeyWarp || warp == kValueWarp)) {  // each its own fills: either may be ahead of the other
     for (uint32_t f = fills > kPairs ? fills - kPairs : 0u; f < fills; ++f)
       barrier_wait_out(smem_address(&C.full[f % kPairs]), (f / kPairs) & 1u);
     if (lane == 0) atomicExch(P.status, 1u);
