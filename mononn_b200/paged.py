@@ -168,7 +168,7 @@ def _same_grid(a, b) -> bool:
         steps += [(n, low.shape[i], high.shape[i]) for n in strides]
     # by growing stride, each step has to reach over all that the smaller ones span
     below, above = low.shape[2], high.shape[2]
-    for stride, of_low, of_high in sorted(steps):
+    for stride, of_low, of_high in sorted(steps, key=lambda s: (s[0], s[1] == 0)):
         if of_low == 0:  # from the one to the other: from here on both are one block
             if stride < below:
                 return False

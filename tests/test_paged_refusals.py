@@ -558,3 +558,19 @@ def test_keys_and_values_of_a_page_share_no_place(lib_built):
     assert append(cache=cache_args(v_pages=FAKE + 2 * 128, token_stride=256, page_stride=2 * page)) in PASSES
     assert append(cache=cache_args(v_pages=FAKE + 2 * 64, token_stride=256, page_stride=2 * page)) == -1
     assert append(cache=cache_args(v_pages=FAKE + 2 * page, num_pages=4, page_stride=page)) in PASSES  # of other pages
+
+
+def test_queries_in_place_behind_a_single_head(lib_built):
+    """A key or value head directly before the queries is as far away as their heads are from one another."""
+    k, v, table, lengths = (t[:, :, :1] if t.dim() == 4 else t for t in small_cache())
+    cache = PagedCache(k, v, table, lengths)
+    wide, indptr = torch.zeros(3, 7, 64, dtype=torch.float16), torch.zeros(3, dtype=torch.int32)
+
+    class OfHost:
+        cuda_stream = 0
+
+    for key, value, q in ((0, 1, 2), (1, 0, 2), (5, 6, 0), (0, 6, 1)):
+        cache.append_runner(wide[:, key:key + 1], wide[:, value:value + 1], indptr, q=wide[:, q:q + 5], stream=OfHost)
+    for key, value, q in ((2, 1, 2), (0, 4, 2), (6, 0, 2)):
+        with pytest.raises(ValueError, match="overlaps"):
+            cache.append_runner(wide[:, key:key + 1], wide[:, value:value + 1], indptr, q=wide[:, q:q + 5], stream=OfHost)
