@@ -375,6 +375,13 @@ int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mono
  * device share: MONONN_OK, or MONONN_ERR_BARRIER_TIMEOUT when a bounded wait expired in one of them
  * since the last report (its output is incomplete). A null stream is the default one of the current device. */
 int mononn_paged_attention_status(void* cuda_stream);
+/* Test aid, as mononn_debug_skew_barrier: this thread's next mononn_paged_attention waits for one arrival that
+ * nobody makes on the given barriers of its kernel, so that a bounded wait there runs out; its output is
+ * incomplete, and mononn_paged_attention_status reports it. 1: keys or values landed, 2: their slot free, 3: a
+ * piece of work told, 4: taken, 5: queries landed; kernel for few rows 6: its warps' meeting; kernel for many rows 7:
+ * scores made, 8: read (64-wide heads), 9: probabilities made, 10: outputs made, 11: queries used, 12 and 13: the second of two
+ * row tiles that take turns done, and read. 0: none. A call that has no wait on the barrier is an ordinary one. */
+int mononn_debug_paged_skew(unsigned barrier);
 
 void mononn_destroy(mononn_module* m);
 const char* mononn_strerror(int code);

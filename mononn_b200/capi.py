@@ -20,7 +20,7 @@ EXPORTS = [
     "mononn_trace_stages", "mononn_plan_json", "mononn_describe", "mononn_free_string", "mononn_launch_stages", "mononn_debug_skew_barrier", "mononn_attention_noalloc",
     "mononn_infer_host", "mononn_debug_mma_issue", "mononn_attention_noalloc_status",
     "mononn_rotary_init", "mononn_rotary_apply", "mononn_paged_append", "mononn_paged_attention",
-    "mononn_paged_attention_workspace", "mononn_paged_attention_status",
+    "mononn_paged_attention_workspace", "mononn_paged_attention_status", "mononn_debug_paged_skew",
 ]
 
 
@@ -129,6 +129,7 @@ def lib() -> C.CDLL:
         l.mononn_paged_attention_workspace.argtypes = [C.POINTER(PagedCacheArgs), C.POINTER(PagedAttentionArgs),
                                                        C.POINTER(C.c_size_t)]
         l.mononn_paged_attention_status.argtypes = [vp]
+        l.mononn_debug_paged_skew.argtypes = [C.c_uint]
         dp = C.POINTER(C.c_double)
         l.mononn_debug_mma_issue.argtypes = [C.c_int, C.c_uint, C.c_uint, C.c_uint, C.c_uint, C.c_uint, dp, dp, dp]
         l.mononn_destroy.argtypes = [vp]

@@ -59,6 +59,7 @@ struct Device {
 Device g_devices[kMaxDevices];
 std::mutex g_mutex;
 EncodeTiledFn g_encode = nullptr;
+thread_local uint32_t t_skewed = kBarrierNone;  // of this thread's next attention call
 
 // One-time set-up of the current device.
 int set_up(int dev, const Device** out) {
@@ -471,6 +472,7 @@ int mononn_paged_attention_workspace(const mononn_paged_cache* cache, const mono
 
 int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_attention_args* args,
                            void* cuda_stream) {
+  const uint32_t skewed = std::exchange(t_skewed, kBarrierNone);
   if (!cache || !args) return invalid("null argument");
   if (args->tokens == 0 || cache->sequences == 0) return MONONN_OK;
   if (int rc = check_attention(cache, args)) return rc;
@@ -524,6 +526,7 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   p.by_item_rows = make_divisor(p.item_rows);
   p.by_page_size = make_divisor(c.page_size);
   p.whole_items = !plan.joins;
+  p.skewed = skewed;
   p.least_shift = plan.joins && plan.least_units == 2 ? 1 : 0;
   p.scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt(static_cast<float>(c.head_dim));
   p.scale_log2 = p.scale * 1.4426950408889634f;
@@ -531,6 +534,12 @@ int mononn_paged_attention(const mononn_paged_cache* cache, const mononn_paged_a
   const bool bf16 = c.dtype == MONONN_BF16;
   if (int rc = launched(plan.many ? launch_many_rows(p, plan, bf16, stream) : launch_few_rows(p, plan, bf16, stream))) return rc;
   return plan.joins ? launched(launch_join(p, plan, bf16, stream)) : MONONN_OK;
+}
+
+int mononn_debug_paged_skew(unsigned barrier) {
+  if (barrier >= kBarriers) return invalid("no such barrier");
+  t_skewed = barrier;
+  return MONONN_OK;
 }
 
 int mononn_paged_attention_status(void* cuda_stream) {

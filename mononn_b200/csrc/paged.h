@@ -56,6 +56,14 @@ constexpr uint32_t kFewRows = 16;
 constexpr uint32_t few_keys(uint32_t padded_dim) { return 8192 / padded_dim; }
 constexpr uint32_t kTileRows = 128, kManyRows = 2 * kTileRows, kManyKeys = 128;
 
+// Barriers of the attention kernels. A launch can be told to wait for one arrival more than there will be on one of them:
+// how the tests let a bounded wait run out.
+enum AttentionBarrier : uint32_t {
+  kBarrierNone, kBarrierFull, kBarrierEmpty, kBarrierTold, kBarrierTaken, kBarrierQueries,
+  kBarrierMeeting,                                                       // few rows only
+  kBarrierScores, kBarrierScoresRead, kBarrierProbabilities, kBarrierOutputs, kBarrierQueriesFree,  // many rows only
+  kBarrierOtherDone, kBarrierOtherRead, kBarriers
+};
 struct AttentionHeader {  // one per CTA: the item that begins in it and goes on in the next `more` CTAs
   uint32_t more;          // 0: none
   uint32_t rows;
@@ -78,6 +86,7 @@ struct AttentionParams {
   uint32_t* status;
   uint32_t sequences, tokens, kv_heads, group, head_dim, page_size, capacity, box_shift, item_rows, item_cost;
   uint32_t causal, window, least_shift, whole_items;
+  uint32_t skewed;          // AttentionBarrier
   Divisor by_group, by_item_rows, by_page_size;
   float scale, scale_log2;  // of the scores; scale * log2(e)
 };

@@ -15,6 +15,10 @@ __device__ __forceinline__ uint32_t smem_address(const void* p) {
 __device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
+// A barrier of an attention kernel: one arrival too many when it is the one that is to run out.
+__device__ __forceinline__ void barrier_init(const AttentionParams& P, AttentionBarrier which, const uint64_t& bar, uint32_t count) {
+  barrier_init(smem_address(&bar), count + (P.skewed == which ? 1u : 0u));
+}
 __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }

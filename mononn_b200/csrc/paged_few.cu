@@ -94,15 +94,15 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
-      barrier_init(smem_address(&C.full[i]), 1);
-      barrier_init(smem_address(&C.empty[i]), kWarps);
+      barrier_init(P, kBarrierFull, C.full[i], 1);
+      barrier_init(P, kBarrierEmpty, C.empty[i], kWarps);
     }
     for (int i = 0; i < kPieces; ++i) {
-      barrier_init(smem_address(&C.told[i]), 1);
-      barrier_init(smem_address(&C.queries[i]), 32);
-      barrier_init(smem_address(&C.taken[i]), kWarps + 1);
+      barrier_init(P, kBarrierTold, C.told[i], 1);
+      barrier_init(P, kBarrierQueries, C.queries[i], 32);
+      barrier_init(P, kBarrierTaken, C.taken[i], kWarps + 1);
     }
-    barrier_init(smem_address(&C.meeting), kWarps);
+    barrier_init(P, kBarrierMeeting, C.meeting, kWarps);
     C.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));

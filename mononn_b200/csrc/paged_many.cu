@@ -309,24 +309,24 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < M::kPairs; ++i) {
-      barrier_init(smem_address(&C.full[i]), 2);
-      barrier_init(smem_address(&C.empty[i]), 1);
+      barrier_init(P, kBarrierFull, C.full[i], 2);
+      barrier_init(P, kBarrierEmpty, C.empty[i], 1);
     }
     for (int t = 0; t < 2; ++t) {
-      barrier_init(smem_address(&C.scores[t]), 1);
-      barrier_init(smem_address(&C.scores_read[t]), 4);
-      barrier_init(smem_address(&C.probabilities[t]), 4);
-      barrier_init(smem_address(&C.queries[t]), 1);
-      barrier_init(smem_address(&C.queries_free[t]), 1);
-      barrier_init(smem_address(&C.outputs[t]), 1);
+      barrier_init(P, kBarrierScores, C.scores[t], 1);
+      barrier_init(P, kBarrierScoresRead, C.scores_read[t], 4);
+      barrier_init(P, kBarrierProbabilities, C.probabilities[t], 4);
+      barrier_init(P, kBarrierQueries, C.queries[t], 1);
+      barrier_init(P, kBarrierQueriesFree, C.queries_free[t], 1);
+      barrier_init(P, kBarrierOutputs, C.outputs[t], 1);
     }
     for (int i = 0; i < kPieces; ++i) {
-      barrier_init(smem_address(&C.told[i]), 1);
-      barrier_init(smem_address(&C.taken[i]), 10);  // all but the warp that tells
+      barrier_init(P, kBarrierTold, C.told[i], 1);
+      barrier_init(P, kBarrierTaken, C.taken[i], 10);  // all but the warp that tells
     }
     barrier_init(smem_address(&C.drained), 1);
-    barrier_init(smem_address(&C.other_done), 4);
-    barrier_init(smem_address(&C.other_read), 4);
+    barrier_init(P, kBarrierOtherDone, C.other_done, 4);
+    barrier_init(P, kBarrierOtherRead, C.other_read, 4);
     C.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&P.k_map));

@@ -8,6 +8,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 from mononn_b200 import PagedCache, Rotary, paged_attention_status, rotary  # noqa: E402
+from mononn_b200.capi import MononnError, lib  # noqa: E402
 from tests.paged_reference import Problem, assert_rotated, rotary_rates, rotate, u  # noqa: E402
 
 F16, BF16 = torch.float16, torch.bfloat16
@@ -610,3 +611,27 @@ def test_workspaces_that_overlap_are_refused():
     with pytest.raises(ValueError, match="workspace overlaps out"):
         p.cache().attention_runner(p.q, p.indptr, out=out, workspace=room)
     assert torch.equal(p.cache().attention(p.q, p.indptr, workspace=room), (need(), need.out)[1])
+
+
+FEW_BARRIERS, MANY_BARRIERS = [1, 2, 3, 4, 5, 6], [1, 2, 3, 4, 5, 7, 9, 10, 11, 12, 13]
+
+
+@pytest.mark.parametrize("new, dim, barrier", [(1, 128, b) for b in FEW_BARRIERS] + [(1, 64, 1), (1, 64, 4)]
+                         + [(40, 128, b) for b in MANY_BARRIERS] + [(40, 64, b) for b in MANY_BARRIERS + [8]])
+def test_waits_that_run_out_are_reported(new, dim, barrier):
+    """An arrival that nobody makes: every CTA gives up after its bound, lets its copies land and returns; the status says
+    so once, rows of no sequence stay as they were, and the next call is right."""
+    news = [new] * 160
+    # one sequence so long that items are split, and the join runs over what is there
+    p = Problem(news, [new + 150 + i for i in range(159)] + [1300], 6, 2, dim, 16, BF16, seed=barrier, spare_rows=3)
+    paged_attention_status()
+    assert lib().mononn_debug_paged_skew(barrier) == 0
+    out = torch.full_like(p.q, 7.0)
+    cache = p.cache()
+    cache.attention(p.q, p.indptr, out=out, max_new=new)
+    with pytest.raises(MononnError) as e:
+        paged_attention_status()
+    assert e.value.code == -6
+    assert (out[p.starts[-1]:] == 7.0).all()
+    paged_attention_status()
+    p.check(*attend(p, max_new=new))

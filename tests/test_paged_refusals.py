@@ -574,3 +574,13 @@ def test_queries_in_place_behind_a_single_head(lib_built):
     for key, value, q in ((2, 1, 2), (0, 4, 2), (6, 0, 2)):
         with pytest.raises(ValueError, match="overlaps"):
             cache.append_runner(wide[:, key:key + 1], wide[:, value:value + 1], indptr, q=wide[:, q:q + 5], stream=OfHost)
+
+
+def test_waits_that_are_to_run_out_are_chosen_from_the_barriers(lib_built):
+    lib = capi.lib()
+    assert lib.mononn_debug_paged_skew(14) == -1
+    for barrier in range(14):
+        assert lib.mononn_debug_paged_skew(barrier) == 0
+    assert lib.mononn_debug_paged_skew(1) == 0
+    assert attend(args=attention_args(tokens=0)) == 0  # the next call, whatever it does, is the one that is meant
+    assert lib.mononn_debug_paged_skew(0) == 0
