@@ -344,7 +344,11 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
  * of a sequence sees and page rows behind a length may hold anything, NaN too; an infinity or NaN among the values
  * that some of a sequence's new tokens see may reach those of its new tokens that do not (its weight there is zero).
  * max_new: at most how many new tokens a sequence has, as a hint that chooses between the kernel for
- * few rows (single tokens, drafts) and the one for many; 0 = unknown. Results are right whatever it says.
+ * few rows (single tokens, drafts) and the one for many; 0 = unknown. Results are right whatever it says. The other
+ * thing that a launch is planned by is the table's width, max_pages, since lengths are on the device: in a table that is much
+ * wider than its sequences items are split although they are short, which costs a workspace and the launch that joins them
+ * (a table of 131072 keys: 1 to 4 us a call). A chunk of a prompt beside many sequences' single tokens takes less time
+ * as two calls.
  * The same arguments and contents give the same bits again. No gradients.
  * Limits: head_dim a multiple of 8 up to 128; page_size a multiple of 8; q_heads / kv_heads whole (up to 128 have
  * a kernel for many rows; above, every 16 rows read the keys again); addresses of pages, q and out, and all their

@@ -635,3 +635,16 @@ def test_waits_that_run_out_are_reported(new, dim, barrier):
     assert (out[p.starts[-1]:] == 7.0).all()
     paged_attention_status()
     p.check(*attend(p, max_new=new))
+
+
+@pytest.mark.parametrize("news, lens, kv_heads, group, dim, dtype, max_new", [
+    ([1], [300], 12, 1, 64, F16, 1), ([1] * 64, [250] * 64, 2, 4, 128, BF16, 1), ([500], [500], 2, 4, 128, BF16, 500),
+    ([16, 1, 0], [2000, 3, 0], 2, 4, 128, BF16, 16), ([1, 40], [129, 40], 2, 2, 80, F16, 0)])
+def test_short_sequences_in_a_table_of_a_whole_context(news, lens, kv_heads, group, dim, dtype, max_new):
+    """The width of the table decides whether items may be split and which kernel runs; the results are as right."""
+    p = Problem(news, lens, kv_heads, group, dim, 16, dtype, seed=dim)
+    p.check(*attend(p, max_new=max_new))
+    wide = torch.full((len(news), 8192), -1, dtype=torch.int32, device="cuda")
+    wide[:, :p.table.shape[1]] = p.table
+    p.table = wide
+    p.check(*attend(p, max_new=max_new))
