@@ -648,3 +648,18 @@ def test_short_sequences_in_a_table_of_a_whole_context(news, lens, kv_heads, gro
     wide[:, :p.table.shape[1]] = p.table
     p.table = wide
     p.check(*attend(p, max_new=max_new))
+
+
+def test_tokens_that_fall_on_one_place():
+    """Two sequences whose new tokens share a page: equal tokens are there whole, others element by element."""
+    p = Problem([1, 1, 3], [20, 20, 40], 2, 1, 64, 16, F16, seed=3)
+    p.table[1] = p.table[0]
+    k, v = (torch.randn(5, 2, 64, device="cuda").to(F16) for _ in range(2))
+    for same in (False, True):
+        if same:
+            k[1], v[1] = k[0], v[0]
+        p.cache().append(k, v, p.indptr)
+        for pages, new in ((p.k, k), (p.v, v)):
+            got = pages[p.table[0, 1].item(), 3]
+            assert ((got == new[0]) | (got == new[1])).all()
+            assert torch.equal(pages[p.table[2, 2].item(), 5:8], new[2:])
