@@ -339,7 +339,8 @@ int mononn_paged_append(const mononn_paged_cache* cache, const mononn_rotary* ro
 /* out[t, h, :] = sum_j p_j v_j,  p = softmax over the visible keys j of scale * q[t, h] . k_j,
  * where head h reads key head h / (q_heads / kv_heads). A token at position p sees the keys j <= p
  * (causal; otherwise all of its sequence), and with window > 0 (causal only) of those the ones with
- * j > p - window. A row that sees nothing becomes zeros (lse: minus infinity). lse: natural
+ * j > p - window. A row that sees nothing becomes zeros (lse: minus infinity), as one whose scores are all minus infinity;
+ * one whose scores, times scale and log2 e, leave 32 bits becomes NaN. lse: natural
  * logarithm of the sum of the exponentials, f32 [tokens, q_heads], or NULL. Keys that no row
  * of a sequence sees and page rows behind a length may hold anything, NaN too; an infinity or NaN among the values
  * that some of a sequence's new tokens see may reach those of its new tokens that do not (its weight there is zero).

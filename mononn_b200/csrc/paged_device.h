@@ -169,6 +169,15 @@ __device__ __forceinline__ void seen_keys(const AttentionParams& P, int32_t posi
   from = P.causal && P.window && position >= 0 && static_cast<uint32_t>(position) >= P.window
              ? position + 1 - static_cast<int32_t>(P.window) : 0;
 }
+// What a row's sum is divided by, as a factor: a row that saw nothing becomes zeros. A sum of 0 beside a score means that the
+// score left 32 bits when it was scaled: 1 / 0 makes NaN of it.
+__device__ __forceinline__ float inverse_of(float top, float sum) {
+  return sum == 0.f && top == __int_as_float(0xff800000) ? 0.f : 1.f / sum;
+}
+__device__ __forceinline__ float log_sum(float top, float sum, float scale) {
+  const float ninf = __int_as_float(0xff800000), nan = __int_as_float(0x7fffffff);
+  return sum == 0.f ? (top == ninf ? ninf : nan) : top * scale + logf(sum);
+}
 // Tiles of an item; one that sees no key has one all the same, in which its zeros are written.
 template <int KEYS>
 __device__ __forceinline__ uint32_t item_tiles(const KeyRange& r) {

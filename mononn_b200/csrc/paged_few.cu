@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
           const uint32_t of = divide(g, P.by_group);
           const int64_t token = piece.token + static_cast<int64_t>(of);
           const uint32_t head = piece.head * P.group + (g - of * P.group);
-          const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+          const float inverse = inverse_of(top, sum);
           if (d < P.head_dim) {
             uint4 v;
             v.x = Pair<T>::pack(o[0] * inverse, o[1] * inverse);
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreadsFew, 2) few_rows_kernel(const __grid_c
                                       static_cast<int64_t>(head) * P.out_head + d) = v;
           }
           if (d == 0 && P.lse)
-            P.lse[token * P.kv_heads * P.group + head] = sum == 0.f ? ninf : top * P.scale + logf(sum);
+            P.lse[token * P.kv_heads * P.group + head] = log_sum(top, sum, P.scale);
         } else {
           if (d == 0) {
             slot_out[row * 2] = top;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     const uint32_t of = divide(g, P.by_group);
     const int64_t token = static_cast<int64_t>(h.token) + of;
     const uint32_t head = h.head * P.group + (g - of * P.group);
-    const float inverse = total == 0.f ? 0.f : 1.f / total;
+    const float inverse = inverse_of(top, total);
     const uint32_t d = lane * kEach;
     if (d < P.head_dim) {
       uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<T*>(P.out) + token * P.out_token +
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
       for (int j = 0; j < kEach; j += 2) to[j / 2] = Pair<T>::pack(o[j] * inverse, o[j + 1] * inverse);
     }
     if (lane == 0 && P.lse)
-      P.lse[token * P.kv_heads * P.group + head] = total == 0.f ? ninf : top * P.scale + logf(total);
+      P.lse[token * P.kv_heads * P.group + head] = log_sum(top, total, P.scale);
   }
 }
 

@@ -763,12 +763,12 @@ __global__ void __launch_bounds__(kThreadsMany, 1) many_rows_kernel(const __grid
         const bool any = to > from, complete = piece.begins && piece.ends;
         const uint32_t token = divide(g, P.by_group), head = piece.head * P.group + (g - token * P.group);
         const int64_t row_of = piece.token + static_cast<int64_t>(token);
-        const float inverse = !complete ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float inverse = !complete ? 1.f : inverse_of(m, l);
         uint64_t row_at;  // where this thread's row goes
         if (complete) {
           row_at = reinterpret_cast<uint64_t>(static_cast<T*>(P.out) + row_of * P.out_token +
                                               static_cast<int64_t>(head) * P.out_head);
-          if (valid && P.lse) P.lse[row_of * P.kv_heads * P.group + head] = l == 0.f ? ninf : m * P.scale + logf(l);
+          if (valid && P.lse) P.lse[row_of * P.kv_heads * P.group + head] = log_sum(m, l, P.scale);
         } else {
           float* slot = P.partial + (2u * blockIdx.x + (piece.begins ? 1u : 0u)) * static_cast<size_t>(kRows * (2 + DIM));
           row_at = reinterpret_cast<uint64_t>(slot + kRows * 2 + r * DIM);

@@ -663,3 +663,28 @@ def test_tokens_that_fall_on_one_place():
             got = pages[p.table[0, 1].item(), 3]
             assert ((got == new[0]) | (got == new[1])).all()
             assert torch.equal(pages[p.table[2, 2].item(), 5:8], new[2:])
+
+
+@pytest.mark.parametrize("max_new", [1, MANY])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("keys", [200, 5000])
+def test_scores_that_leave_32_bits_become_nan(keys, dim, max_new):
+    """q.k is 2^126 and more, 32-bit, but not when it is scaled: never taken for a row that sees nothing. Rows beside them are
+    right, rows without a key are zeros."""
+    p = Problem([1, 40, 3], [keys, keys, 2], 1, 2, dim, 16, BF16, seed=dim)
+    p.q[0], p.q[11] = 2.0 ** 60, 2.0 ** 60
+    for b in (0, 1):
+        rows = p.table[b, : -(-keys // 16)].long()
+        p.k[rows] = 2.0 ** 60
+    p.q[1:11], p.q[12:41] = p.q[1:11] * 2.0 ** -60, p.q[12:41] * 2.0 ** -60
+    out, lse = attend(p, scale=4.0, max_new=max_new)
+    assert out[[0, 11]].isnan().all() and lse[[0, 11]].isnan().all()
+    assert (out[41] == 0).all() and (lse[41] == -math.inf).all()
+    keep = torch.ones(44, dtype=torch.bool, device="cuda")
+    keep[[0, 11]] = False
+    p.q[[0, 11]] = 0
+    want, log, limit, log_limit = p.want(scale=4.0)
+    off = (out.double() - want).abs()
+    assert (off <= limit)[keep].all()
+    keep[41] = False
+    assert ((lse.double() - log).abs() <= log_limit)[keep].all()
