@@ -108,6 +108,7 @@ def _stream(device, stream) -> C.c_void_p:
 
 def _runner(fn, args, keep, written):
     from torch.autograd.graph import increment_version
+    fn = lib()[fn.__name__]  # one of its own, without the conversions of arguments that are C objects already
 
     def run(_keep=keep):
         rc = fn(*args)
