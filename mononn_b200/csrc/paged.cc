@@ -274,20 +274,20 @@ int plan_attention(const mononn_paged_cache& c, const mononn_paged_attention_arg
   p->padded_dim = c.head_dim <= 64 ? 64 : 128;
   const uint32_t few = few_keys(p->padded_dim);
   const uint32_t whole_tokens = group <= kTileRows ? kTileRows / group * group : 0;  // rows of a row tile of the other
-  // More than 16 rows: the kernel for many, which takes 57 to 61 us whatever the rows for 16 sequences of 3350 keys
-  // (8 key heads of 128), where the one for few takes 44 us for 16 rows, 66 for 32 and 94 for 48 (keys read again). But
-  // calls that leave most of the GPU idle are done sooner by the one for few, which starts and ends faster and has
-  // twice the CTAs: up to an item for each of those and seven units in all (8 key heads, 64 rows: a sequence of
-  // 2000 keys 14.9 us instead of 16.7, four 25.1 instead of 19.9; eight of 500 keys 13.8 and 14.8, of 1000 27.6 and 21.6;
-  // 128 rows, eight of 250 keys: 16.0 and 11.5).
+  // More than 16 rows: the kernel for many, which takes 53, 55, 56, 57 and 62 us for 16, 32, 48, 64 and 128 rows of 16 sequences
+  // of 3350 keys (8 key heads of 128), where the one for few takes 46, 62, 114, 146 and 252 (keys read again). But
+  // calls that leave most of the GPU idle are done as soon or sooner by the one for few, which starts and ends faster and has
+  // twice the CTAs: up to an item for each of those and seven units in all (8 key heads, 64 rows, few and many: a sequence of
+  // 2000 keys 16.1 and 16.1 us, four 27.4 and 21.2; eight of 500 keys 14.5 and 14.9, of 1000 30.0 and 22.0;
+  // 128 rows, eight of 250 keys: 16.6 and 12.5).
   const uint64_t few_ctas = 2 * static_cast<uint64_t>(static_cast<unsigned>(sm_count));
   const uint64_t few_items =
       std::min<uint64_t>(c.sequences, a.tokens) * c.kv_heads * ((new_tokens * group + kFewRows - 1) / kFewRows);
   const bool idle = few_items <= few_ctas && few_items * tiles(few) <= 7 * few_ctas;
   p->many = whole_tokens && ((rows > kFewRows && !idle) || items(kFewRows) * (tiles(few) + 2) >= kMostUnits);
   // Where an item's rows fill no more than one row tile, that tile and the other take turns with the keys: 16 drafts of 3 to 8
-  // tokens over 700 to 6000 keys (8 x 5 heads of 128) 52 us instead of 56, 48 of 32 tokens over 2000 keys (8 x 4) 86 instead
-  // of 90, 16 of 128 over 8000 (12 heads of 64) 106 instead of 116. The code for it costs prompts 1 to 4 %, so it is another form.
+  // tokens over 700 to 6000 keys (8 x 5 heads of 128) 53 us instead of 58, 48 of 32 tokens over 2000 keys (8 x 4) 101 instead
+  // of 105, 16 of 128 over 8000 (12 heads of 64) 121 instead of 129. The code for it costs prompts 1 to 4 %, so it is another form.
   p->turns = p->many && new_tokens * group <= whole_tokens;
   p->rows = p->many ? kManyRows : kFewRows;
   p->item_rows = p->many ? 2 * whole_tokens : kFewRows;

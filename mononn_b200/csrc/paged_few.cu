@@ -6,8 +6,8 @@
 // heads: 16 KB) and keeps a maximum, a sum and an output of its own, which are added up when the item ends.
 // The keys are read once, and that bounds it: two loading warps keep 32 to 64 KB of each CTA on their way, two CTAs an SM. The
 // rows are far too few for the 128 of a tensor-memory product, and the 16-row instruction needs no round trip
-// through it. 32 sequences of 500 to 8000 keys, 8 key heads of 128: 558 MB in 90 us (0.94 of what a copy reaches; with the
-// join); 48 of 60 to 2000 keys, 32 heads of 64: 406 MB in 70 us; one of 150001 keys: 307 MB in 57 us; the rest are some 7 us
+// through it. 32 sequences of 500 to 8000 keys, 8 key heads of 128: 558 MB in 92 us (0.93 of what a copy reaches; with the
+// join); 48 of 60 to 2000 keys, 32 heads of 64: 406 MB in 70 us; one of 150001 keys: 307 MB in 56 us; the rest are some 7 us
 // at the begin and the end (launch, shares, first keys, join): a single sequence of 300 keys takes 6.9 us.
 #include "paged_device.h"
 

@@ -19,7 +19,7 @@
 // shorter by halving the units (next scores early, but products of 64 keys read 1.5 times as much shared memory: 228), by two
 // issuing warps (279), or by handing over the probabilities in halves (238); more exponentials by polynomial: 234. 64-wide
 // heads: exponentials and the 8 warps' other instructions, 0.55 of the special-function units' rate. Drafts: the keys, read at
-// 5.5 to 6 TB/s; 16 of 3 to 8 tokens over 700 to 6000 keys 52 us.
+// 5.5 to 6 TB/s once they are on their way; 16 of 3 to 8 tokens over 700 to 6000 keys 55 us.
 #include "paged_device.h"
 
 namespace mononn {
