@@ -320,9 +320,9 @@ typedef struct {
  * (q NULL: none; q_out may be q itself). positions: what is rotated by instead of the position in
  * the cache, or NULL. A token without a place (a negative position, a page number out of range) is not
  * written; its query is rotated all the same. Two tokens that fall on one place of a
- * shared page leave a mixture there, each element one of the two (so equal tokens may share it). k, v and q are not themselves in the pages, and no element is at once
- * in a written page of k_pages and in one of v_pages (within one page that is refused). Alignment as
- * mononn_rotary_apply. */
+ * shared page leave a mixture there, each element one of the two (so equal tokens may share it). k, v and q are
+ * not themselves in the pages, and no element is at once in a written page of k_pages and in one of v_pages
+ * (within one page that is refused). Alignment as mononn_rotary_apply. */
 typedef struct {
   const void *k, *v;
   int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;

@@ -6,8 +6,8 @@ Each operator comes as a function, and as a runner (`rotary_runner`, `PagedCache
 `PagedCache.attention_runner`): the arguments are checked and their addresses and sizes taken once, and
 the returned zero-argument callable does nothing but the library call (and tells autograd what was
 written), for serving loops that reuse their buffers (what page tables, lengths, indptr and positions
-hold is read on the device at each call).  A runner keeps its tensors alive; its stream is the one given, or torch's current stream of
-the tensors' device when it was made.
+hold is read on the device at each call).  A runner keeps its tensors alive; its stream is the one
+given, or torch's current stream of the tensors' device when it was made.
 """
 from __future__ import annotations
 
@@ -153,8 +153,8 @@ def _out_rows(name: str, out, src):
 
 
 def _same_grid(a, b) -> bool:
-    """Slices of one projection (other heads of the same rows, or others of the parts that a head has there): the
-    same strides, and never the same element."""
+    """Slices of one projection (other heads of the same rows, or other ones of the parts that each head has
+    there): the same strides, and never the same element."""
     if a.dim() != 3 or b.dim() != 3 or a.element_size() != b.element_size():
         return False
     low, high = sorted((a, b), key=lambda t: t.data_ptr())
@@ -326,7 +326,8 @@ class PagedCache:
             raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
         if _overlap(out, q) and not _same_grid(out, q):
             raise ValueError("out overlaps q")
-        read = dict(k_pages=self.k_pages, v_pages=self.v_pages, page_table=self.page_table, lengths=self.lengths, indptr=indptr)
+        read = dict(k_pages=self.k_pages, v_pages=self.v_pages, page_table=self.page_table, lengths=self.lengths,
+                    indptr=indptr)
         _apart(dict(out=out, lse=lse), read)
         _apart(dict(lse=lse), dict(q=q))
         a = capi.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
@@ -351,7 +352,8 @@ class PagedCache:
     def attention(self, q, indptr, out=None, lse=None, scale=None, causal=True, window=0, max_new=0, workspace=None,
                   stream=None):
         """Attention of the new tokens' queries q [tokens, q_heads, head_dim] over the cache, which holds
-        their own keys already. Rows indptr[b] .. indptr[b+1]-1 are the last positions of sequence b.
+        their own keys already. Rows indptr[b] .. indptr[b+1]-1 are the last positions of sequence b; rows of no
+        sequence stay as they were in `out` (undefined in one that is made here).
         causal: keys up to the own position; window > 0: the last `window` of those. scale: 1 / sqrt(head_dim)
         unless given. max_new: at most how many new tokens a sequence has, when known (it chooses the
         kernel). lse: float32 [tokens, q_heads] for the logarithm of the sum of exponentials. The
