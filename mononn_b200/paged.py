@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import dataclasses
+import functools
 
 from . import capi
 from .capi import check, lib
@@ -55,17 +56,23 @@ def _dtype(t) -> int:
     return int(t.dtype == torch.bfloat16)
 
 
-def _no_gradient(name: str, t) -> None:
+@functools.cache
+def _autograd():
     import torch
-    if t.requires_grad and torch.is_grad_enabled():
+    return torch.is_grad_enabled, torch.autograd.forward_ad.unpack_dual
+
+
+def _no_gradient(name: str, t) -> None:
+    is_grad_enabled, unpack_dual = _autograd()
+    if t.requires_grad and is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which is not computed here: detach it or use torch.no_grad()")
-    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+    if unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} carries a forward gradient, which is not computed here")
 
 
 def _sizes(name: str, t) -> None:
     """The library counts in 32 bits; ctypes would drop the higher ones."""
-    if max(t.shape) >= 2**32:
+    if t.numel() >= 2**32 and max(t.shape) >= 2**32:
         raise ValueError(f"{name} has a size of 2^32 or more: {list(t.shape)}")
 
 
@@ -118,29 +125,28 @@ def _runner(fn, args, keep, written):
     return run
 
 
-def _span(t):
-    """Addresses from the first element to behind the last; None without elements."""
-    if t.numel() == 0:
-        return None
-    n = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) + 1
-    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+def _span(t) -> tuple[int, int]:
+    """Addresses from the first element to behind the last; (0, 0) without elements, which overlaps nothing."""
+    last = 0
+    for n, stride in zip(t.shape, t.stride()):
+        if n == 0:
+            return 0, 0
+        last += (n - 1) * stride
+    at = t.data_ptr()
+    return at, at + (last + 1) * t.element_size()
 
 
 def _overlap(a, b) -> bool:
     a, b = _span(a), _span(b)
-    return a is not None and b is not None and a[0] < b[1] and b[0] < a[1]
+    return a[0] < b[1] and b[0] < a[1]
 
 
-def _apart(written: dict, read: dict) -> None:
-    """Nothing that a call writes is read by it, or written twice."""
-    spans = [(name, _span(t)) for name, t in (*written.items(), *read.items()) if t is not None]
-    spans = [(name, s) for name, s in spans if s is not None]
-    for i, (name, a) in enumerate(spans):
-        if name not in written:
-            break
-        for other, b in spans[i + 1:]:
-            if a[0] < b[1] and b[0] < a[1]:
-                raise ValueError(f"{name} overlaps {other}")
+def _apart(name: str, span, read) -> None:
+    """What a call writes at `span` is none of what it reads, or writes otherwise: pairs of a name and a span."""
+    begin, end = span
+    for other, (low, high) in read:
+        if begin < high and low < end:
+            raise ValueError(f"{name} overlaps {other}")
 
 
 def _out_rows(name: str, out, src):
@@ -189,7 +195,7 @@ def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):
     _rows("out", out, x, x.shape[1], x.shape[0])
     _out_rows("out", out, x)
     _ints("positions", positions, x, (x.shape[0],))
-    _apart(dict(out=out), dict(positions=positions))
+    _apart("out", _span(out), [("positions", _span(positions))])
     a = capi.RotaryArgs(x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1),
                         positions.data_ptr(), x.shape[0], x.shape[1], x.shape[2], _dtype(x))
     table = rotary.table()
@@ -232,6 +238,7 @@ class PagedCache:
         _ints("page_table", page_table, k_pages, (n, most))
         _ints("lengths", lengths, k_pages, (n,))
         self._tensors = k_pages, v_pages, page_table, lengths
+        self._spans = [(name, _span(t)) for name, t in zip(("k_pages", "v_pages", "page_table", "lengths"), self._tensors)]
         pages, size, heads, dim = k_pages.shape
         ps, ts, hs, _ = k_pages.stride()
         self._args = capi.PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, hs, page_table.data_ptr(),
@@ -273,10 +280,17 @@ class PagedCache:
             for name, t in (("k", k), ("v", v)):
                 if _overlap(q_out, t) and not _same_grid(q_out, t):
                     raise ValueError(f"q_out overlaps {name}")
-        tables = dict(page_table=self.page_table, lengths=self.lengths, indptr=indptr, positions=positions)
-        _apart(dict(q_out=q_out), dict(k_pages=self.k_pages, v_pages=self.v_pages, **tables))
-        for name, pages in (("k_pages", self.k_pages), ("v_pages", self.v_pages)):
-            _apart({name: pages}, dict(k=k, v=v, q=q, **tables))
+        given = [("indptr", _span(indptr))]
+        if positions is not None:
+            given.append(("positions", _span(positions)))
+        if q is not None:
+            at = _span(q_out)
+            _apart("q_out", at, self._spans)
+            _apart("q_out", at, given)
+            given.append(("q", at if q_out is q else _span(q)))
+        given += [("k", _span(k)), ("v", _span(v)), *self._spans[2:]]
+        for name, at in self._spans[:2]:
+            _apart(name, at, given)
         qs, os = (q.stride(), q_out.stride()) if q is not None else ((0, 0), (0, 0))
         a = capi.PagedAppendArgs(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
                                  q.data_ptr() if q is not None else None,
@@ -326,10 +340,11 @@ class PagedCache:
             raise ValueError("window and max_new must be in 0 .. 2^32 - 1")
         if _overlap(out, q) and not _same_grid(out, q):
             raise ValueError("out overlaps q")
-        read = dict(k_pages=self.k_pages, v_pages=self.v_pages, page_table=self.page_table, lengths=self.lengths,
-                    indptr=indptr)
-        _apart(dict(out=out, lse=lse), read)
-        _apart(dict(lse=lse), dict(q=q))
+        taken = [*self._spans, ("indptr", _span(indptr))]
+        if lse is not None:
+            taken.append(("lse", _span(lse)))
+            _apart("lse", taken[-1][1], [*taken[:-1], ("q", _span(q))])
+        _apart("out", _span(out), taken)
         a = capi.PagedAttentionArgs(q.data_ptr(), out.data_ptr(), lse.data_ptr() if lse is not None else None,
                                     q.stride(0), q.stride(1), out.stride(0), out.stride(1), indptr.data_ptr(),
                                     q.shape[0], q.shape[1], 0.0 if scale is None else scale, int(causal), window,
@@ -341,7 +356,7 @@ class PagedCache:
                 workspace = made_here(need.value, dtype=torch.uint8)
             if workspace.device != q.device or not workspace.is_contiguous():
                 raise ValueError(f"workspace must be contiguous on {q.device}")
-            _apart(dict(workspace=workspace), dict(q=q, out=out, lse=lse, **read))
+            _apart("workspace", _span(workspace), [*taken, ("q", _span(q)), ("out", _span(out))])
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
         run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a),
