@@ -113,9 +113,15 @@ def _stream(device, stream) -> C.c_void_p:
     return C.c_void_p(s.cuda_stream)
 
 
-def _runner(fn, args, keep, written):
+@functools.cache
+def _entry(name: str):
+    """An entry point without the conversions of arguments, which are C objects already."""
     from torch.autograd.graph import increment_version
-    fn = lib()[fn.__name__]  # one of its own, without the conversions of arguments that are C objects already
+    return lib()[name], increment_version
+
+
+def _runner(name: str, args, keep, written):
+    fn, increment_version = _entry(name)
 
     def run(_keep=keep):
         rc = fn(*args)
@@ -200,7 +206,7 @@ def rotary_runner(x, positions, rotary: Rotary, out=None, stream=None):
                         positions.data_ptr(), x.shape[0], x.shape[1], x.shape[2], _dtype(x))
     table = rotary.table()
     args = (C.byref(table), C.byref(a), _stream(x.device, stream))
-    return _runner(lib().mononn_rotary_apply, args, (x, out, positions, table, a), (out,))
+    return _runner("mononn_rotary_apply", args, (x, out, positions, table, a), (out,))
 
 
 def rotary(x, positions, rotary: Rotary, out=None, stream=None):
@@ -300,7 +306,7 @@ class PagedCache:
         table = rotary.table() if rotary is not None else None
         args = (C.byref(self._args), C.byref(table) if table is not None else None, C.byref(a),
                 _stream(k.device, stream))
-        return _runner(lib().mononn_paged_append, args, (self, k, v, q, q_out, indptr, positions, table, a),
+        return _runner("mononn_paged_append", args, (self, k, v, q, q_out, indptr, positions, table, a),
                        (self.k_pages, self.v_pages) + ((q_out,) if q is not None else ()))
 
     def append(self, k, v, indptr, rotary: Rotary | None = None, positions=None, q=None, q_out=None, stream=None):
@@ -359,7 +365,7 @@ class PagedCache:
             _apart("workspace", _span(workspace), [*taken, ("q", _span(q)), ("out", _span(out))])
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
         args = (C.byref(self._args), C.byref(a), _stream(q.device, stream))
-        run = _runner(lib().mononn_paged_attention, args, (self, q, out, lse, indptr, workspace, a),
+        run = _runner("mononn_paged_attention", args, (self, q, out, lse, indptr, workspace, a),
                       (out,) + ((lse,) if lse is not None else ()))
         run.out = out
         return run
